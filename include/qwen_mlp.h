@@ -19,6 +19,11 @@
  *   QMLP_FMT_BF4   bf4 block float: the same 16-value groups with 1 sign + 3 magnitude bits
  *                  (0.5625 B/value).  In qmlp_forward it names the reference's mixed layout
  *                  (mlp.py:17-19,164-169): gate_proj and up_proj packed bf4, down_proj packed bfp8.
+ *   QMLP_FMT_MXFP4 microscaled 4-bit floating point (OCP MX): 32 consecutive K values share one
+ *                  power-of-two scale byte, each value is one of 0, .5, 1, 1.5, 2, 3, 4, 6 with a
+ *                  sign (0.53125 B/value).  The activations are quantised to the same format in
+ *                  every call, so both operands go to the scaled matrix-core products as they are
+ *                  (fp32 accumulation); h, between the projections, is quantised once from fp32.
  * Weights are used in the library's packed ("tiled") layout, produced once by qmlp_pack().
  * Matrices are row-major [out_features, in_features] like the HF checkpoint tensors
  * gate_proj.weight [I,H], up_proj.weight [I,H], down_proj.weight [H,I].
@@ -47,6 +52,7 @@ typedef struct ihipStream_t* qmlp_stream_t; /* == hipStream_t */
 #define QMLP_FMT_BF16 0
 #define QMLP_FMT_BFP8 1
 #define QMLP_FMT_BF4 2
+#define QMLP_FMT_MXFP4 4
 
 /* Message for the last failing call on this host thread ("" if none).  Host only. */
 const char* qmlp_last_error(void);
@@ -75,13 +81,17 @@ int qmlp_quantize_bfp8(const void* w_bf16, int rows, int cols, void* q, void* e8
 int qmlp_quantize_bf4(const void* w_bf16, int rows, int cols, void* q, void* e8,
                       uint32_t* bad_groups, qmlp_stream_t stream);
 
-/* Bytes of the packed device buffer for one [rows, cols] matrix (host only, no GPU needed). */
+/* Bytes of the packed device buffer for one [rows, cols] matrix (host only, no GPU needed): rows a
+ * multiple of 16 and cols of 256; QMLP_FMT_MXFP4: any rows, cols a multiple of 32. */
 size_t qmlp_packed_bytes(int rows, int cols, int fmt);
 
 /* Pack one matrix into the library's tiled layout.
  *   fmt == QMLP_FMT_BFP8 or QMLP_FMT_BF4: src0 = q (int8 [rows,cols]), src1 = e8 (uint8
  *   [rows,cols/16]) from the matching quantiser.
  *   fmt == QMLP_FMT_BF16: src0 = bf16 [rows,cols], src1 unused (may be null).
+ *   fmt == QMLP_FMT_MXFP4: src0 = codes (uint8 [rows,cols/2], the even K in the low half of a byte),
+ *   src1 = scales (uint8 [rows,cols/32], 2^(s-127)), as microscaled checkpoints hold them; the
+ *   trailer counts the scales of 255 (not a number) as groups with non-finite values.
  * packed must hold qmlp_packed_bytes(rows, cols, fmt) bytes.  The trailer of the packed buffer
  * records the largest row L2 norm and the number of bfp8 groups too small to keep (see
  * qmlp_packed_info); a nonzero count means the packed matrix is not lossless.
@@ -90,14 +100,16 @@ int qmlp_pack(const void* src0, const void* src1, int rows, int cols, int fmt, v
               size_t packed_bytes, qmlp_stream_t stream);
 
 /* Reads the packed trailer back to host memory: largest row L2 norm (of the dequantised rows)
- * and count of flushed bfp8 groups.  Synchronises `stream`.  Load-time only. */
+ * and count of flushed bfp8 groups (QMLP_FMT_MXFP4: both 0, its kernels need no bound and keep every
+ * group).  Synchronises `stream`.  Load-time only. */
 int qmlp_packed_info(const void* packed, int rows, int cols, int fmt, double* max_row_norm,
                      uint32_t* flushed_groups, qmlp_stream_t stream);
 
 /* qmlp_quantize_bfp8 / _bf4 and qmlp_pack in one pass: bf16 [rows,cols] -> the same packed bytes in
  * any format, without the canonical intermediates.  qmlp_quantize_pack_info reads the trailer back
  * like qmlp_packed_info and also the number of groups that hold a non-finite value (packed as
- * zeros; a matrix with such groups must not be used; always 0 for QMLP_FMT_BF16). */
+ * zeros, with QMLP_FMT_MXFP4 as NaN; a matrix with such groups must not be used; always 0 for
+ * QMLP_FMT_BF16). */
 int qmlp_quantize_pack(const void* w_bf16, int rows, int cols, int fmt, void* packed,
                        size_t packed_bytes, qmlp_stream_t stream);
 int qmlp_quantize_pack_info(const void* packed, int rows, int cols, int fmt, double* max_row_norm,
@@ -112,6 +124,10 @@ int qmlp_unpack_bfp8(const void* packed, int rows, int cols, void* q, void* e8,
 /* Inverse of qmlp_pack for bf4 (same contract as qmlp_unpack_bfp8). */
 int qmlp_unpack_bf4(const void* packed, int rows, int cols, void* q, void* e8,
                     qmlp_stream_t stream);
+
+/* Inverse of qmlp_pack for MXFP4: packed -> codes and scales (lossless). */
+int qmlp_unpack_mxfp4(const void* packed, int rows, int cols, void* codes, void* scales,
+                      qmlp_stream_t stream);
 
 /* Dequantises a packed matrix to fp32 [rows, cols] with the same in-register routine the GEMM
  * kernels use.  Diagnostic/audit use. */
@@ -167,6 +183,53 @@ int qmlp_forward_ex(const void* x, const void* wg, const void* wu, const void* w
 int qmlp_forward_rmsnorm(const void* h, const void* norm_w, float eps, const void* wg, const void* wu,
                          const void* wd, void* out, void* ws, size_t ws_bytes, int M, int H, int I,
                          int fmt, int flags, qmlp_stream_t stream);
+
+/* ---------------------------------------------------------------- MXFP4 operators
+ *
+ * The pieces of the QMLP_FMT_MXFP4 forward as calls of their own, for any sizes: rows M (or N) from
+ * 1, K a multiple of 32.  A packed activation matrix has the weights' packed layout
+ * (qmlp_packed_bytes(M, K, QMLP_FMT_MXFP4) bytes, without a trailer) and feeds any number of products.
+ *
+ * The quantisation of a block: its scale is the binade of its largest magnitude less 2, at least
+ * 2^-126, so that the largest value lands in [4, 8); values are rounded half to even and saturate at
+ * 6.  A block with an infinity or a NaN becomes NaN as a whole (scale byte 255), and so does every
+ * output of its row. */
+#define QMLP_X_BF16 0
+#define QMLP_X_F16 1
+#define QMLP_X_F32 2
+#define QMLP_X_MXFP4 3 /* already packed: x_stride is not used */
+#define QMLP_OUT_MXFP4 4 /* flag of qmlp_mx_swiglu: out is a packed activation matrix [M, N] */
+
+/* x [rows, cols] (x_type BF16, F16 or F32; x_stride elements from row to row, a multiple of 16 bytes)
+ * -> packed activation matrix.  Only the given rows are written. */
+int qmlp_mx_quantize(const void* x, int x_type, int64_t x_stride, int rows, int cols, void* packed,
+                     size_t packed_bytes, qmlp_stream_t stream);
+
+/* The same behind the decoder's zero-centred RMSNorm: n = bf16(h / sqrt(mean(h^2) + eps) * (1 + norm_w)),
+ * h bf16 (layer.py:110-112,352-353). */
+int qmlp_mx_quantize_rmsnorm(const void* h, int64_t h_stride, const void* norm_w, float eps, int rows,
+                             int cols, void* packed, size_t packed_bytes, qmlp_stream_t stream);
+
+/* Packed matrix -> bf16 (out_type QMLP_X_BF16) or fp32 (QMLP_X_F32) [rows, cols], exactly. */
+int qmlp_mx_dequantize(const void* packed, int rows, int cols, void* out, int out_type,
+                       qmlp_stream_t stream);
+
+/* out[M, N] = x W^T (+ residual): x of any x_type, quantised in the call unless it is QMLP_X_MXFP4; w
+ * packed [N, K].  flags: QMLP_OUT_F32, QMLP_RESIDUAL_F32.  out may be the residual itself (of the same
+ * dtype) and must not overlap anything else.  ws: qmlp_mx_workspace_bytes(M, N, K) bytes that may hold
+ * anything (nothing to initialise); calls that overlap need separate ones. */
+int qmlp_mx_linear(const void* x, int x_type, int64_t x_stride, const void* w, const void* residual,
+                   void* out, void* ws, size_t ws_bytes, int M, int N, int K, int flags,
+                   qmlp_stream_t stream);
+
+/* out[M, N] = silu(x Wg^T) * (x Wu^T), the gate/up pair of the block (FusedProjection,
+ * scripts/ci/fused_1d.py:123-196).  flags: QMLP_OUT_F32 or QMLP_OUT_MXFP4 (N a multiple of 256; quantised
+ * from the fp32 values). */
+int qmlp_mx_swiglu(const void* x, int x_type, int64_t x_stride, const void* wg, const void* wu, void* out,
+                   void* ws, size_t ws_bytes, int M, int N, int K, int flags, qmlp_stream_t stream);
+
+/* Workspace bytes of the two products (host only); never shrinks as M grows.  0: sizes out of range. */
+size_t qmlp_mx_workspace_bytes(int M, int N, int K);
 
 /* Workspace bytes needed by qmlp_forward for these sizes (host only, no GPU needed).  The size
  * never decreases as M grows, so a workspace sized for M serves every call with fewer tokens, and

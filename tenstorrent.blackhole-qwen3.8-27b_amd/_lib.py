@@ -14,11 +14,14 @@ LIB_PATH = os.path.join(PKG_DIR, "libqwen_mlp.so")
 FMT_BF16 = 0
 FMT_BFP8 = 1
 FMT_BF4 = 2
-FORMATS = {"bf16": FMT_BF16, "bfp8": FMT_BFP8, "bf4": FMT_BF4}
+FMT_MXFP4 = 4
+FORMATS = {"bf16": FMT_BF16, "bfp8": FMT_BFP8, "bf4": FMT_BF4, "mxfp4": FMT_MXFP4}
 
 QMLP_OK = 0
 OUT_F32 = 1
 RESIDUAL_F32 = 2
+OUT_MXFP4 = 4
+X_BF16, X_F16, X_F32, X_MXFP4 = 0, 1, 2, 3  # QMLP_X_*
 WS_COUNTER_BYTES = 524288  # QMLP_WS_COUNTER_BYTES
 SCRATCH_BYTES = 33554432  # QMLP_SCRATCH_BYTES
 E_SHAPE, E_ALIGN, E_FORMAT, E_LAUNCH, E_WORKSPACE, E_NULL, E_DEVICE = -1, -2, -3, -4, -5, -6, -7
@@ -26,6 +29,7 @@ _VALUE_ERRORS = {E_SHAPE, E_ALIGN, E_FORMAT, E_WORKSPACE, E_NULL}
 
 # name -> (restype, argtypes); mirrors include/qwen_mlp.h
 _P, _I, _SZ, _U32P, _DP = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_void_p
+_L = ctypes.c_int64
 SIGNATURES = {
     "qmlp_last_error": (ctypes.c_char_p, []),
     "qmlp_version": (ctypes.c_char_p, []),
@@ -50,6 +54,13 @@ SIGNATURES = {
     "qmlp_plan_split": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(ctypes.c_int)]),
     "qmlp_forward_rmsnorm": (_I, [_P, _P, ctypes.c_float, _P, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _I, _P]),
     "qmlp_forward_noalloc": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
+    "qmlp_unpack_mxfp4": (_I, [_P, _I, _I, _P, _P, _P]),
+    "qmlp_mx_quantize": (_I, [_P, _I, _L, _I, _I, _P, _SZ, _P]),
+    "qmlp_mx_quantize_rmsnorm": (_I, [_P, _L, _P, ctypes.c_float, _I, _I, _P, _SZ, _P]),
+    "qmlp_mx_dequantize": (_I, [_P, _I, _I, _P, _I, _P]),
+    "qmlp_mx_linear": (_I, [_P, _I, _L, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _P]),
+    "qmlp_mx_swiglu": (_I, [_P, _I, _L, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _P]),
+    "qmlp_mx_workspace_bytes": (_SZ, [_I, _I, _I]),
 }
 
 _lib = None
@@ -121,6 +132,32 @@ def ptr(t):
 
 def stream_handle(stream=None):
     return ctypes.c_void_p(raw_stream() if stream is None else stream.cuda_stream)
+
+
+class on_device:
+    """Makes ``device`` (a GPU) current for a call, and ``stream`` (if one is given) the stream that
+    tensors are allocated on, so that the caching allocator orders their memory with that stream's
+    work.  Does nothing where the device is current already and no stream is given."""
+
+    def __init__(self, device, stream=None):
+        import torch
+
+        if stream is not None and stream.device != device:
+            raise ValueError(f"stream is on {stream.device}, the tensors are on {device}")
+        if stream is not None:
+            self._inner = torch.cuda.stream(stream)  # makes the stream's device current too
+        elif device.index is not None and device.index != torch.cuda.current_device():
+            self._inner = torch.cuda.device(device)
+        else:
+            self._inner = None
+
+    def __enter__(self):
+        if self._inner is not None:
+            self._inner.__enter__()
+
+    def __exit__(self, *exc):
+        if self._inner is not None:
+            self._inner.__exit__(*exc)
 
 
 def raw_stream(index=None):

@@ -10,6 +10,7 @@
 #include "../../include/qwen_mlp.h"
 #include "qmlp_common.h"
 #include "qmlp_internal.h"
+#include "qmlp_mx.h"
 
 namespace qmlp {
 
@@ -44,8 +45,6 @@ bool profile_events(int slot, hipEvent_t* start, hipEvent_t* stop) {
   *stop = g_prof[2 * slot + 1];
   return true;
 }
-
-static size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 WsLayout ws_layout(int M, int H, int I, int fmt) {
   WsLayout L{};
@@ -96,11 +95,6 @@ WsLayout ws_layout(int M, int H, int I, int fmt) {
   return L;
 }
 
-struct DeviceInfo {
-  int ok;  // 1 = gfx950, -1 = unusable
-  int num_cus;
-};
-
 static DeviceInfo device_info(int dev) {
   static std::mutex mu;
   static DeviceInfo cache[64] = {};
@@ -118,7 +112,7 @@ static DeviceInfo device_info(int dev) {
   return cache[dev];
 }
 
-static int current_device_info(DeviceInfo* out) {
+int current_device_info(DeviceInfo* out) {
   int dev = -1;
   if (hipGetDevice(&dev) != hipSuccess) return set_error(QMLP_E_DEVICE, "no HIP device");
   *out = device_info(dev);
@@ -126,14 +120,28 @@ static int current_device_info(DeviceInfo* out) {
   return 0;
 }
 
-static bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
-
-static bool known_fmt(int fmt) { return fmt == QMLP_FMT_BF16 || fmt == QMLP_FMT_BFP8 || fmt == QMLP_FMT_BF4; }
+// The formats of the 16-row tile layout; MXFP4 has a layout of its own.
+static bool tile_fmt(int fmt) { return fmt == QMLP_FMT_BF16 || fmt == QMLP_FMT_BFP8 || fmt == QMLP_FMT_BF4; }
+static bool known_fmt(int fmt) { return tile_fmt(fmt) || fmt == QMLP_FMT_MXFP4; }
 
 static bool shape_ok(int rows, int cols) {
   return rows > 0 && cols > 0 && rows % kTileRows == 0 && cols % kSuperK == 0 && rows <= kMaxDim &&
          cols <= kMaxDim;
 }
+
+// Matrices that can be packed, and their packed size.
+static bool packable(int rows, int cols, int fmt) {
+  return fmt == QMLP_FMT_MXFP4 ? mx_shape_ok(rows, cols) : shape_ok(rows, cols);
+}
+static int set_shape_error(const char* fn, int rows, int cols, int fmt) {
+  if (fmt == QMLP_FMT_MXFP4)
+    return set_error(QMLP_E_SHAPE, "%s: cols must be a multiple of 32 (%dx%d)", fn, rows, cols);
+  return set_error(QMLP_E_SHAPE, "%s: rows must be a multiple of 16 and cols of 256 (%dx%d)", fn, rows, cols);
+}
+static size_t packed_trailer(int rows, int cols, int fmt) {
+  return fmt == QMLP_FMT_MXFP4 ? mx_units_bytes(rows, cols) : trailer_offset(rows, cols, fmt);
+}
+static size_t packed_size(int rows, int cols, int fmt) { return packed_trailer(rows, cols, fmt) + kTrailer; }
 
 // Shared validation and dispatch of the forward entry points.
 int forward_impl(const char* fn, const void* x, const void* wg, const void* wu, const void* wd, const void* residual,
@@ -165,11 +173,14 @@ int forward_impl(const char* fn, const void* x, const void* wg, const void* wu, 
   }
   if (residual == out && residual && ((flags & QMLP_OUT_F32) != 0) != ((flags & QMLP_RESIDUAL_F32) != 0))
     return set_error(QMLP_E_SHAPE, "%s: an in-place residual needs the same dtype as out", fn);
-  const WsLayout L = ws_layout(M, H, I, fmt);
-  if (ws_bytes < L.total)
-    return set_error(QMLP_E_WORKSPACE, "%s: workspace holds %zu bytes, needs %zu", fn, ws_bytes, L.total);
+  const size_t need = qmlp_workspace_bytes(M, H, I, fmt);
+  if (ws_bytes < need)
+    return set_error(QMLP_E_WORKSPACE, "%s: workspace holds %zu bytes, needs %zu", fn, ws_bytes, need);
   DeviceInfo di;
   if (int rc = current_device_info(&di)) return rc;
+  if (fmt == QMLP_FMT_MXFP4)
+    return mx_forward(x, wg, wu, wd, residual, out, ws, M, H, I, flags, normw, eps, di.num_cus, stream);
+  const WsLayout L = ws_layout(M, H, I, fmt);
   ForwardArgs a{x, (const uint8_t*)wg, (const uint8_t*)wu, (const uint8_t*)wd, residual, out, (uint8_t*)ws,
                 M, H, I, fmt, (flags & QMLP_OUT_F32) ? 1 : 0, (flags & QMLP_RESIDUAL_F32) ? 1 : 0, normw, eps, false};
   // M <= 32: split-K weight streaming with LDS-staged activations; where no such split fits (a K
@@ -211,8 +222,8 @@ const char* qmlp_last_error(void) { return g_err; }
 const char* qmlp_version(void) { return "qwen_mlp 0.3 gfx950 src=" QMLP_SOURCE_HASH; }
 
 size_t qmlp_packed_bytes(int rows, int cols, int fmt) {
-  if (!shape_ok(rows, cols) || !known_fmt(fmt)) return 0;
-  return packed_total(rows, cols, fmt);
+  if (!known_fmt(fmt) || !packable(rows, cols, fmt)) return 0;
+  return packed_size(rows, cols, fmt);
 }
 
 static int quantize_impl(const char* fn, const void* w_bf16, int rows, int cols, void* q, void* e8,
@@ -239,14 +250,14 @@ int qmlp_pack(const void* src0, const void* src1, int rows, int cols, int fmt, v
               qmlp_stream_t stream) {
   if (!known_fmt(fmt)) return set_error(QMLP_E_FORMAT, "qmlp_pack: unknown format %d", fmt);
   if (!src0 || !packed || (fmt != QMLP_FMT_BF16 && !src1)) return set_error(QMLP_E_NULL, "qmlp_pack: null pointer");
-  if (!shape_ok(rows, cols))
-    return set_error(QMLP_E_SHAPE, "qmlp_pack: rows must be a multiple of 16 and cols of 256 (%dx%d)", rows, cols);
+  if (!packable(rows, cols, fmt)) return set_shape_error("qmlp_pack", rows, cols, fmt);
   if (!aligned16(src0) || !aligned16(packed)) return set_error(QMLP_E_ALIGN, "qmlp_pack: misaligned pointer");
-  if (packed_bytes < packed_total(rows, cols, fmt))
+  if (packed_bytes < packed_size(rows, cols, fmt))
     return set_error(QMLP_E_WORKSPACE, "qmlp_pack: packed buffer holds %zu bytes, needs %zu", packed_bytes,
-                     packed_total(rows, cols, fmt));
+                     packed_size(rows, cols, fmt));
   DeviceInfo di;
   if (int rc = current_device_info(&di)) return rc;
+  if (fmt == QMLP_FMT_MXFP4) return launch_mx_pack(src0, src1, rows, cols, packed, (hipStream_t)stream);
   return launch_pack(src0, src1, rows, cols, fmt, packed, (hipStream_t)stream);
 }
 
@@ -255,25 +266,25 @@ int qmlp_quantize_pack(const void* w_bf16, int rows, int cols, int fmt, void* pa
   const char* fn = "qmlp_quantize_pack";
   if (!known_fmt(fmt)) return set_error(QMLP_E_FORMAT, "%s: unknown format %d", fn, fmt);
   if (!w_bf16 || !packed) return set_error(QMLP_E_NULL, "%s: null pointer", fn);
-  if (!shape_ok(rows, cols))
-    return set_error(QMLP_E_SHAPE, "%s: rows must be a multiple of 16 and cols of 256 (%dx%d)", fn, rows, cols);
+  if (!packable(rows, cols, fmt)) return set_shape_error(fn, rows, cols, fmt);
   if (!aligned16(w_bf16) || !aligned16(packed)) return set_error(QMLP_E_ALIGN, "%s: misaligned pointer", fn);
-  if (packed_bytes < packed_total(rows, cols, fmt))
+  if (packed_bytes < packed_size(rows, cols, fmt))
     return set_error(QMLP_E_WORKSPACE, "%s: packed buffer holds %zu bytes, needs %zu", fn, packed_bytes,
-                     packed_total(rows, cols, fmt));
+                     packed_size(rows, cols, fmt));
   DeviceInfo di;
   if (int rc = current_device_info(&di)) return rc;
+  if (fmt == QMLP_FMT_MXFP4) return launch_mx_quantize_pack(w_bf16, rows, cols, packed, (hipStream_t)stream);
   return launch_quantize_pack(w_bf16, rows, cols, fmt, packed, (hipStream_t)stream);
 }
 
 static int info_impl(const char* fn, const void* packed, int rows, int cols, int fmt, double* max_row_norm,
                      uint32_t* flushed_groups, uint32_t* bad_groups, qmlp_stream_t stream) {
   if (!packed) return set_error(QMLP_E_NULL, "%s: null pointer", fn);
-  if (!shape_ok(rows, cols) || !known_fmt(fmt)) return set_error(QMLP_E_SHAPE, "%s: bad shape/format", fn);
+  if (!known_fmt(fmt) || !packable(rows, cols, fmt)) return set_error(QMLP_E_SHAPE, "%s: bad shape/format", fn);
   DeviceInfo di;
   if (int rc = current_device_info(&di)) return rc;
   PackTrailer t;
-  const uint8_t* src = (const uint8_t*)packed + trailer_offset(rows, cols, fmt);
+  const uint8_t* src = (const uint8_t*)packed + packed_trailer(rows, cols, fmt);
   if (hipMemcpyAsync(&t, src, sizeof(t), hipMemcpyDeviceToHost, (hipStream_t)stream) != hipSuccess ||
       hipStreamSynchronize((hipStream_t)stream) != hipSuccess)
     return set_error(QMLP_E_LAUNCH, "%s: copy failed", fn);
@@ -300,10 +311,11 @@ int qmlp_quantize_pack_info(const void* packed, int rows, int cols, int fmt, dou
 static int unpack_impl(const char* fn, const void* packed, int rows, int cols, int fmt, void* q, void* e8,
                        qmlp_stream_t stream) {
   if (!packed || !q || !e8) return set_error(QMLP_E_NULL, "%s: null pointer", fn);
-  if (!shape_ok(rows, cols)) return set_error(QMLP_E_SHAPE, "%s: bad shape %dx%d", fn, rows, cols);
+  if (!packable(rows, cols, fmt)) return set_error(QMLP_E_SHAPE, "%s: bad shape %dx%d", fn, rows, cols);
   if (!aligned16(packed) || !aligned16(q)) return set_error(QMLP_E_ALIGN, "%s: misaligned pointer", fn);
   DeviceInfo di;
   if (int rc = current_device_info(&di)) return rc;
+  if (fmt == QMLP_FMT_MXFP4) return launch_mx_unpack(packed, rows, cols, q, e8, (hipStream_t)stream);
   return launch_unpack(packed, rows, cols, fmt, q, e8, (hipStream_t)stream);
 }
 
@@ -315,19 +327,24 @@ int qmlp_unpack_bf4(const void* packed, int rows, int cols, void* q, void* e8, q
   return unpack_impl("qmlp_unpack_bf4", packed, rows, cols, QMLP_FMT_BF4, q, e8, stream);
 }
 
+int qmlp_unpack_mxfp4(const void* packed, int rows, int cols, void* codes, void* scales, qmlp_stream_t stream) {
+  return unpack_impl("qmlp_unpack_mxfp4", packed, rows, cols, QMLP_FMT_MXFP4, codes, scales, stream);
+}
+
 int qmlp_dequant_packed(const void* packed, int rows, int cols, int fmt, float* out, qmlp_stream_t stream) {
   if (!packed || !out) return set_error(QMLP_E_NULL, "qmlp_dequant_packed: null pointer");
   if (!known_fmt(fmt)) return set_error(QMLP_E_FORMAT, "qmlp_dequant_packed: unknown format");
-  if (!shape_ok(rows, cols)) return set_error(QMLP_E_SHAPE, "qmlp_dequant_packed: bad shape %dx%d", rows, cols);
+  if (!packable(rows, cols, fmt)) return set_error(QMLP_E_SHAPE, "qmlp_dequant_packed: bad shape %dx%d", rows, cols);
   if (!aligned16(packed) || !aligned16(out)) return set_error(QMLP_E_ALIGN, "qmlp_dequant_packed: misaligned pointer");
   DeviceInfo di;
   if (int rc = current_device_info(&di)) return rc;
+  if (fmt == QMLP_FMT_MXFP4) return launch_mx_dequantize(packed, rows, cols, out, true, (hipStream_t)stream);
   return launch_dequant(packed, rows, cols, fmt, out, (hipStream_t)stream);
 }
 
 size_t qmlp_workspace_bytes(int M, int H, int I, int fmt) {
   if (M < 1 || M > 65536 || !shape_ok(16, H) || !shape_ok(16, I) || !known_fmt(fmt)) return 0;
-  return ws_layout(M, H, I, fmt).total;
+  return fmt == QMLP_FMT_MXFP4 ? mx_forward_bytes(M, H, I) : ws_layout(M, H, I, fmt).total;
 }
 
 int qmlp_workspace_init(void* ws, size_t ws_bytes, qmlp_stream_t stream) {
@@ -385,7 +402,7 @@ int qmlp_plan_split(int rows, int K, int nmat, int M, int num_cus, int* out6) {
 
 int qmlp_plan_tiles(int M, int H, int I, int fmt, int down, int num_cus, int* out8) {
   if (!out8) return set_error(QMLP_E_NULL, "qmlp_plan_tiles: null pointer");
-  if (M <= 32 || M > 65536 || num_cus < 1 || !shape_ok(16, H) || !shape_ok(16, I) || !known_fmt(fmt))
+  if (M <= 32 || M > 65536 || num_cus < 1 || !shape_ok(16, H) || !shape_ok(16, I) || !tile_fmt(fmt))
     return set_error(QMLP_E_SHAPE, "qmlp_plan_tiles: M=%d H=%d I=%d fmt=%d on %d CUs", M, H, I, fmt, num_cus);
   plan_tiles_info(M, H, I, fmt, down != 0, num_cus, out8);
   return 0;

@@ -19,6 +19,15 @@ struct PackTrailer : Trailer {
 int set_error(int code, const char* fmt, ...);
 int check_launch(const char* what);
 
+struct DeviceInfo {
+  int ok;  // 1 = gfx950, -1 = unusable
+  int num_cus;
+};
+int current_device_info(DeviceInfo* out);
+
+inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
 // Optional per-kernel timing of the forward pass (qmlp_set_profile_events): slot 0 is the
 // gate/up kernel, slot 1 the down kernel.  profile_events() hands out the slot's start / stop
 // events while timing is on.
@@ -128,5 +137,11 @@ int launch_forward_stream(const ForwardArgs& a, int num_cus, hipStream_t s);
 int forward_impl(const char* fn, const void* x, const void* wg, const void* wu, const void* wd, const void* residual,
                  void* out, void* ws, size_t ws_bytes, int M, int H, int I, int fmt, int flags, const void* normw,
                  float eps, hipStream_t stream);
+
+// The MXFP4 forward (qmlp_mx_abi.hip): arguments validated by forward_impl.
+int mx_forward(const void* x, const void* wg, const void* wu, const void* wd, const void* residual, void* out, void* ws,
+               int M, int H, int I, int flags, const void* normw, float eps, int num_cus, hipStream_t stream);
+size_t mx_forward_bytes(int M, int H, int I);
+bool mx_shape_ok(int rows, int cols);
 
 }  // namespace qmlp

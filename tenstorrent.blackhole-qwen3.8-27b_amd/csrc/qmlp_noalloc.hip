@@ -65,7 +65,8 @@ extern "C" int qmlp_forward_noalloc(const void* x, const void* wg, const void* w
   const size_t need = qmlp_workspace_bytes(M, H, I, fmt);
   if (need == 0) {  // sizes or format out of range
     if (!x || !wg || !wu || !wd || !out) return set_error(QMLP_E_NULL, "qmlp_forward_noalloc: null pointer");
-    if (fmt != QMLP_FMT_BF16 && fmt != QMLP_FMT_BFP8 && fmt != QMLP_FMT_BF4)
+    if (fmt != QMLP_FMT_BF16 && fmt != QMLP_FMT_BFP8 && fmt != QMLP_FMT_BF4 &&
+        fmt != QMLP_FMT_MXFP4)
       return set_error(QMLP_E_FORMAT, "qmlp_forward_noalloc: unknown format %d", fmt);
     return set_error(QMLP_E_SHAPE,
                      "qmlp_forward_noalloc: M=%d H=%d I=%d out of range (1 <= M <= 65536, H and I positive multiples "

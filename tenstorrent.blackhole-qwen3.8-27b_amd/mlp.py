@@ -24,8 +24,10 @@ from . import _lib
 
 # MLP weight formats.  "bf4" is the reference's mixed layout (``mlp.py:17-19,164-169``): gate/up in
 # bf4 (3 magnitude bits), down in bfp8.
-WEIGHT_FORMATS = ("bf16", "bfp8", "bf4")
-MATRIX_FORMATS = ("bf16", "bfp8", "bf4")
+# "mxfp4" is microscaled 4-bit floating point (OCP MX) for all three matrices; the activations are
+# quantised to it in every call.
+WEIGHT_FORMATS = ("bf16", "bfp8", "bf4", "mxfp4")
+MATRIX_FORMATS = ("bf16", "bfp8", "bf4", "mxfp4")
 _MANTISSA_BITS = {"bfp8": 7, "bf4": 3}
 
 
@@ -58,7 +60,7 @@ class PackedWeight:
     @property
     def stream_bytes(self):
         """Bytes of the weight values the forward pass streams (excludes row exponents/trailer)."""
-        per_value = {"bfp8": 17 / 16, "bf4": 9 / 16, "bf16": 2}[self.fmt]
+        per_value = {"bfp8": 17 / 16, "bf4": 9 / 16, "bf16": 2, "mxfp4": 17 / 32}[self.fmt]
         return int(self.rows * self.cols * per_value)
 
     def data_ptr(self):
@@ -118,9 +120,16 @@ def pack_canonical_bfp8(q, e8, strict=True, stream=None):
 
 
 def pack_canonical(q, e8, fmt="bfp8", strict=True, stream=None):
-    """Pack canonical block float (``fmt`` "bfp8" or "bf4") into the device layout."""
+    """Pack canonical block float (``fmt`` "bfp8" or "bf4") into the device layout.
+
+    ``fmt`` "mxfp4": ``q`` holds the codes (uint8 ``[rows, cols/2]``, two to a byte, the even column in
+    the low half) and ``e8`` the scales (uint8 ``[rows, cols/32]``, 2^(e8 - 127)), as microscaled
+    checkpoints store them; a scale of 255 (not a number) is refused.
+    """
+    if fmt == "mxfp4":
+        return _pack_canonical_mxfp4(q, e8, stream)
     if fmt not in _MANTISSA_BITS:
-        raise ValueError(f"canonical format must be bfp8 or bf4, got {fmt!r}")
+        raise ValueError(f"canonical format must be bfp8, bf4 or mxfp4, got {fmt!r}")
     _check_device_tensor(q, "q", torch.int8)
     _check_device_tensor(e8, "e8", torch.uint8)
     rows, cols = q.shape
@@ -139,6 +148,32 @@ def pack_canonical(q, e8, fmt="bfp8", strict=True, stream=None):
     return pw
 
 
+def _unsupported_shape(rows, cols, fmt):
+    if fmt == "mxfp4":
+        return ValueError(f"unsupported shape {rows}x{cols}: cols must be a multiple of 32")
+    return ValueError(f"unsupported shape {rows}x{cols}: rows must be a multiple of 16 and cols of 256")
+
+
+def _pack_canonical_mxfp4(codes, scales, stream):
+    _check_device_tensor(codes, "q", torch.uint8)
+    _check_device_tensor(scales, "e8", torch.uint8)
+    if codes.dim() != 2:
+        raise ValueError("q must be 2-D")
+    rows, cols = codes.shape[0], 2 * codes.shape[1]
+    if tuple(scales.shape) != (rows, cols // 32):
+        raise ValueError("e8 must be [rows, cols/32]")
+    if scales.device != codes.device:
+        raise ValueError("q and e8 must be on the same GPU")
+    nbytes = _lib.lib().qmlp_packed_bytes(rows, cols, _lib.FMT_MXFP4)
+    if nbytes == 0:
+        raise _unsupported_shape(rows, cols, "mxfp4")
+    with _lib.on_device(codes.device, stream):
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
+        _lib.check(_lib.lib().qmlp_pack(_lib.ptr(codes), _lib.ptr(scales), rows, cols, _lib.FMT_MXFP4, _lib.ptr(buf),
+                                        nbytes, _lib.stream_handle(stream)), "qmlp_pack")
+        return _pack_weight_end(PackedWeight(buf, rows, cols, "mxfp4"), True, stream)
+
+
 def _pack_weight_begin(w, fmt, stream):
     """Enqueues the conversion of a bf16 ``[rows, cols]`` GPU tensor; ``_pack_weight_end`` checks it."""
     if fmt not in MATRIX_FORMATS:
@@ -150,7 +185,7 @@ def _pack_weight_begin(w, fmt, stream):
     code = _lib.FORMATS[fmt]
     nbytes = _lib.lib().qmlp_packed_bytes(rows, cols, code)
     if nbytes == 0:
-        raise ValueError(f"unsupported shape {rows}x{cols}: rows must be a multiple of 16 and cols of 256")
+        raise _unsupported_shape(rows, cols, fmt)
     buf = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
     _lib.check(_lib.lib().qmlp_quantize_pack(_lib.ptr(w), rows, cols, code, _lib.ptr(buf), nbytes,
                                              _lib.stream_handle(stream)), "qmlp_quantize_pack")
@@ -175,7 +210,7 @@ def _pack_weight_end(pw, strict, stream):
 
 def pack_weight(w, fmt="bfp8", strict=True, stream=None):
     """bf16 ``[rows, cols]`` GPU tensor (HF layout: [out, in]) -> PackedWeight in the matrix format
-    ``fmt`` ("bf16", "bfp8" or "bf4")."""
+    ``fmt`` ("bf16", "bfp8", "bf4" or "mxfp4")."""
     return _pack_weight_end(_pack_weight_begin(w, fmt, stream), strict, stream)
 
 
@@ -187,9 +222,17 @@ def unpack_bfp8(pw, stream=None):
 
 
 def unpack_canonical(pw, stream=None):
-    """Packed bfp8 or bf4 -> canonical (q, e8) (lossless for unflushed groups)."""
+    """Packed bfp8 or bf4 -> canonical (q, e8) (lossless for unflushed groups); packed mxfp4 (a weight
+    or an ``MxTensor``) -> (codes, scales) (lossless)."""
+    if pw.fmt == "mxfp4":
+        with _lib.on_device(pw.buf.device, stream):
+            codes = torch.empty((pw.rows, pw.cols // 2), dtype=torch.uint8, device=pw.buf.device)
+            scales = torch.empty((pw.rows, pw.cols // 32), dtype=torch.uint8, device=pw.buf.device)
+            _lib.check(_lib.lib().qmlp_unpack_mxfp4(_lib.ptr(pw.buf), pw.rows, pw.cols, _lib.ptr(codes),
+                                                    _lib.ptr(scales), _lib.stream_handle(stream)), "qmlp_unpack_mxfp4")
+        return codes, scales
     if pw.fmt not in _MANTISSA_BITS:
-        raise ValueError("unpacking needs a bfp8 or bf4 weight")
+        raise ValueError("unpacking needs a bfp8, bf4 or mxfp4 weight")
     q = torch.empty((pw.rows, pw.cols), dtype=torch.int8, device=pw.buf.device)
     e8 = torch.empty((pw.rows, pw.cols // 16), dtype=torch.uint8, device=pw.buf.device)
     fn = "qmlp_unpack_" + pw.fmt
@@ -198,8 +241,20 @@ def unpack_canonical(pw, stream=None):
     return q, e8
 
 
-def dequantize(pw, stream=None):
-    """Packed weight -> float32 ``[rows, cols]`` via the kernels' own dequant routine."""
+def dequantize(pw, stream=None, dtype=torch.float32):
+    """Packed weight -> float32 ``[rows, cols]`` via the kernels' own dequant routine.  mxfp4 (a weight
+    or an ``MxTensor``) also to bfloat16, which holds every value of the format exactly."""
+    if pw.fmt == "mxfp4":
+        if dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError("dtype must be bf16 or fp32")
+        with _lib.on_device(pw.buf.device, stream):
+            out = torch.empty((pw.rows, pw.cols), dtype=dtype, device=pw.buf.device)
+            _lib.check(_lib.lib().qmlp_mx_dequantize(_lib.ptr(pw.buf), pw.rows, pw.cols, _lib.ptr(out),
+                                                     _lib.X_F32 if dtype == torch.float32 else _lib.X_BF16,
+                                                     _lib.stream_handle(stream)), "qmlp_mx_dequantize")
+        return out
+    if dtype != torch.float32:
+        raise ValueError("dtype must be fp32")
     out = torch.empty((pw.rows, pw.cols), dtype=torch.float32, device=pw.buf.device)
     _lib.check(_lib.lib().qmlp_dequant_packed(_lib.ptr(pw.buf), pw.rows, pw.cols, pw.fmt_code, _lib.ptr(out),
                                               _lib.stream_handle(stream)), "qmlp_dequant_packed")

@@ -1,0 +1,222 @@
+"""Microscaled 4-bit floating point (OCP MXFP4): the activations' side of the format and the products.
+
+32 consecutive K values share one power-of-two scale byte, each value is one of 0, .5, 1, 1.5, 2, 3, 4,
+6 with a sign.  A block's scale is the binade of its largest magnitude less 2 (at least 2^-126); values
+are rounded half to even and saturate at 6; a block that holds an infinity or a NaN becomes NaN.
+
+* ``quantize_mxfp4(x)`` -> ``MxTensor``, a packed activation matrix that feeds any number of products
+  (``dequantize`` and ``unpack_canonical`` take it too);
+* ``mxfp4_linear(x, w, residual=...)``: ``out = x w^T (+ residual)``;
+* ``mxfp4_swiglu(x, w1, w3)``: ``silu(x w1^T) * (x w3^T)``, the gate/up pair of the block, as rows or
+  (``quantize=True``) as the ``MxTensor`` that the down projection takes.
+
+``x`` is an ``MxTensor`` or a bf16, fp16 or fp32 ``[M, K]`` tensor, which the call quantises; weights come
+from ``pack_weight(w, "mxfp4")`` or, for checkpoints that hold the format, ``pack_canonical(codes, scales,
+"mxfp4")``.  Sizes: any M up to 65536 and any N, K a multiple of 32.  The reference's counterparts are the
+4-bit linears of its block (``docker/qwen-c2-graft/graft/mlp.py:17-19,402-423``) and the fused gate/up
+projection (``scripts/ci/fused_1d.py:123-196``).
+
+Every call runs on the inputs' GPU, on ``stream`` or that GPU's current stream, may be captured into a
+HIP graph and allocates its output and scratch memory from torch's caching allocator there.  Errors:
+``ValueError`` for wrong shapes, dtypes or devices, ``QmlpError`` for launch failures.
+"""
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from .mlp import PackedWeight, _check_device_tensor
+
+_X_TYPES = {torch.bfloat16: _lib.X_BF16, torch.float16: _lib.X_F16, torch.float32: _lib.X_F32}
+
+
+@dataclass
+class MxTensor:
+    """A packed MXFP4 activation matrix ``[rows, cols]`` (device bytes + shape)."""
+
+    buf: torch.Tensor  # uint8, qmlp_packed_bytes(rows, cols, QMLP_FMT_MXFP4) bytes
+    rows: int
+    cols: int
+
+    fmt = "mxfp4"
+    fmt_code = _lib.FMT_MXFP4
+
+    @property
+    def shape(self):
+        return (self.rows, self.cols)
+
+    @property
+    def device(self):
+        return self.buf.device
+
+    @property
+    def nbytes(self):
+        return self.buf.numel()
+
+    def data_ptr(self):
+        return self.buf.data_ptr()
+
+
+def _check_rows(x, name):
+    """A 2-D GPU tensor whose rows are contiguous; the rows themselves may be strided."""
+    if not isinstance(x, torch.Tensor):
+        raise ValueError(f"{name} must be a torch.Tensor or an MxTensor")
+    if x.device.type != "cuda":
+        raise ValueError(f"{name} must be on the GPU, got {x.device}")
+    if x.dtype not in _X_TYPES:
+        raise ValueError(f"{name} must be bf16, fp16 or fp32, got {x.dtype}")
+    if x.dim() != 2 or 0 in x.shape:
+        raise ValueError(f"{name} must be a non-empty 2-D tensor, got {tuple(x.shape)}")
+    if x.shape[1] % 32:
+        raise ValueError(f"{name} must have a multiple of 32 columns (the format's block), got {x.shape[1]}")
+    if x.stride(1) != 1:
+        raise ValueError(f"{name} must have contiguous rows")
+    stride = x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    if stride < x.shape[1] or stride * x.element_size() % 16 or x.data_ptr() % 16:
+        raise ValueError(f"{name}: rows must start at multiples of 16 bytes and not overlap (stride {stride})")
+    return _X_TYPES[x.dtype], stride
+
+
+def _packed_bytes(rows, cols):
+    n = _lib.lib().qmlp_packed_bytes(rows, cols, _lib.FMT_MXFP4)
+    if n == 0:
+        raise ValueError(f"unsupported shape {rows}x{cols}: cols must be a multiple of 32")
+    return n
+
+
+def quantize_mxfp4(x, norm_weight=None, eps=1e-6, stream=None):
+    """bf16, fp16 or fp32 ``[M, K]`` GPU tensor (rows may be strided) -> ``MxTensor``.
+
+    With ``norm_weight`` (bf16 ``[K]``, x bf16) the decoder's zero-centred RMSNorm runs in front, in the
+    same pass: ``n = bf16(rmsnorm(x) * (1 + norm_weight))`` is what is quantised.
+    """
+    x_type, stride = _check_rows(x, "x")
+    M, K = x.shape
+    if norm_weight is not None:
+        _check_device_tensor(norm_weight, "norm_weight", torch.bfloat16)
+        if x.dtype != torch.bfloat16:
+            raise ValueError("x must be bf16 in front of a norm")
+        if tuple(norm_weight.shape) != (K,):
+            raise ValueError(f"norm_weight must have shape ({K},)")
+        _same_device(x.device, norm_weight=norm_weight)
+    with _lib.on_device(x.device, stream):
+        nbytes = _packed_bytes(M, K)
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        if norm_weight is None:
+            _lib.check(_lib.lib().qmlp_mx_quantize(_lib.ptr(x), x_type, stride, M, K, _lib.ptr(buf), nbytes,
+                                                   _lib.stream_handle(stream)), "qmlp_mx_quantize")
+        else:
+            _lib.check(_lib.lib().qmlp_mx_quantize_rmsnorm(_lib.ptr(x), stride, _lib.ptr(norm_weight), float(eps), M, K,
+                                                           _lib.ptr(buf), nbytes, _lib.stream_handle(stream)),
+                       "qmlp_mx_quantize_rmsnorm")
+    return MxTensor(buf, M, K)
+
+
+def _same_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, x on {device}")
+
+
+def _check_weight(w, name, K):
+    if not isinstance(w, PackedWeight) or w.fmt != "mxfp4":
+        raise ValueError(f'{name} must be a PackedWeight in the "mxfp4" format')
+    if w.cols != K:
+        raise ValueError(f"{name} has {w.cols} columns, x has {K}")
+
+
+def _activation(x):
+    """(pointer, QMLP_X_* code, row stride, M, K, device) of an activation argument."""
+    if isinstance(x, MxTensor):
+        return _lib.ptr(x.buf), _lib.X_MXFP4, 0, x.rows, x.cols, x.buf.device
+    x_type, stride = _check_rows(x, "x")
+    return _lib.ptr(x), x_type, stride, x.shape[0], x.shape[1], x.device
+
+
+def _check_out(out, out_dtype, shape):
+    if out is None:
+        if out_dtype not in (None, torch.bfloat16, torch.float32):
+            raise ValueError("out_dtype must be bf16 or fp32")
+        return torch.bfloat16 if out_dtype is None else out_dtype
+    _check_device_tensor(out, "out")
+    if out.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("out must be bf16 or fp32")
+    if out_dtype not in (None, out.dtype):
+        raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
+    if tuple(out.shape) != shape:
+        raise ValueError(f"out must have shape {shape}")
+    return out.dtype
+
+
+def _workspace(M, N, K, device):
+    n = _lib.lib().qmlp_mx_workspace_bytes(M, N, K)
+    if n == 0:
+        raise ValueError(f"unsupported sizes M={M} N={N} K={K}")
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def mxfp4_linear(x, w, residual=None, out=None, out_dtype=None, stream=None):
+    """``out = x w^T (+ residual)`` with both operands in MXFP4 and fp32 sums.
+
+    ``x``: ``MxTensor`` or bf16 / fp16 / fp32 ``[M, K]`` (quantised in the call); ``w``: mxfp4
+    ``PackedWeight`` ``[N, K]``; ``residual`` bf16 or fp32 ``[M, N]``; ``out`` (or ``out_dtype`` when
+    ``out`` is None) bf16, rounded once to nearest-even, or fp32.  ``out`` may be the residual itself.
+    """
+    xp, x_type, stride, M, K, device = _activation(x)
+    _check_weight(w, "w", K)
+    shape = (M, w.rows)
+    dtype = _check_out(out, out_dtype, shape)
+    flags = _lib.OUT_F32 if dtype == torch.float32 else 0
+    if residual is not None:
+        _check_device_tensor(residual, "residual")
+        if residual.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError("residual must be bf16 or fp32")
+        if tuple(residual.shape) != shape:
+            raise ValueError(f"residual must have shape {shape}")
+        if residual.dtype == torch.float32:
+            flags |= _lib.RESIDUAL_F32
+    _same_device(device, w=w.buf, residual=residual, out=out)
+    with _lib.on_device(device, stream):
+        if out is None:
+            out = torch.empty(shape, dtype=dtype, device=device)
+        ws = _workspace(M, w.rows, K, device)
+        _lib.check(_lib.lib().qmlp_mx_linear(xp, x_type, stride, _lib.ptr(w.buf), _lib.ptr(residual), _lib.ptr(out),
+                                             _lib.ptr(ws), ws.numel(), M, w.rows, K, flags,
+                                             _lib.stream_handle(stream)), "qmlp_mx_linear")
+    return out
+
+
+def mxfp4_swiglu(x, w1, w3, out=None, out_dtype=None, quantize=False, stream=None):
+    """``silu(x w1^T) * (x w3^T)`` with every operand in MXFP4 and fp32 sums.
+
+    ``x`` as in ``mxfp4_linear``; ``w1`` (gate) and ``w3`` (up): mxfp4 ``PackedWeight`` ``[N, K]``.  The
+    result is a bf16 or fp32 ``[M, N]`` tensor (``out`` / ``out_dtype``) or, with ``quantize=True`` (N a
+    multiple of 256), an ``MxTensor``, quantised from the fp32 values.
+    """
+    xp, x_type, stride, M, K, device = _activation(x)
+    _check_weight(w1, "w1", K)
+    _check_weight(w3, "w3", K)
+    N = w1.rows
+    if w3.rows != N:
+        raise ValueError(f"w1 has {N} rows, w3 {w3.rows}")
+    if quantize:
+        if out is not None or out_dtype is not None:
+            raise ValueError("quantize=True makes its own MxTensor: out and out_dtype do not apply")
+        if N % 256:
+            raise ValueError(f"quantize=True needs N to be a multiple of 256, got {N}")
+        flags = _lib.OUT_MXFP4
+    else:
+        dtype = _check_out(out, out_dtype, (M, N))
+        flags = _lib.OUT_F32 if dtype == torch.float32 else 0
+    _same_device(device, w1=w1.buf, w3=w3.buf, out=out)
+    with _lib.on_device(device, stream):
+        if quantize:
+            res = MxTensor(torch.empty(_packed_bytes(M, N), dtype=torch.uint8, device=device), M, N)
+            out = res.buf
+        else:
+            out = res = torch.empty((M, N), dtype=dtype, device=device) if out is None else out
+        ws = _workspace(M, N, K, device)
+        _lib.check(_lib.lib().qmlp_mx_swiglu(xp, x_type, stride, _lib.ptr(w1.buf), _lib.ptr(w3.buf), _lib.ptr(out),
+                                             _lib.ptr(ws), ws.numel(), M, N, K, flags, _lib.stream_handle(stream)),
+                   "qmlp_mx_swiglu")
+    return res

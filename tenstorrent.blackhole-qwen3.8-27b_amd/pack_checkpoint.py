@@ -11,7 +11,8 @@ conversion ahead of time for every layer:
   (``--format bf4`` writes gate/up as bf4 and down as bfp8, the reference's mixed layout);
 * with ``--planar`` (block-float formats) also the canonical planar form, ``<name>.q.npy`` (int8
   ``[rows, cols]`` signed mantissas) and ``<name>.e8.npy`` (uint8 ``[rows, cols/16]`` group
-  exponents, scale ``2^(e8 - 127)``), plain ``.npy`` files that ``numpy.load(mmap_mode="r")`` maps.
+  exponents, scale ``2^(e8 - 127)``; ``--format mxfp4``: uint8 ``[rows, cols/2]`` codes and uint8
+  ``[rows, cols/32]`` scales), plain ``.npy`` files that ``numpy.load(mmap_mode="r")`` maps.
 
 Quantisation and packing run on the GPU with the library's own kernels, so the caches are
 bit-identical to what a load-time conversion produces.
@@ -19,7 +20,7 @@ bit-identical to what a load-time conversion produces.
 Usage (from the repository root)::
 
     python tenstorrent.blackhole-qwen3.8-27b_amd/pack_checkpoint.py --checkpoint DIR --out DIR
-        [--format bfp8|bf4|bf16] [--layers 0-63] [--planar]
+        [--format bfp8|bf4|bf16|mxfp4] [--layers 0-63] [--planar]
 """
 import argparse
 import glob
@@ -85,7 +86,7 @@ def pack_layer(entries, out_dir, fmt, device, planar=False):
 
     gu_fmt, down_fmt = mlp.matrix_formats(fmt)
     if planar and fmt == "bf16":
-        raise ValueError("--planar writes block-float mantissa/exponent planes (bfp8 or bf4)")
+        raise ValueError("--planar writes block-float mantissa/exponent planes (bfp8, bf4 or mxfp4)")
     written = []
     for name in ("gate_proj", "up_proj", "down_proj"):
         mfmt = down_fmt if name == "down_proj" else gu_fmt
@@ -100,7 +101,10 @@ def pack_layer(entries, out_dir, fmt, device, planar=False):
         weight_cache.save(cache, pw)
         written.append(cache)
         if planar:
-            q, e8 = mlp.quantize_bf4(w) if mfmt == "bf4" else mlp.quantize_bfp8(w)
+            if mfmt == "mxfp4":
+                q, e8 = mlp.unpack_canonical(pw)
+            else:
+                q, e8 = mlp.quantize_bf4(w) if mfmt == "bf4" else mlp.quantize_bfp8(w)
             np.save(os.path.join(out_dir, f"{name}.q.npy"), q.cpu().numpy())
             np.save(os.path.join(out_dir, f"{name}.e8.npy"), e8.cpu().numpy())
         del w, pw
@@ -111,7 +115,7 @@ def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("--checkpoint", required=True, help="directory holding the HF *.safetensors files")
     ap.add_argument("--out", required=True, help="output directory (one layer_<i> subdirectory per layer)")
-    ap.add_argument("--format", default="bfp8", choices=("bfp8", "bf4", "bf16"))
+    ap.add_argument("--format", default="bfp8", choices=("bfp8", "bf4", "bf16", "mxfp4"))
     ap.add_argument("--layers", default=None, help="e.g. 0-63 or 0,5,7 (default: every layer found)")
     ap.add_argument("--planar", action="store_true", help="also write the canonical block-float planes as .npy")
     ap.add_argument("--device", default="cuda:0")
