@@ -296,6 +296,13 @@ int qmlp_plan_tiles(int M, int H, int I, int fmt, int down, int num_cus, int* ou
  * superblocks of the longest split, groups, tiles one wave may touch}. */
 int qmlp_plan_split(int rows, int K, int nmat, int M, int num_cus, int* out6);
 
+/* How an MXFP4 product of M tokens, N output and K input features and `nmat` matrices (2 = gate/up)
+ * runs on `num_cus` compute units.  Fills out[0..4] = {kernel: 0 a workgroup of four waves per 32
+ * features and 32 tokens, 1 of eight, 2 per 32 features and 64 tokens, 2 + h tiles of 256 features
+ * (of both matrices together) x 64 h tokens; pieces of the K range; workgroups; KB of partial tiles; 1
+ * where the kernel also quantises unpacked rows}. */
+int qmlp_mx_plan(int M, int N, int K, int nmat, int num_cus, int* out5);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,7 +16,8 @@ OBJ_DIR = os.path.join(PKG_DIR, "_build")
 LIB_NAME = "libqwen_mlp.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = ["qmlp_abi.hip", "qmlp_pack.hip", "qmlp_prep.hip", "qmlp_gemv.hip", "qmlp_stream.hip",
-           "qmlp_tiled.hip", "qmlp_noalloc.hip", "qmlp_mx_abi.hip", "qmlp_mx_pack.hip", "qmlp_mx_stream.hip"]
+           "qmlp_tiled.hip", "qmlp_noalloc.hip", "qmlp_mx_abi.hip", "qmlp_mx_plan.hip", "qmlp_mx_pack.hip",
+           "qmlp_mx_stream.hip", "qmlp_mx_tiled.hip"]
 ARCH = "gfx950"
 INCLUDE_DIR = os.path.join(os.path.dirname(PKG_DIR), "include")
 

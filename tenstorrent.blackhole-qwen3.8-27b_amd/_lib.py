@@ -60,6 +60,7 @@ SIGNATURES = {
     "qmlp_mx_dequantize": (_I, [_P, _I, _I, _P, _I, _P]),
     "qmlp_mx_linear": (_I, [_P, _I, _L, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _P]),
     "qmlp_mx_swiglu": (_I, [_P, _I, _L, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _P]),
+    "qmlp_mx_plan": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(ctypes.c_int)]),
     "qmlp_mx_workspace_bytes": (_SZ, [_I, _I, _I]),
 }
 

@@ -22,6 +22,7 @@ constexpr int kMxK = 256;
 constexpr int kMxBlock = 32;
 constexpr int kMxCodes = kMxRows * kMxK / 2;     // 4096
 constexpr int kMxUnit = kMxCodes + kMxRows * 8;  // 4352
+constexpr int kMxPackedX = 3;  // QMLP_X_MXFP4
 constexpr uint32_t kMxNan = 255u;
 constexpr uint32_t kMxMinScale = 1u;  // 2^-126: the smallest scale that is a normal fp32 number
 
@@ -65,6 +66,50 @@ __device__ __forceinline__ uint32_t mx_codes4(f32x4 v, uint32_t byte) {
   return byte == kMxNan ? 0u : o;
 }
 
+// ---------------------------------------------------------------- 8 values of a row
+//
+// Four neighbouring lanes own a block, 8 values each.
+__device__ __forceinline__ uint32_t max4(uint32_t v) {  // over the block's four lanes
+  v = max(v, (uint32_t)__shfl_xor((int)v, 1));
+  return max(v, (uint32_t)__shfl_xor((int)v, 2));
+}
+
+// T: 0 bf16, 1 fp16, 2 fp32 (QMLP_X_*)
+template <int T>
+struct MxWords {
+  u32x4 w[T == 2 ? 2 : 1];
+};
+template <int T>
+__device__ __forceinline__ MxWords<T> mx_load8(const uint8_t* p) {
+  MxWords<T> v;
+  v.w[0] = *(const u32x4*)p;
+  if constexpr (T == 2) v.w[1] = *(const u32x4*)(p + 16);
+  return v;
+}
+template <int T>
+__device__ __forceinline__ void mx_floats(const MxWords<T>& v, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (T == 0) {
+      f[2 * i] = __uint_as_float(v.w[0][i] << 16);
+      f[2 * i + 1] = __uint_as_float(v.w[0][i] & 0xffff0000u);
+    } else if constexpr (T == 1) {
+      const f16x2 h = as_f16x2(v.w[0][i]);
+      f[2 * i] = (float)h.x;
+      f[2 * i + 1] = (float)h.y;
+    } else {
+      f[i] = __uint_as_float(v.w[0][i]);
+      f[4 + i] = __uint_as_float(v.w[1][i]);
+    }
+  }
+}
+__device__ __forceinline__ uint32_t abs_max8(const float (&f)[8]) {
+  uint32_t m = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+  return m;
+}
+
 // D += A B on 32 rows x 32 columns x 64 K; J: the step inside a unit, whose scales are byte J of each
 // lane's scale dword.
 template <int J>
@@ -90,14 +135,35 @@ struct MxOut {
 
 // One product: packed activations x [M, K] times one packed weight matrix [N, K], or two of them.
 struct MxProduct {
-  const uint8_t* x;
+  const uint8_t* x;  // packed, or with x_type < QMLP_X_MXFP4 rows that the product kernel quantises
   const uint8_t* w0;
   const uint8_t* w1;  // up (gated modes)
   int K, mode;
   MxOut o;
   int slot;  // launch_timed's slot, -1: not timed
+  int x_type;        // QMLP_X_*
+  size_t row_bytes;  // of unpacked rows
+  void* parts;       // kMxPartBytes for the partial tiles of split K ranges (many tokens)
 };
-int launch_mx_product(const MxProduct& p, hipStream_t s);
+constexpr size_t kMxPartBytes = 64u << 20;
+constexpr int kMxInside = 4;  // at most this many token rows are quantised inside the streamed product
+bool mx_quantizes_inside(int M, int K);
+constexpr int kMxFewTokens = 32;  // up to here every product is streamed
+
+// How a product runs (mx_plan, qmlp_mx_abi.hip).  Streamed: a workgroup per 32 features, four waves
+// (kMxStream) or eight with two units of K under way each (kMxStreamLong), 32 tokens a workgroup, or
+// 64 (kMxStreamWide).  Tiled (kMxTiles): 256 features (128 of gate and up each) x 64 height tokens a
+// workgroup, the K range in ks pieces.
+enum MxKind { kMxStream, kMxStreamLong, kMxStreamWide, kMxTiles };
+struct MxPlan {
+  MxKind kind;
+  int height, ks;
+  int workgroups;
+  size_t part_bytes;  // of all pieces
+};
+MxPlan mx_plan(int M, int N, int K, int nmat, int num_cus);
+int launch_mx_stream(const MxProduct& p, const MxPlan& pl, hipStream_t s);
+int launch_mx_tiled(const MxProduct& p, const MxPlan& pl, hipStream_t s);
 int launch_mx_quantize(const void* x, int type, size_t row_bytes, int rows, int cols, void* packed, hipStream_t s);
 int launch_mx_norm_quantize(const void* x, size_t row_bytes, const void* w, float eps, int rows, int cols,
                             void* packed, hipStream_t s);
@@ -105,6 +171,13 @@ int launch_mx_quantize_pack(const void* w, int rows, int cols, void* packed, hip
 int launch_mx_pack(const void* codes, const void* scales, int rows, int cols, void* packed, hipStream_t s);
 int launch_mx_unpack(const void* packed, int rows, int cols, void* codes, void* scales, hipStream_t s);
 int launch_mx_dequantize(const void* packed, int rows, int cols, void* out, bool f32, hipStream_t s);
+
+// Two fp32 values -> bf16, rounded half to even (v_cvt_pk_bf16_f32, one instruction where the word
+// arithmetic of f32_to_bf16 takes a dozen).
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t mx_bf16x2(float a, float b) {
+  return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+}
 
 // Four neighbouring features n..n+3 of token m.  N may be any number: rows whose length is not a
 // multiple of 4 start misaligned for vector stores.
@@ -125,8 +198,7 @@ __device__ __forceinline__ void mx_store4(const MxOut& o, int m, int n, f32x4 v)
       *(f32x4*)((float*)o.out + at) = v;
     } else {
       *(u32x2*)((uint16_t*)o.out + at) =
-          u32x2{(uint32_t)f32_to_bf16(v.x) | ((uint32_t)f32_to_bf16(v.y) << 16),
-                (uint32_t)f32_to_bf16(v.z) | ((uint32_t)f32_to_bf16(v.w) << 16)};
+          u32x2{mx_bf16x2(v.x, v.y), mx_bf16x2(v.z, v.w)};
     }
     return;
   }

@@ -15,33 +15,50 @@ bool mx_shape_ok(int rows, int cols) {
 static bool mx_tokens_ok(int M) { return M >= 1 && M <= 65536; }
 
 // Forward workspace: the arrival counters that every format's workspace starts with (a pool's
-// workspace may serve other formats in turn; these kernels leave them alone), the quantised x and h.
+// workspace may serve other formats in turn; these kernels leave them alone), the quantised x and h, and
+// for many tokens the partial tiles of split K ranges, which both products use in turn.
+static size_t part_bytes(int M) { return M > kMxFewTokens ? kMxPartBytes : 0; }
 struct MxWs {
-  size_t x, h, total;
+  size_t x, h, parts, total;
 };
 static MxWs mx_ws(int M, int H, int I) {
   MxWs L{};
   L.x = align256(QMLP_WS_COUNTER_BYTES);
   L.h = L.x + align256(mx_units_bytes(M, H));
-  L.total = L.h + align256(mx_units_bytes(M, I));
+  L.parts = L.h + align256(mx_units_bytes(M, I));
+  L.total = L.parts + part_bytes(M);
   return L;
 }
 size_t mx_forward_bytes(int M, int H, int I) { return mx_ws(M, H, I).total; }
+
+// One product as planned for its sizes; unpacked rows are quantised into packed_x first unless the
+// kernel does that itself.
+static int run_product(MxProduct p, void* packed_x, int num_cus, hipStream_t s) {
+  const MxPlan plan = mx_plan(p.o.M, p.o.N, p.K, p.mode == kMxRowsOut ? 1 : 2, num_cus);
+  if (p.x_type != QMLP_X_MXFP4 && !mx_quantizes_inside(p.o.M, p.K)) {
+    if (int rc = launch_mx_quantize(p.x, p.x_type, p.row_bytes, p.o.M, p.K, packed_x, s)) return rc;
+    p.x = (const uint8_t*)packed_x;
+    p.x_type = QMLP_X_MXFP4;
+  }
+  return plan.kind == kMxTiles ? launch_mx_tiled(p, plan, s) : launch_mx_stream(p, plan, s);
+}
 
 int mx_forward(const void* x, const void* wg, const void* wu, const void* wd, const void* residual, void* out, void* ws,
                int M, int H, int I, int flags, const void* normw, float eps, int num_cus, hipStream_t s) {
   const MxWs L = mx_ws(M, H, I);
   uint8_t* base = (uint8_t*)ws;
+  MxProduct gu{(const uint8_t*)x, (const uint8_t*)wg, (const uint8_t*)wu, H, kMxPacked,
+               {base + L.h, nullptr, M, I, 0, 0}, 0, QMLP_X_BF16, (size_t)H * 2, base + L.parts};
   if (normw) {
     if (int rc = launch_mx_norm_quantize(x, (size_t)H * 2, normw, eps, M, H, base + L.x, s)) return rc;
-  } else {
-    if (int rc = launch_mx_quantize(x, QMLP_X_BF16, (size_t)H * 2, M, H, base + L.x, s)) return rc;
+    gu.x = base + L.x;
+    gu.x_type = QMLP_X_MXFP4;
   }
-  MxProduct gu{base + L.x, (const uint8_t*)wg, (const uint8_t*)wu, H, kMxPacked, {base + L.h, nullptr, M, I, 0, 0}, 0};
-  if (int rc = launch_mx_product(gu, s)) return rc;
+  if (int rc = run_product(gu, base + L.x, num_cus, s)) return rc;
   MxProduct down{base + L.h, (const uint8_t*)wd, nullptr, I, kMxRowsOut,
-                 {out, residual, M, H, (flags & QMLP_OUT_F32) ? 1 : 0, (flags & QMLP_RESIDUAL_F32) ? 1 : 0}, 1};
-  return launch_mx_product(down, s);
+                 {out, residual, M, H, (flags & QMLP_OUT_F32) ? 1 : 0, (flags & QMLP_RESIDUAL_F32) ? 1 : 0},
+                 1, QMLP_X_MXFP4, 0, base + L.parts};
+  return run_product(down, nullptr, num_cus, s);
 }
 
 // [p, p + n) and [q, q + m) have a byte in common.
@@ -100,15 +117,11 @@ static int product_impl(const char* fn, const void* x, int x_type, int64_t x_str
     return set_error(QMLP_E_SHAPE, "%s: the workspace must not overlap another argument", fn);
   DeviceInfo di;
   if (int rc = current_device_info(&di)) return rc;
-  const uint8_t* xp = (const uint8_t*)x;
-  if (x_type != QMLP_X_MXFP4) {
-    if (int rc = launch_mx_quantize(x, x_type, (size_t)x_stride * x_size(x_type), M, K, ws, s)) return rc;
-    xp = (const uint8_t*)ws;
-  }
-  MxProduct p{xp, (const uint8_t*)w0, (const uint8_t*)w1, K,
+  MxProduct p{(const uint8_t*)x, (const uint8_t*)w0, (const uint8_t*)w1, K,
               nmat == 1 ? kMxRowsOut : packed_out ? kMxPacked : kMxGated,
-              {out, residual, M, N, (flags & QMLP_OUT_F32) ? 1 : 0, (flags & QMLP_RESIDUAL_F32) ? 1 : 0}, -1};
-  return launch_mx_product(p, s);
+              {out, residual, M, N, (flags & QMLP_OUT_F32) ? 1 : 0, (flags & QMLP_RESIDUAL_F32) ? 1 : 0},
+              -1, x_type, (size_t)x_stride * x_size(x_type), (uint8_t*)ws + align256(mx_units_bytes(M, K))};
+  return run_product(p, ws, di.num_cus, s);
 }
 
 }  // namespace qmlp
@@ -119,7 +132,20 @@ extern "C" {
 
 size_t qmlp_mx_workspace_bytes(int M, int N, int K) {
   if (!mx_tokens_ok(M) || !mx_shape_ok(N, K)) return 0;
-  return align256(mx_units_bytes(M, K));
+  return align256(mx_units_bytes(M, K)) + part_bytes(M);
+}
+
+int qmlp_mx_plan(int M, int N, int K, int nmat, int num_cus, int* out5) {
+  if (!out5) return set_error(QMLP_E_NULL, "qmlp_mx_plan: null pointer");
+  if (!mx_tokens_ok(M) || !mx_shape_ok(N, K) || nmat < 1 || nmat > 2 || num_cus < 1)
+    return set_error(QMLP_E_SHAPE, "qmlp_mx_plan: M=%d N=%d K=%d, %d matrices on %d CUs", M, N, K, nmat, num_cus);
+  const MxPlan p = mx_plan(M, N, K, nmat, num_cus);
+  out5[0] = p.kind == kMxTiles ? 2 + p.height : (int)p.kind;
+  out5[1] = p.ks;
+  out5[2] = p.workgroups;
+  out5[3] = (int)(p.part_bytes >> 10);
+  out5[4] = mx_quantizes_inside(M, K) ? 1 : 0;
+  return 0;
 }
 
 static int quantize_checks(const char* fn, const void* x, int x_type, int64_t x_stride, int rows, int cols,

@@ -21,47 +21,6 @@ __device__ __forceinline__ MxItem mx_item(int tid) {
   return MxItem{tid & 3, (tid >> 2) & 7, (tid >> 6) * 2 + ((tid >> 5) & 1)};
 }
 
-__device__ __forceinline__ uint32_t max4(uint32_t v) {  // over the block's four lanes
-  v = max(v, (uint32_t)__shfl_xor((int)v, 1));
-  return max(v, (uint32_t)__shfl_xor((int)v, 2));
-}
-
-// T: 0 bf16, 1 fp16, 2 fp32 (QMLP_X_*)
-template <int T>
-struct MxWords {
-  u32x4 w[T == 2 ? 2 : 1];
-};
-template <int T>
-__device__ __forceinline__ MxWords<T> mx_load8(const uint8_t* p) {
-  MxWords<T> v;
-  v.w[0] = *(const u32x4*)p;
-  if constexpr (T == 2) v.w[1] = *(const u32x4*)(p + 16);
-  return v;
-}
-template <int T>
-__device__ __forceinline__ void mx_floats(const MxWords<T>& v, float (&f)[8]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (T == 0) {
-      f[2 * i] = __uint_as_float(v.w[0][i] << 16);
-      f[2 * i + 1] = __uint_as_float(v.w[0][i] & 0xffff0000u);
-    } else if constexpr (T == 1) {
-      const f16x2 h = as_f16x2(v.w[0][i]);
-      f[2 * i] = (float)h.x;
-      f[2 * i + 1] = (float)h.y;
-    } else {
-      f[i] = __uint_as_float(v.w[0][i]);
-      f[4 + i] = __uint_as_float(v.w[1][i]);
-    }
-  }
-}
-__device__ __forceinline__ uint32_t abs_max8(const float (&f)[8]) {
-  uint32_t m = 0u;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
-  return m;
-}
-
 // ---------------------------------------------------------------- quantisation
 //
 // Bound by memory for many rows (2 or 4 bytes read and 17/32 written per value), by latency for few.
