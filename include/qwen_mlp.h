@@ -216,8 +216,9 @@ int qmlp_mx_dequantize(const void* packed, int rows, int cols, void* out, int ou
 
 /* out[M, N] = x W^T (+ residual): x of any x_type, quantised in the call unless it is QMLP_X_MXFP4; w
  * packed [N, K].  flags: QMLP_OUT_F32, QMLP_RESIDUAL_F32.  out may be the residual itself (of the same
- * dtype) and must not overlap anything else.  ws: qmlp_mx_workspace_bytes(M, N, K) bytes that may hold
- * anything (nothing to initialise); calls that overlap need separate ones. */
+ * dtype) and must not overlap anything else.  ws: qmlp_mx_workspace_bytes(M, N, K, x_type) bytes that may
+ * hold anything (nothing to initialise), null where that is 0; calls that run at the same time need
+ * separate ones. */
 int qmlp_mx_linear(const void* x, int x_type, int64_t x_stride, const void* w, const void* residual,
                    void* out, void* ws, size_t ws_bytes, int M, int N, int K, int flags,
                    qmlp_stream_t stream);
@@ -228,8 +229,10 @@ int qmlp_mx_linear(const void* x, int x_type, int64_t x_stride, const void* w, c
 int qmlp_mx_swiglu(const void* x, int x_type, int64_t x_stride, const void* wg, const void* wu, void* out,
                    void* ws, size_t ws_bytes, int M, int N, int K, int flags, qmlp_stream_t stream);
 
-/* Workspace bytes of the two products (host only); never shrinks as M grows.  0: sizes out of range. */
-size_t qmlp_mx_workspace_bytes(int M, int N, int K);
+/* Workspace bytes of the two products (host only); never shrinks as M grows.  0 where none is needed
+ * (packed x up to 32 tokens, a token or two that the product quantises itself), and for sizes out of
+ * range, which the product refuses. */
+size_t qmlp_mx_workspace_bytes(int M, int N, int K, int x_type);
 
 /* Workspace bytes needed by qmlp_forward for these sizes (host only, no GPU needed).  The size
  * never decreases as M grows, so a workspace sized for M serves every call with fewer tokens, and
@@ -298,8 +301,8 @@ int qmlp_plan_split(int rows, int K, int nmat, int M, int num_cus, int* out6);
 
 /* How an MXFP4 product of M tokens, N output and K input features and `nmat` matrices (2 = gate/up)
  * runs on `num_cus` compute units.  Fills out[0..4] = {kernel: 0 a workgroup of four waves per 32
- * features and 32 tokens, 1 of eight, 2 per 32 features and 64 tokens, 2 + h tiles of 256 features
- * (of both matrices together) x 64 h tokens; pieces of the K range; workgroups; KB of partial tiles; 1
+ * features and 32 tokens, 1 the same with twice the loads under way, 2 of eight waves, 3 per 32 features
+ * and 64 tokens, 3 + h tiles of 256 features (of both matrices together) x 64 h tokens; pieces of the K range; workgroups; KB of partial tiles; 1
  * where the kernel also quantises unpacked rows}. */
 int qmlp_mx_plan(int M, int N, int K, int nmat, int num_cus, int* out5);
 

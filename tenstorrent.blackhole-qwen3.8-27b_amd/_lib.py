@@ -61,7 +61,7 @@ SIGNATURES = {
     "qmlp_mx_linear": (_I, [_P, _I, _L, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _P]),
     "qmlp_mx_swiglu": (_I, [_P, _I, _L, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _P]),
     "qmlp_mx_plan": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(ctypes.c_int)]),
-    "qmlp_mx_workspace_bytes": (_SZ, [_I, _I, _I]),
+    "qmlp_mx_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
 }
 
 _lib = None
@@ -135,30 +135,35 @@ def stream_handle(stream=None):
     return ctypes.c_void_p(raw_stream() if stream is None else stream.cuda_stream)
 
 
-class on_device:
-    """Makes ``device`` (a GPU) current for a call, and ``stream`` (if one is given) the stream that
-    tensors are allocated on, so that the caching allocator orders their memory with that stream's
-    work.  Does nothing where the device is current already and no stream is given."""
-
-    def __init__(self, device, stream=None):
-        import torch
-
-        if stream is not None and stream.device != device:
-            raise ValueError(f"stream is on {stream.device}, the tensors are on {device}")
-        if stream is not None:
-            self._inner = torch.cuda.stream(stream)  # makes the stream's device current too
-        elif device.index is not None and device.index != torch.cuda.current_device():
-            self._inner = torch.cuda.device(device)
-        else:
-            self._inner = None
-
+class _Nothing:
     def __enter__(self):
-        if self._inner is not None:
-            self._inner.__enter__()
+        return None
 
     def __exit__(self, *exc):
-        if self._inner is not None:
-            self._inner.__exit__(*exc)
+        return False
+
+
+_NOTHING = _Nothing()
+
+
+def on_device(device, stream=None):
+    """A context that makes ``device`` (a GPU) current for a call, and ``stream`` (if one is given) the
+    stream that tensors are allocated on, so that the caching allocator orders their memory with that
+    stream's work.  Does nothing where the device is current already and no stream is given."""
+    import torch
+
+    if stream is None:
+        return _NOTHING if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+    if stream.device != device:
+        raise ValueError(f"stream is on {stream.device}, the tensors are on {device}")
+    return torch.cuda.stream(stream)  # makes the stream's device current too
+
+
+def device_stream(device, stream=None):
+    """The handle of ``stream``, or of ``device``'s current stream."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(device.index) if stream is None else stream.cuda_stream
 
 
 def raw_stream(index=None):

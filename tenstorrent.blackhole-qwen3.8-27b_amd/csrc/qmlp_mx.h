@@ -150,11 +150,11 @@ constexpr int kMxInside = 4;  // at most this many token rows are quantised insi
 bool mx_quantizes_inside(int M, int K);
 constexpr int kMxFewTokens = 32;  // up to here every product is streamed
 
-// How a product runs (mx_plan, qmlp_mx_abi.hip).  Streamed: a workgroup per 32 features, four waves
-// (kMxStream) or eight with two units of K under way each (kMxStreamLong), 32 tokens a workgroup, or
-// 64 (kMxStreamWide).  Tiled (kMxTiles): 256 features (128 of gate and up each) x 64 height tokens a
-// workgroup, the K range in ks pieces.
-enum MxKind { kMxStream, kMxStreamLong, kMxStreamWide, kMxTiles };
+// How a product runs (mx_plan, qmlp_mx_plan.hip).  Streamed: a workgroup of 32 features x 32 tokens, four
+// waves with one unit of K under way (kMxStream) or two (kMxStreamDeep, one matrix only), or eight with
+// two (kMxStreamLong); or of 32 features x 64 tokens (kMxStreamWide).  Tiled (kMxTiles): 256 features (128
+// of gate and up each) x 64 height tokens a workgroup, the K range in ks pieces.
+enum MxKind { kMxStream, kMxStreamDeep, kMxStreamLong, kMxStreamWide, kMxTiles };
 struct MxPlan {
   MxKind kind;
   int height, ks;

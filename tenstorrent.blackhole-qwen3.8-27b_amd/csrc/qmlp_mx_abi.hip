@@ -18,6 +18,10 @@ static bool mx_tokens_ok(int M) { return M >= 1 && M <= 65536; }
 // workspace may serve other formats in turn; these kernels leave them alone), the quantised x and h, and
 // for many tokens the partial tiles of split K ranges, which both products use in turn.
 static size_t part_bytes(int M) { return M > kMxFewTokens ? kMxPartBytes : 0; }
+// Unpacked rows that the product does not quantise by itself.
+static size_t packed_x_bytes(int M, int K, int x_type) {
+  return x_type == QMLP_X_MXFP4 || mx_quantizes_inside(M, K) ? 0 : align256(mx_units_bytes(M, K));
+}
 struct MxWs {
   size_t x, h, parts, total;
 };
@@ -86,7 +90,7 @@ static size_t rows_extent(int type, int64_t stride, int M, int K) {
 static int product_impl(const char* fn, const void* x, int x_type, int64_t x_stride, const void* w0, const void* w1,
                         int nmat, const void* residual, void* out, void* ws, size_t ws_bytes, int M, int N, int K,
                         int flags, hipStream_t s) {
-  if (!x || !w0 || (nmat > 1 && !w1) || !out || !ws) return set_error(QMLP_E_NULL, "%s: null pointer", fn);
+  if (!x || !w0 || (nmat > 1 && !w1) || !out) return set_error(QMLP_E_NULL, "%s: null pointer", fn);
   const int known = nmat > 1 ? (QMLP_OUT_F32 | QMLP_OUT_MXFP4) : (QMLP_OUT_F32 | QMLP_RESIDUAL_F32);
   if ((flags & ~known) || ((flags & QMLP_OUT_F32) && (flags & QMLP_OUT_MXFP4)))
     return set_error(QMLP_E_FORMAT, "%s: bad flags 0x%x", fn, flags);
@@ -109,7 +113,8 @@ static int product_impl(const char* fn, const void* x, int x_type, int64_t x_str
     return set_error(QMLP_E_SHAPE, "%s: out may equal residual but must not partially overlap it", fn);
   if (residual && residual == out && ((flags & QMLP_OUT_F32) != 0) != ((flags & QMLP_RESIDUAL_F32) != 0))
     return set_error(QMLP_E_SHAPE, "%s: an in-place residual needs the same dtype as out", fn);
-  const size_t need = qmlp_mx_workspace_bytes(M, N, K);
+  const size_t need = qmlp_mx_workspace_bytes(M, N, K, x_type);
+  if (need && !ws) return set_error(QMLP_E_NULL, "%s: null workspace", fn);
   if (ws_bytes < need)
     return set_error(QMLP_E_WORKSPACE, "%s: workspace holds %zu bytes, needs %zu", fn, ws_bytes, need);
   if (overlap(ws, need, x, xbytes) || overlap(ws, need, out, obytes) || overlap(ws, need, residual, rbytes) ||
@@ -120,7 +125,7 @@ static int product_impl(const char* fn, const void* x, int x_type, int64_t x_str
   MxProduct p{(const uint8_t*)x, (const uint8_t*)w0, (const uint8_t*)w1, K,
               nmat == 1 ? kMxRowsOut : packed_out ? kMxPacked : kMxGated,
               {out, residual, M, N, (flags & QMLP_OUT_F32) ? 1 : 0, (flags & QMLP_RESIDUAL_F32) ? 1 : 0},
-              -1, x_type, (size_t)x_stride * x_size(x_type), (uint8_t*)ws + align256(mx_units_bytes(M, K))};
+              -1, x_type, (size_t)x_stride * x_size(x_type), (uint8_t*)ws + packed_x_bytes(M, K, x_type)};
   return run_product(p, ws, di.num_cus, s);
 }
 
@@ -130,9 +135,9 @@ using namespace qmlp;
 
 extern "C" {
 
-size_t qmlp_mx_workspace_bytes(int M, int N, int K) {
+size_t qmlp_mx_workspace_bytes(int M, int N, int K, int x_type) {
   if (!mx_tokens_ok(M) || !mx_shape_ok(N, K)) return 0;
-  return align256(mx_units_bytes(M, K)) + part_bytes(M);
+  return packed_x_bytes(M, K, x_type) + part_bytes(M);
 }
 
 int qmlp_mx_plan(int M, int N, int K, int nmat, int num_cus, int* out5) {
@@ -140,7 +145,7 @@ int qmlp_mx_plan(int M, int N, int K, int nmat, int num_cus, int* out5) {
   if (!mx_tokens_ok(M) || !mx_shape_ok(N, K) || nmat < 1 || nmat > 2 || num_cus < 1)
     return set_error(QMLP_E_SHAPE, "qmlp_mx_plan: M=%d N=%d K=%d, %d matrices on %d CUs", M, N, K, nmat, num_cus);
   const MxPlan p = mx_plan(M, N, K, nmat, num_cus);
-  out5[0] = p.kind == kMxTiles ? 2 + p.height : (int)p.kind;
+  out5[0] = p.kind == kMxTiles ? kMxStreamWide + p.height : (int)p.kind;
   out5[1] = p.ks;
   out5[2] = p.workgroups;
   out5[3] = (int)(p.part_bytes >> 10);

@@ -209,6 +209,9 @@ static int launch_mode(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
   if constexpr (XT == kMxPackedX) {
     if (pl.kind == kMxStreamWide) return launch_stream<NMAT, NMAT == 1 ? 8 : 4, 2, 2, MODE, XT>(p, s);
   }
+  if constexpr (NMAT == 1) {
+    if (pl.kind == kMxStreamDeep) return launch_stream<1, 4, 1, 2, MODE, XT>(p, s);
+  }
   if (pl.kind == kMxStreamLong) return launch_stream<NMAT, 8, 1, 2, MODE, XT>(p, s);
   return launch_stream<NMAT, 4, 1, 1, MODE, XT>(p, s);
 }

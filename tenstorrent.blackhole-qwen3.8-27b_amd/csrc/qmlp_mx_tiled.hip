@@ -1,5 +1,6 @@
 // qmlp_mx_tiled.hip -- MXFP4 products of many tokens: both operands staged through LDS (layout:
 // qmlp_mx.h).
+#include <atomic>
 #include <type_traits>
 
 #include "qmlp_internal.h"
@@ -316,22 +317,40 @@ __global__ __launch_bounds__(256) void mx_sum_kernel(const f32x4* __restrict__ p
                         s_turn[threadIdx.x >> 6], v);
 }
 
+template <typename T, int NMAT, int MODE, int WF, int WT, int NF, int NT>
+static int launch_sum(const MxProduct& p, int tiles, int ntt, int ks, hipStream_t s) {
+  constexpr int kItems = T::kWaves * WF / NMAT * WT;
+  launch_timed_part(p.slot, 2, mx_sum_kernel<NMAT, WF, WT, NF, NT, MODE>, dim3((tiles * kItems + 3) / 4), dim3(256), 0, s,
+                    (const f32x4*)p.parts, tiles, ntt, ks, p.o);
+  return check_launch("mx_sum_kernel");
+}
+
+// Raises a kernel's dynamic LDS limit, once per device (a mask per kernel, bit: device).
+template <typename K>
+static int raise_lds_once(K kern, int bytes, std::atomic<uint64_t>& raised) {
+  int dev = -1;
+  if (hipGetDevice(&dev) != hipSuccess) return check_launch("hipGetDevice");
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(raised.load(std::memory_order_relaxed) & bit)) {
+    if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+      return check_launch("hipFuncSetAttribute");
+    raised.fetch_or(bit, std::memory_order_relaxed);
+  }
+  return 0;
+}
+
 template <int NMAT, int WF, int WT, int NF, int NT, int MODE>
 static int launch_tile(const MxProduct& p, int ks, hipStream_t s) {
   using T = MxTile<NMAT, WF, WT, NF, NT>;
   auto kern = mx_tiled_kernel<NMAT, WF, WT, NF, NT, MODE>;
-  if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds) != hipSuccess)
-    return check_launch("hipFuncSetAttribute");
+  static std::atomic<uint64_t> raised{0};
+  if (int rc = raise_lds_once(kern, T::kLds, raised)) return rc;
   const int nft = (p.o.N + T::kFeatures - 1) / T::kFeatures, ntt = (p.o.M + T::kTokens - 1) / T::kTokens;
   const int tiles = nft * ntt;
   launch_timed_part(p.slot, ks > 1 ? 1 : 3, kern, dim3(tiles * ks), dim3(T::kWaves * 64), T::kLds, s, p.x, p.w0, p.w1,
                     mx_ksb(p.K), ntt, ks, (f32x4*)p.parts, p.o);
   if (int rc = check_launch("mx_tiled_kernel")) return rc;
-  if (ks == 1) return 0;
-  constexpr int kItems = T::kWaves * WF / NMAT * WT;
-  launch_timed_part(p.slot, 2, mx_sum_kernel<NMAT, WF, WT, NF, NT, MODE>, dim3((tiles * kItems + 3) / 4), dim3(256), 0, s,
-                    (const f32x4*)p.parts, tiles, ntt, ks, p.o);
-  return check_launch("mx_sum_kernel");
+  return ks == 1 ? 0 : launch_sum<T, NMAT, MODE, WF, WT, NF, NT>(p, tiles, ntt, ks, s);
 }
 
 template <int MODE>

@@ -170,7 +170,7 @@ def _pack_canonical_mxfp4(codes, scales, stream):
     with _lib.on_device(codes.device, stream):
         buf = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
         _lib.check(_lib.lib().qmlp_pack(_lib.ptr(codes), _lib.ptr(scales), rows, cols, _lib.FMT_MXFP4, _lib.ptr(buf),
-                                        nbytes, _lib.stream_handle(stream)), "qmlp_pack")
+                                        nbytes, _lib.device_stream(codes.device, stream)), "qmlp_pack")
         return _pack_weight_end(PackedWeight(buf, rows, cols, "mxfp4"), True, stream)
 
 
@@ -229,7 +229,8 @@ def unpack_canonical(pw, stream=None):
             codes = torch.empty((pw.rows, pw.cols // 2), dtype=torch.uint8, device=pw.buf.device)
             scales = torch.empty((pw.rows, pw.cols // 32), dtype=torch.uint8, device=pw.buf.device)
             _lib.check(_lib.lib().qmlp_unpack_mxfp4(_lib.ptr(pw.buf), pw.rows, pw.cols, _lib.ptr(codes),
-                                                    _lib.ptr(scales), _lib.stream_handle(stream)), "qmlp_unpack_mxfp4")
+                                                    _lib.ptr(scales), _lib.device_stream(pw.buf.device, stream)),
+                       "qmlp_unpack_mxfp4")
         return codes, scales
     if pw.fmt not in _MANTISSA_BITS:
         raise ValueError("unpacking needs a bfp8, bf4 or mxfp4 weight")
@@ -249,9 +250,10 @@ def dequantize(pw, stream=None, dtype=torch.float32):
             raise ValueError("dtype must be bf16 or fp32")
         with _lib.on_device(pw.buf.device, stream):
             out = torch.empty((pw.rows, pw.cols), dtype=dtype, device=pw.buf.device)
-            _lib.check(_lib.lib().qmlp_mx_dequantize(_lib.ptr(pw.buf), pw.rows, pw.cols, _lib.ptr(out),
-                                                     _lib.X_F32 if dtype == torch.float32 else _lib.X_BF16,
-                                                     _lib.stream_handle(stream)), "qmlp_mx_dequantize")
+            rc = _lib.lib().qmlp_mx_dequantize(pw.buf.data_ptr(), pw.rows, pw.cols, out.data_ptr(),
+                                               _lib.X_F32 if dtype == torch.float32 else _lib.X_BF16,
+                                               _lib.device_stream(pw.buf.device, stream))
+            _lib.check(rc, "qmlp_mx_dequantize")
         return out
     if dtype != torch.float32:
         raise ValueError("dtype must be fp32")

@@ -20,6 +20,7 @@ Every call runs on the inputs' GPU, on ``stream`` or that GPU's current stream, 
 HIP graph and allocates its output and scratch memory from torch's caching allocator there.  Errors:
 ``ValueError`` for wrong shapes, dtypes or devices, ``QmlpError`` for launch failures.
 """
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -57,26 +58,32 @@ class MxTensor:
         return self.buf.data_ptr()
 
 
-def _check_rows(x, name):
-    """A 2-D GPU tensor whose rows are contiguous; the rows themselves may be strided."""
+def _check_rows(x):
+    """(QMLP_X_* code, row stride) of a 2-D GPU tensor whose rows are contiguous; the rows themselves may
+    be strided."""
     if not isinstance(x, torch.Tensor):
-        raise ValueError(f"{name} must be a torch.Tensor or an MxTensor")
-    if x.device.type != "cuda":
-        raise ValueError(f"{name} must be on the GPU, got {x.device}")
-    if x.dtype not in _X_TYPES:
-        raise ValueError(f"{name} must be bf16, fp16 or fp32, got {x.dtype}")
+        raise ValueError("x must be a torch.Tensor or an MxTensor")
+    if not x.is_cuda:
+        raise ValueError(f"x must be on the GPU, got {x.device}")
+    x_type = _X_TYPES.get(x.dtype)
+    if x_type is None:
+        raise ValueError(f"x must be bf16, fp16 or fp32, got {x.dtype}")
     if x.dim() != 2 or 0 in x.shape:
-        raise ValueError(f"{name} must be a non-empty 2-D tensor, got {tuple(x.shape)}")
-    if x.shape[1] % 32:
-        raise ValueError(f"{name} must have a multiple of 32 columns (the format's block), got {x.shape[1]}")
-    if x.stride(1) != 1:
-        raise ValueError(f"{name} must have contiguous rows")
-    stride = x.stride(0) if x.shape[0] > 1 else x.shape[1]
-    if stride < x.shape[1] or stride * x.element_size() % 16 or x.data_ptr() % 16:
-        raise ValueError(f"{name}: rows must start at multiples of 16 bytes and not overlap (stride {stride})")
-    return _X_TYPES[x.dtype], stride
+        raise ValueError(f"x must be a non-empty 2-D tensor, got {tuple(x.shape)}")
+    rows, cols = x.shape
+    if cols % 32:
+        raise ValueError(f"x must have a multiple of 32 columns (the format's block), got {cols}")
+    stride, step = x.stride()
+    if step != 1:
+        raise ValueError("x must have contiguous rows")
+    if rows == 1:
+        stride = cols
+    if stride < cols or stride * (4 if x_type == _lib.X_F32 else 2) % 16 or x.data_ptr() % 16:
+        raise ValueError(f"x: rows must start at multiples of 16 bytes and not overlap (stride {stride})")
+    return x_type, stride
 
 
+@functools.lru_cache(maxsize=4096)
 def _packed_bytes(rows, cols):
     n = _lib.lib().qmlp_packed_bytes(rows, cols, _lib.FMT_MXFP4)
     if n == 0:
@@ -90,7 +97,7 @@ def quantize_mxfp4(x, norm_weight=None, eps=1e-6, stream=None):
     With ``norm_weight`` (bf16 ``[K]``, x bf16) the decoder's zero-centred RMSNorm runs in front, in the
     same pass: ``n = bf16(rmsnorm(x) * (1 + norm_weight))`` is what is quantised.
     """
-    x_type, stride = _check_rows(x, "x")
+    x_type, stride = _check_rows(x)
     M, K = x.shape
     if norm_weight is not None:
         _check_device_tensor(norm_weight, "norm_weight", torch.bfloat16)
@@ -99,16 +106,16 @@ def quantize_mxfp4(x, norm_weight=None, eps=1e-6, stream=None):
         if tuple(norm_weight.shape) != (K,):
             raise ValueError(f"norm_weight must have shape ({K},)")
         _same_device(x.device, norm_weight=norm_weight)
-    with _lib.on_device(x.device, stream):
-        nbytes = _packed_bytes(M, K)
-        buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    device, nbytes = x.device, _packed_bytes(M, K)
+    with _lib.on_device(device, stream):
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
         if norm_weight is None:
-            _lib.check(_lib.lib().qmlp_mx_quantize(_lib.ptr(x), x_type, stride, M, K, _lib.ptr(buf), nbytes,
-                                                   _lib.stream_handle(stream)), "qmlp_mx_quantize")
+            rc = _lib.lib().qmlp_mx_quantize(x.data_ptr(), x_type, stride, M, K, buf.data_ptr(), nbytes,
+                                             _lib.device_stream(device, stream))
         else:
-            _lib.check(_lib.lib().qmlp_mx_quantize_rmsnorm(_lib.ptr(x), stride, _lib.ptr(norm_weight), float(eps), M, K,
-                                                           _lib.ptr(buf), nbytes, _lib.stream_handle(stream)),
-                       "qmlp_mx_quantize_rmsnorm")
+            rc = _lib.lib().qmlp_mx_quantize_rmsnorm(x.data_ptr(), stride, norm_weight.data_ptr(), float(eps), M, K,
+                                                     buf.data_ptr(), nbytes, _lib.device_stream(device, stream))
+        _lib.check(rc, "quantize_mxfp4")
     return MxTensor(buf, M, K)
 
 
@@ -128,9 +135,10 @@ def _check_weight(w, name, K):
 def _activation(x):
     """(pointer, QMLP_X_* code, row stride, M, K, device) of an activation argument."""
     if isinstance(x, MxTensor):
-        return _lib.ptr(x.buf), _lib.X_MXFP4, 0, x.rows, x.cols, x.buf.device
-    x_type, stride = _check_rows(x, "x")
-    return _lib.ptr(x), x_type, stride, x.shape[0], x.shape[1], x.device
+        return x.buf.data_ptr(), _lib.X_MXFP4, 0, x.rows, x.cols, x.buf.device
+    x_type, stride = _check_rows(x)
+    M, K = x.shape
+    return x.data_ptr(), x_type, stride, M, K, x.device
 
 
 def _check_out(out, out_dtype, shape):
@@ -148,11 +156,18 @@ def _check_out(out, out_dtype, shape):
     return out.dtype
 
 
-def _workspace(M, N, K, device):
-    n = _lib.lib().qmlp_mx_workspace_bytes(M, N, K)
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(M, N, K, x_type):
+    return _lib.lib().qmlp_mx_workspace_bytes(M, N, K, x_type)
+
+
+def _workspace(M, N, K, x_type, device):
+    """(tensor that has to live until the call is enqueued, pointer, bytes); none where none is needed."""
+    n = _workspace_bytes(M, N, K, x_type)
     if n == 0:
-        raise ValueError(f"unsupported sizes M={M} N={N} K={K}")
-    return torch.empty(n, dtype=torch.uint8, device=device)
+        return None, None, 0
+    ws = torch.empty(n, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), n
 
 
 def mxfp4_linear(x, w, residual=None, out=None, out_dtype=None, stream=None):
@@ -179,10 +194,11 @@ def mxfp4_linear(x, w, residual=None, out=None, out_dtype=None, stream=None):
     with _lib.on_device(device, stream):
         if out is None:
             out = torch.empty(shape, dtype=dtype, device=device)
-        ws = _workspace(M, w.rows, K, device)
-        _lib.check(_lib.lib().qmlp_mx_linear(xp, x_type, stride, _lib.ptr(w.buf), _lib.ptr(residual), _lib.ptr(out),
-                                             _lib.ptr(ws), ws.numel(), M, w.rows, K, flags,
-                                             _lib.stream_handle(stream)), "qmlp_mx_linear")
+        ws, wp, wn = _workspace(M, w.rows, K, x_type, device)
+        rc = _lib.lib().qmlp_mx_linear(xp, x_type, stride, w.buf.data_ptr(),
+                                       None if residual is None else residual.data_ptr(), out.data_ptr(), wp, wn, M,
+                                       w.rows, K, flags, _lib.device_stream(device, stream))
+        _lib.check(rc, "mxfp4_linear")
     return out
 
 
@@ -215,8 +231,8 @@ def mxfp4_swiglu(x, w1, w3, out=None, out_dtype=None, quantize=False, stream=Non
             out = res.buf
         else:
             out = res = torch.empty((M, N), dtype=dtype, device=device) if out is None else out
-        ws = _workspace(M, N, K, device)
-        _lib.check(_lib.lib().qmlp_mx_swiglu(xp, x_type, stride, _lib.ptr(w1.buf), _lib.ptr(w3.buf), _lib.ptr(out),
-                                             _lib.ptr(ws), ws.numel(), M, N, K, flags, _lib.stream_handle(stream)),
-                   "qmlp_mx_swiglu")
+        ws, wp, wn = _workspace(M, N, K, x_type, device)
+        rc = _lib.lib().qmlp_mx_swiglu(xp, x_type, stride, w1.buf.data_ptr(), w3.buf.data_ptr(), out.data_ptr(), wp, wn,
+                                       M, N, K, flags, _lib.device_stream(device, stream))
+        _lib.check(rc, "mxfp4_swiglu")
     return res

@@ -11,6 +11,7 @@ import pytest
 import torch
 
 from oracle import mxfp4 as omx
+from test_mxfp4 import PLAN_SHAPES
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
@@ -224,6 +225,47 @@ def test_swiglu(pkg, cuda, M, N, K):
         q = pkg.mxfp4_swiglu(x, w1, w3, quantize=True)
         for a, b in zip(pkg.unpack_canonical(q), pkg.unpack_canonical(pkg.quantize_mxfp4(y))):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("nmat,M,N,K", PLAN_SHAPES)
+def test_every_planned_kernel(pkg, cuda, nmat, M, N, K):
+    """Each kernel that a plan can choose, whole and in K pieces; the reference is a float64 product on
+    the GPU of the dequantised operands (their quantisation is pinned above)."""
+    print(f"case plan nmat={nmat} {M}x{N}x{K}", flush=True)
+    dtype = DTYPES[(M + K) % 3]
+    g = torch.Generator(device=cuda).manual_seed(N)
+    x = torch.randn(M, K, generator=g, device=cuda).to(dtype)
+    t = pkg.quantize_mxfp4(x)
+    xd = pkg.dequantize(t).double()
+    ws, refs, errs = [], [], []
+    for _ in range(nmat):
+        codes = torch.randint(0, 256, (N, K // 2), generator=g, device=cuda, dtype=torch.uint8)
+        scales = torch.randint(116, 122, (N, K // 32), generator=g, device=cuda, dtype=torch.uint8)
+        ws.append(pkg.pack_canonical(codes, scales, "mxfp4"))
+        wd = pkg.dequantize(ws[-1]).double()
+        refs.append(xd @ wd.T)
+        errs.append(_sum_error(K, xd.abs() @ wd.abs().T))
+        del wd
+    if nmat == 1:
+        ref, err = refs[0], errs[0]
+        y = pkg.mxfp4_linear(x, ws[0], out_dtype=torch.float32)
+        r = torch.randn(M, N, generator=g, device=cuda)
+        z = pkg.mxfp4_linear(t, ws[0], residual=r)
+        full = ref + r.double()
+        assert ((z.double() - full).abs() <= err + 2.0 ** -8 * (full.abs() + err)).all()
+        assert torch.equal(pkg.mxfp4_linear(t, ws[0], out_dtype=torch.float32), y)
+    else:
+        (gt, u), (ge, ue) = refs, errs
+        s = gt * torch.sigmoid(gt)
+        ref = s * u
+        err = (1.1 * ge * (u.abs() + ue) + (s.abs() + 1.1 * ge) * ue + (8 + gt.abs()) * 2.0 ** -23 * ref.abs()) + 1e-37
+        y = pkg.mxfp4_swiglu(x, *ws, out_dtype=torch.float32)
+        if N % 256 == 0:
+            q = pkg.mxfp4_swiglu(t, *ws, quantize=True)
+            for a, b in zip(pkg.unpack_canonical(q), pkg.unpack_canonical(pkg.quantize_mxfp4(y))):
+                assert torch.equal(a, b)
+        assert torch.equal(pkg.mxfp4_swiglu(t, *ws), y.bfloat16())
+    assert ((y.double() - ref).abs() <= err).all()
 
 
 def test_rows_that_are_not_numbers_stay_in_their_row(pkg, cuda):

@@ -78,16 +78,65 @@ def test_workspaces_never_shrink_as_m_grows(pkg):
     lib = pkg.lib()
     Ms = list(range(1, 700)) + [1023, 1024, 2047, 2048, 2049, 65536]
     for N, K in ((5120, 17408), (17408, 5120), (100, 32), (1, 1056)):
-        sizes = [lib.qmlp_mx_workspace_bytes(M, N, K) for M in Ms]
-        assert sizes[0] > 0 and sizes == sorted(sizes)
+        for x_type in range(4):
+            sizes = [lib.qmlp_mx_workspace_bytes(M, N, K, x_type) for M in Ms]
+            assert sizes[Ms.index(33)] > 0 and sizes == sorted(sizes)
+            assert (sizes[Ms.index(32)] == 0) == (x_type == 3)
     for H, I in ((5120, 17408), (256, 256)):
         sizes = [lib.qmlp_workspace_bytes(M, H, I, pkg.FMT_MXFP4) for M in Ms]
         assert sizes[0] > 0 and sizes == sorted(sizes)
     assert lib.qmlp_workspace_bytes(16, 5120 + 32, 17408, pkg.FMT_MXFP4) == 0  # the block's sizes: multiples of 256
     for bad in ((0, 256, 256), (65537, 256, 256), (1, 0, 256), (1, 256, 48)):
-        assert lib.qmlp_mx_workspace_bytes(*bad) == 0
+        assert lib.qmlp_mx_workspace_bytes(*bad, 0) == 0
     # a 16-token forward fits the library's own scratch
     assert lib.qmlp_workspace_bytes(32, 5120, 17408, pkg.FMT_MXFP4) <= 33554432
+
+
+# ---------------------------------------------------------------- plans
+
+# (matrices, M, N, K): sizes whose plans take every kernel that the products launch, whole and with the K
+# range in pieces, and quantise inside and in front; the GPU tests run them all.
+PLAN_SHAPES = [(1, 33, 4277, 96), (1, 5, 65, 96), (1, 1, 65, 96), (1, 5, 73, 1056), (1, 1, 69, 1056), (1, 4, 300, 8480),
+               (1, 33, 4131, 1120), (1, 1107, 65, 96), (1, 36, 72, 21472), (1, 780, 4910, 544), (1, 2083, 67, 40384),
+               (1, 1725, 4622, 544), (1, 138, 7557, 12992), (1, 1968, 7205, 832), (1, 417, 5445, 29344),
+               (2, 34, 4352, 96), (2, 5, 256, 96), (2, 1, 256, 96), (2, 33, 4352, 2112), (2, 1029, 256, 96),
+               (2, 33, 256, 26688), (2, 291, 6912, 96), (2, 65, 2560, 13920), (2, 546, 6656, 96), (2, 132, 2048, 20288),
+               (2, 774, 6656, 96), (2, 202, 6656, 17088)]
+
+
+def _plan(pkg, nmat, M, N, K, cus=256):
+    out = (ctypes.c_int * 5)()
+    assert pkg.lib().qmlp_mx_plan(M, N, K, nmat, cus, out) == 0
+    return list(out)
+
+
+def test_plan_shapes_reach_every_kernel(pkg):
+    got = set()
+    for nmat, M, N, K in PLAN_SHAPES:
+        kind, ks, _, _, inside = _plan(pkg, nmat, M, N, K)
+        got.add((nmat, kind, ks > 1, inside))
+    want = {(n, k, False, 0) for n in (1, 2) for k in range(8) if (n, k) != (2, 1)}
+    want |= {(n, k, True, 0) for n in (1, 2) for k in range(4, 8)} | {(1, 1, False, 1), (1, 2, False, 1), (2, 2, False, 1)}
+    assert got == want
+
+
+@pytest.mark.parametrize("nmat", [1, 2])
+def test_plans_cover_the_outputs_and_fit(pkg, nmat):
+    for cus in (256, 304, 64, 1):
+        for N, K in ((5120, 17408), (17408, 5120), (1, 32), (33, 288), (1000, 1 << 20), (1 << 20, 64)):
+            for M in (*range(1, 70), 100, 129, 256, 777, 1024, 1025, 2048, 65536):
+                kind, ks, groups, kb, inside = _plan(pkg, nmat, M, N, K, cus)
+                units, feats = -(-K // 256), 32 if kind < 4 else 256 // nmat
+                toks = 64 * (kind - 3) if kind > 3 else 64 if kind == 3 else 32
+                tiles = -(-N // feats) * -(-M // toks)
+                assert groups == tiles * ks and 1 <= ks <= units and (kind > 3 or ks == 1)
+                assert kb * 1024 == (tiles * ks * 256 * toks * 4 if ks > 1 else 0) <= 64 << 20
+                assert kind < 4 or M > 32
+                assert inside == (M <= 4 and M * units <= 136) and not (inside and kind > 2)
+    out = (ctypes.c_int * 5)()
+    for bad in ((0, 256, 256, 1, 256), (1, 0, 256, 1, 256), (1, 256, 48, 1, 256), (1, 256, 256, 3, 256), (1, 256, 256, 1, 0)):
+        assert pkg.lib().qmlp_mx_plan(*bad, out) == E_SHAPE
+    assert pkg.lib().qmlp_mx_plan(1, 256, 256, 1, 256, None) == E_NULL
 
 
 # ---------------------------------------------------------------- refusals of the C entry points
@@ -112,8 +161,9 @@ def _swiglu(lib, x=X, xt=0, xs=256, w=W0, w1=W1, out=OUT, ws=WS, wsb=BIG, M=4, N
 @pytest.mark.parametrize("call", [_linear, _swiglu])
 def test_product_refusals(pkg, call):
     lib = pkg.lib()
-    for arg in ("x", "w", "out", "ws"):
+    for arg in ("x", "w", "out"):
         assert call(lib, **{arg: None}) == E_NULL
+    for arg in ("x", "w", "out", "ws"):
         assert call(lib, **{arg: P((1 << 40) + 8)}) == E_ALIGN
     for kw in ({"M": 0}, {"M": -1}, {"M": 65537}, {"N": 0}, {"N": -3}, {"K": 0}, {"K": 48}, {"N": 1 << 21},
                {"K": 1 << 21, "xs": 1 << 21}):
@@ -123,12 +173,12 @@ def test_product_refusals(pkg, call):
     for kw in ({"xs": 255}, {"xs": 260}, {"xs": -256}, {"xs": 258, "xt": 2}, {"xs": 1 << 50}):
         assert call(lib, **kw) == E_SHAPE, kw
     assert b"stride" in lib.qmlp_last_error()
-    need = lib.qmlp_mx_workspace_bytes(4, 256 if call is _swiglu else 64, 256)
-    assert call(lib, wsb=need - 1) == E_WORKSPACE
+    need = lib.qmlp_mx_workspace_bytes(40, 256 if call is _swiglu else 64, 256, 0)
+    assert call(lib, wsb=need - 1, M=40) == E_WORKSPACE and call(lib, ws=None, M=40) == E_NULL
     # out on x, on a weight, on the last strided row of x; the workspace on an argument
     assert call(lib, out=X) == E_SHAPE and call(lib, out=W0) == E_SHAPE
     assert call(lib, xs=1 << 20, out=P((1 << 32) + 3 * (2 << 20) + 16)) == E_SHAPE
-    assert call(lib, ws=X) == E_SHAPE and call(lib, ws=OUT) == E_SHAPE and call(lib, ws=W0) == E_SHAPE
+    assert all(call(lib, ws=at, M=40) == E_SHAPE for at in (X, OUT, W0))
     assert call(lib, xt=3, out=X) == E_SHAPE
 
 
@@ -139,7 +189,7 @@ def test_linear_residual_refusals(pkg):
     assert _linear(lib, res=OUT, flags=1) == E_SHAPE                # in place, out fp32 and residual bf16
     assert _linear(lib, res=OUT, flags=2) == E_SHAPE
     assert b"dtype" in lib.qmlp_last_error()
-    assert _linear(lib, res=WS) == E_SHAPE
+    assert _linear(lib, res=WS, M=40) == E_SHAPE
     assert _linear(lib, flags=4) == E_FORMAT                        # a packed output is the gate/up pair's
 
 
