@@ -5,11 +5,12 @@
 namespace qmlp {
 
 // Every candidate's time in microseconds, linear in what it does, and the cheapest one wins.  The
-// constants were fitted (non-negative least squares on the relative error) to 4600 measured (sizes,
-// candidate) points on 256 CUs: 16 shapes from N = 96 to 17408 and K = 512 to 17408 with one and two
-// matrices, 8 to 2048 tokens.  The plan they pick was on average 2.5 % (one matrix) and 1.3 % (two) slower
-// than the fastest measured one, at worst 32 % (10.0 against 7.6 us at 128 tokens of 3000 x 5120, where
-// streamed and tiled kernels meet).
+// constants were fitted (non-negative least squares, points near the fastest of their sizes weighing
+// most) to 5900 measured (sizes, candidate) points on 256 CUs: 16 shapes from N = 96 to 17408 and K = 512 to
+// 17408 with one and two matrices, 21 token counts from 8 to 2048 (for the streamed kernels the points of
+// matrices beyond 40 million values weigh six times).  The plan they pick was on average 1.9 % (one
+// matrix) and 1.3 % (two) slower than the fastest measured one, at worst 25 % (9.4 against 7.5 us at 96
+// tokens of 3000 x 5120, where streamed and tiled kernels meet).
 //
 // Streamed, per workgroup: launch and tail; units of K a wave takes in turn; all (32 features x token
 // group x unit) products of the launch and all weight units it reads, per CU; rounds of workgroups.
@@ -18,24 +19,27 @@ struct StreamCost {
   int waves, groups;  // token groups of 32 a workgroup
   double start, unit, product, weight, round;
 };
-constexpr StreamCost kStreamCost[] = {{kMxStream, 4, 1, 1.41, 0.861, 0.076, 0.182, 0.142},
-                                      {kMxStreamDeep, 4, 1, 1.47, 0.518, 0.085, 0.102, 0.303},
-                                      {kMxStreamLong, 8, 1, 1.07, 0.739, 0.112, 0.079, 0.728},
-                                      {kMxStreamWide, 8, 2, 0.39, 1.158, 0.154, 0.043, 1.482}};
-constexpr StreamCost kPairCost[] = {{kMxStream, 4, 1, 2.36, 0.920, 0.118, 0.268, 0.149},
-                                    {kMxStreamLong, 8, 1, 1.05, 0.668, 0.163, 0.308, 1.359},
-                                    {kMxStreamWide, 4, 2, 0.96, 0.519, 0.148, 0.393, 2.707}};
-// Tiled: launch; a tile's start and end; a unit of K of a tile, alone on its CU and by how many CUs are
-// busy (the shared power and bandwidth: on a full machine a unit takes half as long again), of which the
-// weights' part falls with the token blocks that share them; the sum launch and a MB of partial tiles.
+constexpr StreamCost kStreamCost[] = {{kMxStream, 4, 1, 1.15, 0.982, 0.062, 0.125, 0.187},
+                                      {kMxStreamDeep, 4, 1, 1.92, 0.343, 0.115, 0.066, 0.235},
+                                      {kMxStreamLong, 8, 1, 1.22, 0.461, 0.133, 0.029, 1.022},
+                                      {kMxStreamWide, 8, 2, 0.0, 0.862, 0.174, 0.006, 2.188}};
+constexpr StreamCost kPairCost[] = {{kMxStream, 4, 1, 2.26, 0.739, 0.222, 0.140, 0.0},
+                                    {kMxStreamLong, 8, 1, 0.76, 0.685, 0.252, 0.159, 1.407},
+                                    {kMxStreamWide, 4, 2, 0.20, 0.558, 0.219, 0.257, 3.209}};
+// Tiled: launch; a tile's start and end; a unit of K of a tile, alone on its CU, and by how many CUs are
+// busy with tokens (the shared power and bandwidth: on a full machine a unit takes 1.4 to 2.6 times as
+// long); the weights' part, which falls with the token blocks that share them; the sum launch and a MB
+// of partial tiles.
 struct TileCost {
   double start, round, unit, busy, weight, sum, mbyte;
 };
 constexpr TileCost kTileCost[2][4] = {
-    {{4.10, 0.171, 0.408, 0.197, 0.117, 2.65, 0.319}, {4.99, 0.540, 0.456, 0.307, 0.0, 2.46, 0.320},
-     {3.80, 2.460, 0.640, 0.372, 0.0, 2.66, 0.256}, {0.0, 6.968, 0.870, 0.400, 0.0, 3.16, 0.232}},
-    {{1.97, 1.892, 0.360, 0.227, 0.685, 5.20, 0.177}, {2.59, 2.480, 0.436, 0.379, 0.454, 3.86, 0.239},
-     {2.16, 3.695, 0.633, 0.506, 0.150, 4.04, 0.224}, {0.0, 6.789, 0.870, 0.494, 0.0, 4.10, 0.262}}};
+    {{2.72, 1.699, 0.412, 0.207, 0.161, 3.18, 0.229}, {2.25, 3.522, 0.415, 0.430, 0.126, 2.64, 0.241},
+     {3.24, 3.465, 0.483, 0.869, 0.0, 0.0, 0.0}, {0.0, 7.281, 0.663, 1.031, 0.0, 0.0, 0.0}},
+    {{1.50, 2.410, 0.378, 0.250, 0.499, 4.19, 0.169}, {1.25, 3.590, 0.394, 0.505, 0.522, 3.70, 0.217},
+     {1.78, 3.979, 0.476, 0.916, 0.296, 0.0, 0.0}, {0.59, 5.642, 0.638, 1.219, 0.218, 0.0, 0.0}}};
+// Tiles of more than two heights stay whole: split, they won nowhere.
+constexpr int kMostSplit = 2;
 constexpr int kPieces[] = {1, 2, 3, 4, 6, 8, 12};
 constexpr int kMostStreamed = 1024;  // tokens: beyond, the tiles win at every measured shape
 
@@ -64,14 +68,16 @@ MxPlan mx_plan(int M, int N, int K, int nmat, int num_cus) {
   for (int h = 1; h <= 4; ++h) {
     const TileCost& c = kTileCost[nmat - 1][h - 1];
     const long ntt = up(M, 64 * h), tiles = up(N, 256 / nmat) * ntt;
+    const double filled = (double)up(M, 32) / (double)(ntt * 2 * h);  // token units that hold tokens
     for (int ks : kPieces) {
-      if (ks > nsb) break;
+      if (ks > nsb || (ks > 1 && h > kMostSplit)) break;
       const long pieces = tiles * ks, full = pieces / num_cus, rest = pieces % num_cus, units = up(nsb, ks);
       const size_t bytes = ks > 1 ? (size_t)pieces * 256 * 64 * h * 4 : 0;
       if (bytes > kMxPartBytes) break;
       const double turns = full + (rest ? 1 : 0), busy = full + rest / cus;
-      const double us = c.start + c.round * turns + units * (c.unit * turns + c.busy * busy + c.weight * busy / ntt) +
-                        (ks > 1 ? c.sum + c.mbyte * (double)bytes * 1e-6 : 0.0);
+      const double us = c.start + c.round * turns +
+                        units * (c.unit * turns + c.busy * busy * filled + c.weight * busy / ntt) +
+                        (ks > 1 ? c.sum + c.mbyte * (double)bytes * 1e-6 * filled : 0.0);
       if (us < best_us) {
         best_us = us;
         best = MxPlan{kMxTiles, h, ks, (int)pieces, bytes};

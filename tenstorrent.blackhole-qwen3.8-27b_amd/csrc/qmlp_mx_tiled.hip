@@ -3,6 +3,7 @@
 #include <atomic>
 #include <type_traits>
 
+#include "../../include/qwen_mlp.h"
 #include "qmlp_internal.h"
 #include "qmlp_mx.h"
 #include "qmlp_xcd.h"
@@ -177,10 +178,14 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
     else if (k < WF + WT)
       fs_next[k - WT] = *(const uint32_t*)(s + (wf * WF + k - WT) * 256);
   };
+  // Token units of this wave that hold tokens (none where its features lie behind the last one): the
+  // last tokens' tile does no product that no output needs.
+  const int mine_f = (ft * (T::kFeatUnits / NMAT) + wf * (WF / NMAT)) < ftiles ? WT : 0;
+  const int nv = max(0, min(mine_f, ttiles - (tt * T::kTokUnits + wt * WT)));
   // One K-step's products, in groups of two; before each group `beside(group)` asks for what comes in
   // beside them (the order is kept as written).
   constexpr int kGroups = WF * WT / 2;
-  auto multiply = [&](auto jc, auto beside) {
+  auto multiply = [&](auto jc, auto full, auto beside) {
     constexpr int J = decltype(jc)::value;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
@@ -188,7 +193,8 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
 #pragma unroll
       for (int k = 2 * g; k < 2 * g + 2; ++k) {
         const int f = k / WT, t = k % WT;
-        acc[f][t] = mx_product<J>(a[J & 1][f], b[J & 1][t], acc[f][t], fs[f], xs[t]);
+        if (decltype(full)::value || t < nv)
+          acc[f][t] = mx_product<J>(a[J & 1][f], b[J & 1][t], acc[f][t], fs[f], xs[t]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -205,28 +211,28 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
   // barrier inside half i has shown that every wave has read its last operands.  That barrier also
   // shows that half i + 1 is in LDS; the two after it may still be under way.
   // LEFT: K units behind this one, at most 2.
-  auto unit = [&](int sb, auto left) {
+  auto unit = [&](int sb, auto left, auto full) {
     constexpr int LEFT = decltype(left)::value;
     constexpr int kAhead = T::kMine * 5;  // loads of two halves, one of them with scales
 #pragma unroll
     for (int t = 0; t < WT; ++t) xs[t] = xs_next[t];
 #pragma unroll
     for (int f = 0; f < WF; ++f) fs[f] = fs_next[f];
-    multiply(std::integral_constant<int, 0>{}, [&](int g) {
+    multiply(std::integral_constant<int, 0>{}, full, [&](int g) {
       spread(g, WF + WT, [&](int k) { fetch(sb, 0, 1, k); });
       if constexpr (LEFT >= 1) spread(g, 2 * kPart1, [&](int k) { issue(sb + 1, 1, 1, k); });
     });
     stage_barrier<(LEFT >= 1 ? kAhead : 0)>();
-    multiply(std::integral_constant<int, 1>{}, [&](int g) {
+    multiply(std::integral_constant<int, 1>{}, full, [&](int g) {
       spread(g, WF + WT, [&](int k) { fetch(sb, 1, 0, k); });
       if constexpr (LEFT >= 2) spread(g, 3 * kPart0, [&](int k) { issue(sb + 2, 0, 0, k); });
     });
-    multiply(std::integral_constant<int, 2>{}, [&](int g) {
+    multiply(std::integral_constant<int, 2>{}, full, [&](int g) {
       spread(g, WF + WT, [&](int k) { fetch(sb, 1, 1, k); });
       if constexpr (LEFT >= 2) spread(g, 3 * kPart1, [&](int k) { issue(sb + 2, 0, 1, k); });
     });
     stage_barrier<(LEFT >= 2 ? kAhead : 0)>();
-    multiply(std::integral_constant<int, 3>{}, [&](int g) {
+    multiply(std::integral_constant<int, 3>{}, full, [&](int g) {
       if constexpr (LEFT >= 1) {
         spread(g, WF + WT, [&](int k) { fetch(sb + 1, 0, 0, k); });
         spread(g, WF + WT, [&](int k) { fetch_scale(sb + 1, k); });
@@ -251,12 +257,18 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
     fetch_scale(0, k);
     fetch(0, 0, 0, k);
   }
-  int sb = 0;
-  for (; sb + 2 < n; ++sb) unit(sb, std::integral_constant<int, 2>{});
-  if (sb + 1 < n) unit(sb++, std::integral_constant<int, 1>{});
-  unit(sb, std::integral_constant<int, 0>{});
+  auto units = [&](auto full) {
+    int sb = 0;
+    for (; sb + 2 < n; ++sb) unit(sb, std::integral_constant<int, 2>{}, full);
+    if (sb + 1 < n) unit(sb++, std::integral_constant<int, 1>{}, full);
+    unit(sb, std::integral_constant<int, 0>{}, full);
+  };
+  if (nv == WT)
+    units(std::true_type{});
+  else
+    units(std::false_type{});
   constexpr int per = WF / NMAT;
-  if (ks > 1) {  // the sums as the lanes hold them; mx_sum_kernel adds the pieces up
+  if (WT <= 2 && ks > 1) {  // the sums as the lanes hold them; mx_sum_kernel adds the pieces up
     f32x4* at = parts + ((size_t)piece * T::kWaves + wave) * (WF * WT * 4 * 64) + lane;
 #pragma unroll
     for (int f = 0; f < WF; ++f)
@@ -264,7 +276,7 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
       for (int t = 0; t < WT; ++t)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          at[((f * WT + t) * 4 + k) * 64] =
+          if (t < nv) at[((f * WT + t) * 4 + k) * 64] =
               f32x4{acc[f][t][4 * k], acc[f][t][4 * k + 1], acc[f][t][4 * k + 2], acc[f][t][4 * k + 3]};
     return;
   }
@@ -273,6 +285,7 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
   if constexpr (MODE != kMxPacked) __syncthreads();  // the stages' readers are done
 #pragma unroll
   for (int t = 0; t < WT; ++t) {
+    if (t >= nv) break;
 #pragma unroll
     for (int f = 0; f < per; ++f) {
       f32x4 v[NMAT][4];
@@ -299,6 +312,9 @@ __global__ __launch_bounds__(256) void mx_sum_kernel(const f32x4* __restrict__ p
   const int item = blockIdx.x * 4 + (threadIdx.x >> 6), tile = item / kItems, r = item % kItems;
   if (tile >= tiles) return;
   const int wave = r / (per * WT), f = r / WT % per, t = r % WT;
+  const int wf = wave % NF, wt = wave / NF, ft = tile / ntt, tt = tile % ntt;
+  const int tok = tt * T::kTokUnits + wt * WT + t, feat = ft * (T::kFeatUnits / NMAT) + wf * per + f;
+  if (tok >= mx_row_tiles(o.M) || feat >= mx_row_tiles(o.N)) return;  // left out by the product
   f32x4 v[NMAT][4];
 #pragma unroll
   for (int m = 0; m < NMAT; ++m)
@@ -312,9 +328,7 @@ __global__ __launch_bounds__(256) void mx_sum_kernel(const f32x4* __restrict__ p
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[m][k] += at[(((f + m * per) * WT + t) * 4 + k) * 64];
   }
-  const int wf = wave % NF, wt = wave / NF, ft = tile / ntt, tt = tile % ntt;
-  mx_finish<NMAT, MODE>(o, tt * T::kTokUnits + wt * WT + t, ft * (T::kFeatUnits / NMAT) + wf * per + f, lane,
-                        s_turn[threadIdx.x >> 6], v);
+  mx_finish<NMAT, MODE>(o, tok, feat, lane, s_turn[threadIdx.x >> 6], v);
 }
 
 template <typename T, int NMAT, int MODE, int WF, int WT, int NF, int NT>
@@ -347,10 +361,15 @@ static int launch_tile(const MxProduct& p, int ks, hipStream_t s) {
   if (int rc = raise_lds_once(kern, T::kLds, raised)) return rc;
   const int nft = (p.o.N + T::kFeatures - 1) / T::kFeatures, ntt = (p.o.M + T::kTokens - 1) / T::kTokens;
   const int tiles = nft * ntt;
+  if (ks > 1 && (WT > 2 || (size_t)tiles * ks * (T::kWaves * WF * WT * 4096) > kMxPartBytes))  // never planned
+    return set_error(QMLP_E_WORKSPACE, "mx_tiled_kernel: %d tiles in %d pieces", tiles, ks);
   launch_timed_part(p.slot, ks > 1 ? 1 : 3, kern, dim3(tiles * ks), dim3(T::kWaves * 64), T::kLds, s, p.x, p.w0, p.w1,
                     mx_ksb(p.K), ntt, ks, (f32x4*)p.parts, p.o);
   if (int rc = check_launch("mx_tiled_kernel")) return rc;
-  return ks == 1 ? 0 : launch_sum<T, NMAT, MODE, WF, WT, NF, NT>(p, tiles, ntt, ks, s);
+  if constexpr (WT <= 2) {  // mx_plan splits no higher tile
+    if (ks > 1) return launch_sum<T, NMAT, MODE, WF, WT, NF, NT>(p, tiles, ntt, ks, s);
+  }
+  return 0;
 }
 
 template <int MODE>
