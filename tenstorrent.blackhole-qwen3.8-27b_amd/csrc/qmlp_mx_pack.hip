@@ -23,7 +23,8 @@ __device__ __forceinline__ MxItem mx_item(int tid) {
 
 // ---------------------------------------------------------------- quantisation
 //
-// Bound by memory for many rows (2 or 4 bytes read and 17/32 written per value), by latency for few.
+// Bound by memory for many rows (2 or 4 bytes read and 17/32 written per value: 2048 x 17408 bf16 in 14.6-16.3
+// us, 5.5-6.2 TB/s), by latency for few (one row of 5120: 2.4-2.6 us).
 // R groups of 8 rows keep R 16-byte loads of a thread in flight.  The scale bytes of a workgroup
 // gather in LDS, so that they leave as whole dwords.  Rows [rows, fill_rows) are written as zeros
 // (weights, whose packed bytes depend on the weights alone); bad (weights): count of blocks that hold
@@ -97,7 +98,8 @@ int launch_mx_quantize(const void* x, int type, size_t row_bytes, int rows, int 
 //
 // The decoder's zero-centred norm, n = bf16(x * (1 / sqrt(mean(x^2) + eps)) * (1 + w)), then n's blocks.
 // One workgroup per row, the sums in rows_kernel's order, so that the result is that of the norm pass
-// followed by the quantisation, bit for bit.  REGS: rows of up to 8192 values stay in registers.
+// followed by the quantisation, bit for bit.  Bound by latency (a row's load, a reduction, its store):
+// 3.4-4.5 us at 16 rows of 5120.  REGS: rows of up to 8192 values stay in registers.
 constexpr int kNormCh = 4;
 template <bool REGS>
 __global__ __launch_bounds__(kQThreads) void mx_norm_quantize_kernel(const uint8_t* __restrict__ x, size_t row_bytes,
@@ -246,7 +248,7 @@ int launch_mx_unpack(const void* packed, int rows, int cols, void* codes, void* 
 //
 // Packed -> bf16 or fp32 values, exactly: a code has two significant bits, and 2^-128, the smallest
 // magnitude (scale byte 0, which packed checkpoints may hold), is a bf16 number too.  Bound by the
-// write; the thread mapping is the quantiser's.
+// write (2048 x 17408 to bf16 in 16.1-18.1 us, 5.0-5.6 TB/s); the thread mapping is the quantiser's.
 template <bool F32, int R>
 __global__ __launch_bounds__(kQThreads) void mx_dequantize_kernel(const uint8_t* __restrict__ packed, int rows,
                                                                  int cols, uint8_t* __restrict__ out) {

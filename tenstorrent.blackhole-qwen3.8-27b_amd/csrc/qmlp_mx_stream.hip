@@ -1,5 +1,18 @@
-// qmlp_mx_stream.hip -- MXFP4 products: packed weights times packed activations, one workgroup per 32
-// features x 32 tokens (layout: qmlp_mx.h).
+// qmlp_mx_stream.hip -- MXFP4 products of few tokens: one workgroup per 32 features x 32 (or 64) tokens
+// (layout: qmlp_mx.h).
+//
+// Bound by the weights: 17/32 byte each, read once.  A lane's 16-byte load is an operand of the scaled
+// 32x32x64 product as it comes, so a wave does nothing but load and multiply (a CU's matrix cores could
+// take 128 B a cycle, its share of the memory is 13), and one or two K units (4352 B of each matrix) a
+// wave, 5 to 9 waves a CU, keep 11-19 MB under way on the card.  With M <= 4 (and few enough values) x is
+// quantised by the workgroups themselves, which saves a launch.  Weights pass the caches by
+// (non-temporal): eight layers' in turn, 47 MB each, take 11.4 us instead of 12.0; three, which the
+// memory-side cache holds, 11.1 instead of 9.2.
+// Measured (eight matrices in turn): 5120 x 17408 one token 11.4 us (4.2 TB/s), 17408 x 5120 16 tokens
+// 11.9 (4.0 TB/s), two of them one token 19.4 (4.9 TB/s); reading the same bytes and nothing else takes
+// 8.7 and 15.7 us.  The token operands come from the L2 with the weights' loads; staged in LDS first they
+// cost 0.7 us less at 5120 x 17408 and one token, and 1.7 to 4 us more at 17408 x 5120 and 16.  Half units
+// as the waves' steps, which share K out more evenly, read the scales twice: 12.8-14.2 us for 11.5.
 #include "qmlp_internal.h"
 #include "qmlp_mx.h"
 
@@ -156,40 +169,40 @@ __global__ __launch_bounds__(WAVES * 64) void mx_stream_kernel(const uint8_t* __
     __syncthreads();
   }
   for (int item = threadIdx.x; item < MG * 256; item += WAVES * 64) {
-  const int g = item >> 8, t = (item >> 3) & 31, f = (item & 7) * 4, tt = tt0 + g;
-  f32x4 sum[NMAT];
+    const int g = item >> 8, t = (item >> 3) & 31, f = (item & 7) * 4, tt = tt0 + g;
+    f32x4 sum[NMAT];
 #pragma unroll
-  for (int n = 0; n < NMAT; ++n) {
-    sum[n] = *(const f32x4*)&s_part[n][g][0][t * kRow + f];
+    for (int n = 0; n < NMAT; ++n) {
+      sum[n] = *(const f32x4*)&s_part[n][g][0][t * kRow + f];
 #pragma unroll
-    for (int w = 1; w < kHalfWaves; ++w) sum[n] += *(const f32x4*)&s_part[n][g][w][t * kRow + f];
-  }
-  const int m = tt * 32 + t, n0 = ft * 32 + f;
-  if constexpr (MODE == kMxRowsOut) {
-    mx_store4(o, m, n0, sum[0]);
-  } else {
-    f32x4 h;
+      for (int w = 1; w < kHalfWaves; ++w) sum[n] += *(const f32x4*)&s_part[n][g][w][t * kRow + f];
+    }
+    const int m = tt * 32 + t, n0 = ft * 32 + f;
+    if constexpr (MODE == kMxRowsOut) {
+      mx_store4(o, m, n0, sum[0]);
+    } else {
+      f32x4 h;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = silu_mul(sum[0][i], sum[NMAT - 1][i]);
-    if constexpr (MODE == kMxGated) {
-      mx_store4(o, m, n0, h);
-    } else {  // the 32 features of a token are one block, in 8 neighbouring lanes
-      uint32_t mx = 0u;
+      for (int i = 0; i < 4; ++i) h[i] = silu_mul(sum[0][i], sum[NMAT - 1][i]);
+      if constexpr (MODE == kMxGated) {
+        mx_store4(o, m, n0, h);
+      } else {  // the 32 features of a token are one block, in 8 neighbouring lanes
+        uint32_t mx = 0u;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mx = max(mx, __float_as_uint(h[i]) & 0x7fffffffu);
+        for (int i = 0; i < 4; ++i) mx = max(mx, __float_as_uint(h[i]) & 0x7fffffffu);
 #pragma unroll
-      for (int d = 1; d < 8; d <<= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, d));
-      const uint32_t s = mx_scale_byte(mx);
-      const uint32_t c = mx_codes4(h, s);
-      const uint32_t hi = (uint32_t)__shfl_xor((int)c, 1);
-      if (m < o.M) {
-        uint8_t* unit = (uint8_t*)o.out + ((size_t)tt * mx_ksb(o.N) + n0 / kMxK) * kMxUnit;
-        const int kb = (n0 % kMxK) / kMxBlock;
-        if ((item & 1) == 0) *(uint32_t*)(unit + (kb * 32 + t) * 16 + f / 2) = c | (hi << 16);
-        if ((item & 7) == 0) unit[kMxCodes + 4 * (t + 32 * (kb & 1)) + (kb >> 1)] = (uint8_t)s;
+        for (int d = 1; d < 8; d <<= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, d));
+        const uint32_t s = mx_scale_byte(mx);
+        const uint32_t c = mx_codes4(h, s);
+        const uint32_t hi = (uint32_t)__shfl_xor((int)c, 1);
+        if (m < o.M) {
+          uint8_t* unit = (uint8_t*)o.out + ((size_t)tt * mx_ksb(o.N) + n0 / kMxK) * kMxUnit;
+          const int kb = (n0 % kMxK) / kMxBlock;
+          if ((item & 1) == 0) *(uint32_t*)(unit + (kb * 32 + t) * 16 + f / 2) = c | (hi << 16);
+          if ((item & 7) == 0) unit[kMxCodes + 4 * (t + 32 * (kb & 1)) + (kb >> 1)] = (uint8_t)s;
+        }
       }
     }
-  }
   }
 }
 

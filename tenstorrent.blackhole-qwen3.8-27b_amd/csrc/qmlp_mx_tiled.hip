@@ -1,5 +1,20 @@
-// qmlp_mx_tiled.hip -- MXFP4 products of many tokens: both operands staged through LDS (layout:
-// qmlp_mx.h).
+// qmlp_mx_tiled.hip -- MXFP4 products of many tokens (layout: qmlp_mx.h).
+//
+// out^T[features, tokens] = W x^T in 256 features (128 of gate and of up) x 64, 128, 192 or 256 tokens a
+// workgroup of 8 waves, on the scaled 32x32x64 product, which takes codes and scale bytes as they lie in
+// memory: 32 cycles for 131072 flop, 10 PFLOP/s at 2.4 GHz.  Per K unit a 256 x 256 tile reads 69.6 KB
+// and multiplies for 2048 cycles of each SIMD, so what costs is moving operands about:
+//   * memory -> LDS by loads that bypass the registers: the packed layout is the products' operand
+//     order, so a unit comes in as it lies, and LDS is read lane by lane (no conflicts, no swizzle);
+//   * LDS holds four halves (128 K) of a K unit, so that a load has two of them, 2000 cycles and more,
+//     to arrive; one workgroup takes a CU;
+//   * the operands of a K-step are read while the products of the one before run, one or two reads to a
+//     pair of products, in the order written here.
+// Measured (256 tiles of 256 x 256, K = 17408, random codes): 126-131 us, 4.5-4.6 PFLOP/s; without the
+// loads into LDS 110-130, without the LDS reads 105-120, without both 94-104, while the clock goes from
+// 1.70 to 1.81, 1.93 and 2.12 GHz at 64-70 % busy matrix cores: the clock falls as more data moves, so
+// power, and not a unit, bounds it.  Products from registers alone reach 6.1-6.5 PFLOP/s on random codes
+// (8.1-8.8 on constant ones).  Four waves of 128 x 128, which read a third less from LDS, took 127-129 us.
 #include <atomic>
 #include <type_traits>
 
@@ -37,10 +52,16 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// The lanes of a wave see each other's LDS accesses in program order; this keeps the compiler to it.
+__device__ __forceinline__ void turn_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // Finishes 32 features x 32 tokens from the matrices' sums as the product leaves them: lane: token lane %
 // 32, v[.][k][i]: feature 8 k + 4 (lane / 32) + i.  Rows go through `turn`, kMxTurn floats of LDS that
-// belong to the wave, so that 8 lanes write 32 features of a token together: written as the product
-// leaves them, 16 bytes here and there, a tile's output took 3 us more.
+// belong to the wave, so that 8 lanes write 32 features of a token together: 2048 x 17408 x 512 took
+// 24.5 us; written as the product leaves them, 16 bytes here and there, 34.6.
 constexpr int kMxTurnRow = 36;  // floats of a token's row: 8 lanes' 16-byte accesses meet no bank twice
 constexpr int kMxTurn = 32 * kMxTurnRow;
 template <int NMAT, int MODE>
@@ -55,14 +76,14 @@ __device__ __forceinline__ void mx_finish(const MxOut& o, int tok_unit, int feat
   if constexpr (MODE != kMxPacked) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) *(f32x4*)(turn + row * kMxTurnRow + 8 * k + 4 * half) = y[k];
-    __builtin_amdgcn_wave_barrier();  // a wave's LDS accesses are done in order: none moves past here
+    turn_fence();
     const int r = lane >> 3, f = (lane & 7) * 4;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const f32x4 w = *(const f32x4*)(turn + (8 * k + r) * kMxTurnRow + f);
       mx_store4(o, tok_unit * 32 + 8 * k + r, feat_unit * 32 + f, w);
     }
-    __builtin_amdgcn_wave_barrier();
+    turn_fence();
   } else {  // a token's 32 features are one block, in lanes l and l + 32
     uint32_t mx = 0u;
 #pragma unroll
@@ -276,8 +297,9 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
       for (int t = 0; t < WT; ++t)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (t < nv) at[((f * WT + t) * 4 + k) * 64] =
-              f32x4{acc[f][t][4 * k], acc[f][t][4 * k + 1], acc[f][t][4 * k + 2], acc[f][t][4 * k + 3]};
+          if (t < nv)
+            at[((f * WT + t) * 4 + k) * 64] = f32x4{acc[f][t][4 * k], acc[f][t][4 * k + 1], acc[f][t][4 * k + 2],
+                                                    acc[f][t][4 * k + 3]};
     return;
   }
   static_assert(T::kLds >= T::kWaves * kMxTurn * 4);
@@ -301,7 +323,9 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
   }
 }
 
-// Adds the pieces of split tiles up, in K order, and finishes them: one wave for 32 features x 32 tokens.
+// Adds the pieces of split tiles up, in K order (deterministic), and finishes them: one wave for 32
+// features x 32 tokens.  Bound by its reads and its launch: 4.1-4.8 us for 15.7 MB of pieces (201 tokens of
+// 5120 x 8704).  A launch of its own, so that every CU takes part and no block waits for another.
 template <int NMAT, int WF, int WT, int NF, int NT, int MODE>
 __global__ __launch_bounds__(256) void mx_sum_kernel(const f32x4* __restrict__ parts, int tiles, int ntt, int ks,
                                                      MxOut o) {
@@ -361,7 +385,8 @@ static int launch_tile(const MxProduct& p, int ks, hipStream_t s) {
   if (int rc = raise_lds_once(kern, T::kLds, raised)) return rc;
   const int nft = (p.o.N + T::kFeatures - 1) / T::kFeatures, ntt = (p.o.M + T::kTokens - 1) / T::kTokens;
   const int tiles = nft * ntt;
-  if (ks > 1 && (WT > 2 || (size_t)tiles * ks * (T::kWaves * WF * WT * 4096) > kMxPartBytes))  // never planned
+  const size_t part_bytes = (size_t)tiles * ks * (T::kWaves * WF * WT * 4096);
+  if (ks > mx_ksb(p.K) || (ks > 1 && (WT > 2 || part_bytes > kMxPartBytes)))  // never planned
     return set_error(QMLP_E_WORKSPACE, "mx_tiled_kernel: %d tiles in %d pieces", tiles, ks);
   launch_timed_part(p.slot, ks > 1 ? 1 : 3, kern, dim3(tiles * ks), dim3(T::kWaves * 64), T::kLds, s, p.x, p.w0, p.w1,
                     mx_ksb(p.K), ntt, ks, (f32x4*)p.parts, p.o);

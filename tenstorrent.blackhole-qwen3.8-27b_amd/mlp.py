@@ -15,6 +15,7 @@ Errors: ``ValueError`` for wrong shape/dtype/device (as ``FusedProjection.__call
 ``scripts/ci/fused_1d.py:124-128``), ``QmlpError`` for launch failures.  There is no CPU fallback.
 """
 import ctypes
+import functools
 import os
 from dataclasses import dataclass
 
@@ -154,6 +155,23 @@ def _unsupported_shape(rows, cols, fmt):
     return ValueError(f"unsupported shape {rows}x{cols}: rows must be a multiple of 16 and cols of 256")
 
 
+@functools.lru_cache(maxsize=4096)
+def _mxfp4_bytes(rows, cols):
+    n = _lib.lib().qmlp_packed_bytes(rows, cols, _lib.FMT_MXFP4)
+    if n == 0:
+        raise _unsupported_shape(rows, cols, "mxfp4")
+    return n
+
+
+def _check_mxfp4_buffer(t, name):
+    """The packed buffer of an mxfp4 weight or ``MxTensor`` is what its shape needs."""
+    buf = t.buf
+    if not (isinstance(buf, torch.Tensor) and buf.is_cuda):
+        raise ValueError(f"{name} must be on the GPU")
+    if buf.dtype != torch.uint8 or not buf.is_contiguous() or buf.numel() < _mxfp4_bytes(t.rows, t.cols):
+        raise ValueError(f"{name}: the buffer does not hold a packed mxfp4 [{t.rows}, {t.cols}]")
+
+
 def _pack_canonical_mxfp4(codes, scales, stream):
     _check_device_tensor(codes, "q", torch.uint8)
     _check_device_tensor(scales, "e8", torch.uint8)
@@ -164,9 +182,7 @@ def _pack_canonical_mxfp4(codes, scales, stream):
         raise ValueError("e8 must be [rows, cols/32]")
     if scales.device != codes.device:
         raise ValueError("q and e8 must be on the same GPU")
-    nbytes = _lib.lib().qmlp_packed_bytes(rows, cols, _lib.FMT_MXFP4)
-    if nbytes == 0:
-        raise _unsupported_shape(rows, cols, "mxfp4")
+    nbytes = _mxfp4_bytes(rows, cols)
     with _lib.on_device(codes.device, stream):
         buf = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
         _lib.check(_lib.lib().qmlp_pack(_lib.ptr(codes), _lib.ptr(scales), rows, cols, _lib.FMT_MXFP4, _lib.ptr(buf),
@@ -225,6 +241,7 @@ def unpack_canonical(pw, stream=None):
     """Packed bfp8 or bf4 -> canonical (q, e8) (lossless for unflushed groups); packed mxfp4 (a weight
     or an ``MxTensor``) -> (codes, scales) (lossless)."""
     if pw.fmt == "mxfp4":
+        _check_mxfp4_buffer(pw, "the tensor")
         with _lib.on_device(pw.buf.device, stream):
             codes = torch.empty((pw.rows, pw.cols // 2), dtype=torch.uint8, device=pw.buf.device)
             scales = torch.empty((pw.rows, pw.cols // 32), dtype=torch.uint8, device=pw.buf.device)
@@ -248,6 +265,7 @@ def dequantize(pw, stream=None, dtype=torch.float32):
     if pw.fmt == "mxfp4":
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("dtype must be bf16 or fp32")
+        _check_mxfp4_buffer(pw, "the tensor")
         with _lib.on_device(pw.buf.device, stream):
             out = torch.empty((pw.rows, pw.cols), dtype=dtype, device=pw.buf.device)
             rc = _lib.lib().qmlp_mx_dequantize(pw.buf.data_ptr(), pw.rows, pw.cols, out.data_ptr(),

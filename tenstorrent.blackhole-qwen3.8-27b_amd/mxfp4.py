@@ -26,7 +26,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .mlp import PackedWeight, _check_device_tensor
+from .mlp import PackedWeight, _check_device_tensor, _check_mxfp4_buffer, _mxfp4_bytes
 
 _X_TYPES = {torch.bfloat16: _lib.X_BF16, torch.float16: _lib.X_F16, torch.float32: _lib.X_F32}
 
@@ -83,14 +83,6 @@ def _check_rows(x):
     return x_type, stride
 
 
-@functools.lru_cache(maxsize=4096)
-def _packed_bytes(rows, cols):
-    n = _lib.lib().qmlp_packed_bytes(rows, cols, _lib.FMT_MXFP4)
-    if n == 0:
-        raise ValueError(f"unsupported shape {rows}x{cols}: cols must be a multiple of 32")
-    return n
-
-
 def quantize_mxfp4(x, norm_weight=None, eps=1e-6, stream=None):
     """bf16, fp16 or fp32 ``[M, K]`` GPU tensor (rows may be strided) -> ``MxTensor``.
 
@@ -106,7 +98,7 @@ def quantize_mxfp4(x, norm_weight=None, eps=1e-6, stream=None):
         if tuple(norm_weight.shape) != (K,):
             raise ValueError(f"norm_weight must have shape ({K},)")
         _same_device(x.device, norm_weight=norm_weight)
-    device, nbytes = x.device, _packed_bytes(M, K)
+    device, nbytes = x.device, _mxfp4_bytes(M, K)
     with _lib.on_device(device, stream):
         buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
         if norm_weight is None:
@@ -123,6 +115,13 @@ def _same_device(device, **tensors):
     for name, t in tensors.items():
         if t is not None and t.device != device:
             raise ValueError(f"{name} is on {t.device}, x on {device}")
+
+
+def _check_buffers(x, **weights):
+    if isinstance(x, MxTensor):
+        _check_mxfp4_buffer(x, "x")
+    for name, w in weights.items():
+        _check_mxfp4_buffer(w, name)
 
 
 def _check_weight(w, name, K):
@@ -190,6 +189,7 @@ def mxfp4_linear(x, w, residual=None, out=None, out_dtype=None, stream=None):
             raise ValueError(f"residual must have shape {shape}")
         if residual.dtype == torch.float32:
             flags |= _lib.RESIDUAL_F32
+    _check_buffers(x, w=w)
     _same_device(device, w=w.buf, residual=residual, out=out)
     with _lib.on_device(device, stream):
         if out is None:
@@ -224,10 +224,11 @@ def mxfp4_swiglu(x, w1, w3, out=None, out_dtype=None, quantize=False, stream=Non
     else:
         dtype = _check_out(out, out_dtype, (M, N))
         flags = _lib.OUT_F32 if dtype == torch.float32 else 0
+    _check_buffers(x, w1=w1, w3=w3)
     _same_device(device, w1=w1.buf, w3=w3.buf, out=out)
     with _lib.on_device(device, stream):
         if quantize:
-            res = MxTensor(torch.empty(_packed_bytes(M, N), dtype=torch.uint8, device=device), M, N)
+            res = MxTensor(torch.empty(_mxfp4_bytes(M, N), dtype=torch.uint8, device=device), M, N)
             out = res.buf
         else:
             out = res = torch.empty((M, N), dtype=dtype, device=device) if out is None else out

@@ -308,6 +308,24 @@ def test_misfits_are_refused(pkg, cuda):
             pkg.mxfp4_linear(t, w, **kw)
     with pytest.raises(ValueError):
         pkg.mxfp4_linear(x[:, :128], w)
+    with pytest.raises(ValueError, match="columns"):
+        pkg.mxfp4_linear(t, pkg.pack_weight(torch.ones(64, 288, dtype=torch.bfloat16, device=cuda), "mxfp4"))
+    narrow = pkg.pack_weight(torch.ones(32, 256, dtype=torch.bfloat16, device=cuda), "mxfp4")
+    with pytest.raises(ValueError, match="rows"):
+        pkg.mxfp4_swiglu(t, w, narrow)
+    with pytest.raises(ValueError, match="256"):
+        pkg.mxfp4_swiglu(t, w, w, quantize=True)
+    with pytest.raises(ValueError, match="quantize"):
+        pkg.mxfp4_swiglu(t, w, w, quantize=True, out_dtype=torch.float32)
+    with pytest.raises(ValueError, match="out_dtype"):
+        pkg.mxfp4_linear(t, w, out_dtype=torch.float16)
+    for short in (pkg.MxTensor(t.buf, 33, 256), pkg.MxTensor(t.buf[16:], 4, 256), pkg.MxTensor(t.buf.view(torch.int8), 4, 256),
+                  pkg.MxTensor(t.buf, 0, 256), pkg.MxTensor(t.buf, 4, 48)):  # a buffer that is not the shape's
+        for f in (pkg.dequantize, pkg.unpack_canonical, lambda v: pkg.mxfp4_linear(v, w)):
+            with pytest.raises(ValueError):
+                f(short)
+    with pytest.raises(ValueError):
+        pkg.mxfp4_linear(t, pkg.PackedWeight(w.buf, 65, 256, "mxfp4"))
     r = torch.zeros(4, 64, device=cuda)
     with pytest.raises(ValueError):  # in place of another dtype
         pkg.mxfp4_linear(t, w, residual=r, out=r.view(torch.bfloat16)[:, :64])

@@ -274,6 +274,10 @@ def test_python_refusals_need_no_gpu(pkg):
         pkg.mxfp4_swiglu(t, w, w, quantize=True, out_dtype=torch.float32)
     with pytest.raises(ValueError, match="out_dtype"):
         pkg.mxfp4_linear(t, w, out_dtype=torch.float16)
+    for f in (pkg.dequantize, pkg.unpack_canonical, lambda v: pkg.mxfp4_linear(v, w),
+              lambda v: pkg.mxfp4_swiglu(v, w, w)):  # host memory never reaches a kernel
+        with pytest.raises(ValueError, match="GPU"):
+            f(t)
     with pytest.raises(ValueError, match="dtype"):
         pkg.dequantize(t, dtype=torch.float16)
     with pytest.raises(ValueError, match="dtype"):
