@@ -230,7 +230,7 @@ int qmlp_mx_swiglu(const void* x, int x_type, int64_t x_stride, const void* wg, 
                    void* ws, size_t ws_bytes, int M, int N, int K, int flags, qmlp_stream_t stream);
 
 /* Workspace bytes of the two products (host only); never shrinks as M grows.  0 where none is needed
- * (packed x up to 32 tokens, a token or two that the product quantises itself), and for sizes out of
+ * (packed x up to 32 tokens, up to four tokens that the product quantises itself), and for sizes out of
  * range, which the product refuses. */
 size_t qmlp_mx_workspace_bytes(int M, int N, int K, int x_type);
 
@@ -300,10 +300,10 @@ int qmlp_plan_tiles(int M, int H, int I, int fmt, int down, int num_cus, int* ou
 int qmlp_plan_split(int rows, int K, int nmat, int M, int num_cus, int* out6);
 
 /* How an MXFP4 product of M tokens, N output and K input features and `nmat` matrices (2 = gate/up)
- * runs on `num_cus` compute units.  Fills out[0..4] = {kernel: 0 a workgroup of four waves per 32
- * features and 32 tokens, 1 the same with twice the loads under way, 2 of eight waves, 3 per 32 features
- * and 64 tokens, 3 + h tiles of 256 features (of both matrices together) x 64 h tokens; pieces of the K range; workgroups; KB of partial tiles; 1
- * where the kernel also quantises unpacked rows}. */
+ * runs on `num_cus` compute units.  Fills out[0..4] = {kernel, pieces of the K range, workgroups, KB of
+ * partial tiles, 1 where the kernel also quantises unpacked rows}.  Kernels: 0 a workgroup of four waves
+ * per 32 features and 32 tokens, 1 the same with twice the loads under way, 2 of eight waves, 3 per 32
+ * features and 64 tokens, 3 + h tiles of 256 features (of both matrices together) x 64 h tokens. */
 int qmlp_mx_plan(int M, int N, int K, int nmat, int num_cus, int* out5);
 
 #ifdef __cplusplus

@@ -282,6 +282,52 @@ def test_rows_that_are_not_numbers_stay_in_their_row(pkg, cuda):
         assert torch.isnan(d[1]).all() and torch.isnan(d[M - 1]).all() and torch.isfinite(d[0]).all()
 
 
+@pytest.mark.parametrize("byte", [0, 1, 64, 127, 200, 225])
+def test_scales_over_their_whole_range(pkg, cuda, byte):
+    """Checkpoint scales down to the smallest.  |x| < 2^9 and a weight is at most 6 2^(byte - 127), so that
+    no sum of 288 products reaches 2^(9 + 3 + 9 + byte - 127) < 2^127.  On top of the sums' rounding each
+    product, and each of at most as many sums, may lose what is below the smallest normal number, 2^-126."""
+    K, N = 288, 256
+    codes = np.random.default_rng(byte).integers(0, 16, (N, K), dtype=np.uint8)
+    scales = np.full((N, K // 32), byte, dtype=np.uint8)
+    w = pkg.pack_canonical(torch.from_numpy(omx.join(codes)).to(cuda), torch.from_numpy(scales).to(cuda), "mxfp4")
+    for M in (1, 5, 40, 300):
+        print(f"case scale {byte} M={M}", flush=True)
+        x = _rows(M, K, torch.float32, M).clamp(-256, 256)
+        ref, mag = omx.linear(omx.dequantize(*omx.quantize(x.double().numpy())), omx.dequantize(codes, scales))
+        y = pkg.mxfp4_linear(x.to(cuda), w, out_dtype=torch.float32)
+        assert (np.abs(_np(y) - ref) <= _sum_error(K, mag) + 2 * K * 2.0 ** -126).all()
+
+
+def test_offsets_beyond_32_bits(pkg, cuda):
+    # rows 3.4 GB apart
+    K, stride = 256, 1600 * 2 ** 20
+    w, wd = _weight(pkg, 64, K, 3, cuda)
+    wide = torch.empty(2 * stride + K, dtype=torch.bfloat16, device=cuda)
+    x = wide.as_strided((3, K), (stride, 1))
+    rows = _rows(3, K, torch.bfloat16, 1)
+    x.copy_(rows.to(cuda))
+    near = rows.to(cuda)
+    for a, b in zip(pkg.unpack_canonical(pkg.quantize_mxfp4(x)), pkg.unpack_canonical(pkg.quantize_mxfp4(near))):
+        assert torch.equal(a, b)
+    assert torch.equal(pkg.mxfp4_linear(x, w), pkg.mxfp4_linear(near, w))
+    norm = torch.zeros(K, dtype=torch.bfloat16, device=cuda)
+    for a, b in zip(pkg.unpack_canonical(pkg.quantize_mxfp4(x, norm_weight=norm)),
+                    pkg.unpack_canonical(pkg.quantize_mxfp4(near, norm_weight=norm))):
+        assert torch.equal(a, b)
+    del wide, x
+    # an output of more than 2^31 values, and a product's largest number of tokens
+    M, N, K = 65536, 33000, 32
+    w, wd = _weight(pkg, N, K, 4, cuda)
+    some = torch.randn(64, K, generator=torch.Generator().manual_seed(5)).bfloat16()
+    y = pkg.mxfp4_linear(some.to(cuda).repeat(M // 64, 1), w)
+    ref, mag = omx.linear(omx.dequantize(*omx.quantize(some.double().numpy())), wd)
+    first = y[:64]
+    assert (np.abs(_np(first) - ref) <= _bf16_error(ref, _sum_error(K, mag))).all()
+    for r in (64, 32768, M - 64):
+        assert torch.equal(y[r:r + 64], first)
+
+
 def test_guarded_outputs(pkg, cuda):
     """Nothing is written outside the output, whatever the tail sizes."""
     for M, N, K in ((1, 33, 64), (5, 3, 256), (33, 250, 512), (70, 515, 288), (200, 129, 544)):

@@ -296,3 +296,13 @@ def test_formats(pkg):
     mlp.check_formats(pkg.MLPWeights(w, w, w))
     with pytest.raises(ValueError, match="formats"):
         mlp.check_formats(pkg.MLPWeights(w, pkg.PackedWeight(w.buf, 64, 256, "bfp8"), w))
+
+
+def test_a_stream_of_another_gpu_is_refused(pkg):
+    from qwen_mlp_amd import _lib
+
+    class Stream:
+        device = torch.device("cuda", 1)
+
+    with pytest.raises(ValueError, match="cuda:1"):
+        _lib.on_device(torch.device("cuda", 0), Stream())
