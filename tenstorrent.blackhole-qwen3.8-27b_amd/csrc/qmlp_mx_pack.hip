@@ -23,8 +23,8 @@ __device__ __forceinline__ MxItem mx_item(int tid) {
 
 // ---------------------------------------------------------------- quantisation
 //
-// Bound by memory for many rows (2 or 4 bytes read and 17/32 written per value: 2048 x 17408 bf16 in 14.6-16.3
-// us, 5.5-6.2 TB/s), by latency for few (one row of 5120: 2.4-2.6 us).
+// Bound by memory for many rows (2 or 4 bytes read and 17/32 written per value: 2048 x 17408 bf16 in
+// 14.0-16.4 us, 5.5-6.4 TB/s), by latency for few (one row of 5120: 2.4-2.6 us).
 // R groups of 8 rows keep R 16-byte loads of a thread in flight.  The scale bytes of a workgroup
 // gather in LDS, so that they leave as whole dwords.  Rows [rows, fill_rows) are written as zeros
 // (weights, whose packed bytes depend on the weights alone); bad (weights): count of blocks that hold
@@ -248,7 +248,7 @@ int launch_mx_unpack(const void* packed, int rows, int cols, void* codes, void* 
 //
 // Packed -> bf16 or fp32 values, exactly: a code has two significant bits, and 2^-128, the smallest
 // magnitude (scale byte 0, which packed checkpoints may hold), is a bf16 number too.  Bound by the
-// write (2048 x 17408 to bf16 in 16.1-18.1 us, 5.0-5.6 TB/s); the thread mapping is the quantiser's.
+// write (2048 x 17408 to bf16 in 16.0-18.4 us, 4.9-5.7 TB/s); the thread mapping is the quantiser's.
 template <bool F32, int R>
 __global__ __launch_bounds__(kQThreads) void mx_dequantize_kernel(const uint8_t* __restrict__ packed, int rows,
                                                                  int cols, uint8_t* __restrict__ out) {
