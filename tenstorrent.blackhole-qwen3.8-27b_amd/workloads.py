@@ -27,7 +27,7 @@ class Workload:
     def weight_bytes(self):
         """Bytes of the three matrices' values (gate/up and down per the weight format; "bf4"
         pairs bf4 gate/up with a bfp8 down)."""
-        per = {"bfp8": 17 / 16, "bf4": 9 / 16, "bf16": 2}
+        per = {"bfp8": 17 / 16, "bf4": 9 / 16, "bf16": 2, "mxfp4": 17 / 32}
         gu = self.fmt
         down = "bfp8" if self.fmt == "bf4" else self.fmt
         return int(self.hidden * self.intermediate * (2 * per[gu] + per[down]))

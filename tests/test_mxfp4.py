@@ -306,3 +306,14 @@ def test_a_stream_of_another_gpu_is_refused(pkg):
 
     with pytest.raises(ValueError, match="cuda:1"):
         _lib.on_device(torch.device("cuda", 0), Stream())
+
+
+def test_workload_bytes_of_every_format(pkg):
+    """A workload's weight bytes are those that the packed matrices' kernels stream."""
+    from qwen_mlp_amd import workloads
+
+    for fmt in pkg.WEIGHT_FORMATS:
+        wl = workloads.Workload("any", 512, 1024, 16, fmt, False)
+        gate_up, down = (pkg.PackedWeight(None, 512, 1024, f) for f in pkg.matrix_formats(fmt))
+        assert wl.weight_bytes() == 2 * gate_up.stream_bytes + down.stream_bytes
+        assert wl.algorithmic_bytes() == wl.weight_bytes() + 4 * 16 * 512
