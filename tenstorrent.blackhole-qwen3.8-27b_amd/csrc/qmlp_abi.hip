@@ -173,14 +173,14 @@ int forward_impl(const char* fn, const void* x, const void* wg, const void* wu, 
   }
   if (residual == out && residual && ((flags & QMLP_OUT_F32) != 0) != ((flags & QMLP_RESIDUAL_F32) != 0))
     return set_error(QMLP_E_SHAPE, "%s: an in-place residual needs the same dtype as out", fn);
-  const size_t need = qmlp_workspace_bytes(M, H, I, fmt);
+  const WsLayout L = tile_fmt(fmt) ? ws_layout(M, H, I, fmt) : WsLayout{};
+  const size_t need = tile_fmt(fmt) ? L.total : mx_forward_bytes(M, H, I);
   if (ws_bytes < need)
     return set_error(QMLP_E_WORKSPACE, "%s: workspace holds %zu bytes, needs %zu", fn, ws_bytes, need);
   DeviceInfo di;
   if (int rc = current_device_info(&di)) return rc;
   if (fmt == QMLP_FMT_MXFP4)
     return mx_forward(x, wg, wu, wd, residual, out, ws, M, H, I, flags, normw, eps, di.num_cus, stream);
-  const WsLayout L = ws_layout(M, H, I, fmt);
   ForwardArgs a{x, (const uint8_t*)wg, (const uint8_t*)wu, (const uint8_t*)wd, residual, out, (uint8_t*)ws,
                 M, H, I, fmt, (flags & QMLP_OUT_F32) ? 1 : 0, (flags & QMLP_RESIDUAL_F32) ? 1 : 0, normw, eps, false};
   // M <= 32: split-K weight streaming with LDS-staged activations; where no such split fits (a K
