@@ -513,3 +513,41 @@ def test_load_cache_and_packer(pkg, cuda, tmp_path):
     q, e = np.load(tmp_path / "out" / "layer_0" / "up_proj.q.npy"), np.load(tmp_path / "out" / "layer_0" / "up_proj.e8.npy")
     want, wants = omx.quantize(_np(sd["up_proj.weight"]))
     assert np.array_equal(q, omx.join(want)) and np.array_equal(e, wants)
+
+
+def _head(pkg, t, rows):
+    """The first ``rows`` rows (a multiple of 32) of a packed matrix."""
+    return pkg.MxTensor(t.buf[:omx.packed_bytes(rows, t.cols)], rows, t.cols)
+
+
+def test_block_beyond_32_bit_offsets(pkg, cuda):
+    """The block at its largest number of tokens, with more than 2^30 values of h: its pieces, the same in
+    every copy of the tokens, and right in the first."""
+    H, I, M, rows = 256, 16640, 65536, 64
+    mlp = pkg.Qwen36MLP(cuda, _state_dict(H, I, cuda), weight_format="mxfp4", max_tokens=64, pool=pkg.WorkspacePool())
+    w = mlp.weights
+    some = _rows(rows, H, torch.bfloat16, 3, 0.05).to(cuda)
+    x = some.repeat(M // rows, 1)
+    r = torch.randn(M, H, generator=torch.Generator(device=cuda).manual_seed(4), device=cuda)
+    h = pkg.mxfp4_swiglu(x, w.w1, w.w3, quantize=True)
+    y = mlp.forward(x, residual=r, out_dtype=torch.float32)
+    assert torch.equal(y, pkg.mxfp4_linear(h, w.w2, residual=r, out_dtype=torch.float32))
+    plain = mlp.forward(x)
+    for at in (rows, M // 2, M - rows):
+        assert torch.equal(plain[at:at + rows], plain[:rows])
+    # h of the first copy: half a step of a value of its block (at most the scale itself), a block's
+    # largest values saturate by at most twice the scale, and the sums' rounding
+    (codes, scales), xd = _unpack(pkg, _head(pkg, h, rows)), omx.dequantize(*omx.quantize(_np(some)))
+    hd = omx.dequantize(codes, scales)
+    (g, gm), (u, um) = (omx.linear(xd, _np(pkg.dequantize(v))) for v in (w.w1, w.w3))
+    ge, ue, s = _sum_error(H, gm), _sum_error(H, um), _silu(g)
+    err = 1.1 * ge * (np.abs(u) + ue) + (np.abs(s) + 1.1 * ge) * ue + (8 + np.abs(g)) * 2.0 ** -23 * np.abs(s * u)
+    step = np.repeat(np.exp2(scales.astype(np.float64) - 127), 32, axis=1)
+    assert (np.abs(hd - s * u) <= 2 * step + err).all()
+    ref, mag = omx.linear(hd, _np(pkg.dequantize(w.w2)))
+    ref, err = ref + _np(r[:rows]), _sum_error(I, mag)
+    assert (np.abs(_np(y[:rows]) - ref) <= err + 2.0 ** -24 * (np.abs(ref) + err)).all()
+    # the norm in front
+    nw = (torch.randn(H, generator=torch.Generator().manual_seed(5)) * 0.1).bfloat16().to(cuda)
+    hn = pkg.mxfp4_swiglu(pkg.quantize_mxfp4(x, norm_weight=nw), w.w1, w.w3, quantize=True)
+    assert torch.equal(mlp.forward_rmsnorm(x, nw), pkg.mxfp4_linear(hn, w.w2, residual=x))

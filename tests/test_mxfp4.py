@@ -317,3 +317,14 @@ def test_workload_bytes_of_every_format(pkg):
         gate_up, down = (pkg.PackedWeight(None, 512, 1024, f) for f in pkg.matrix_formats(fmt))
         assert wl.weight_bytes() == 2 * gate_up.stream_bytes + down.stream_bytes
         assert wl.algorithmic_bytes() == wl.weight_bytes() + 4 * 16 * 512
+
+
+def test_the_block_takes_activations_beyond_32_bit_offsets(pkg):
+    """As its products do: the last refusal before a device is touched is the workspace's."""
+    lib, F = pkg.lib(), pkg.FMT_MXFP4
+    for M, H, I in ((65536, 256, 16640), (65536, 5120, 17408), (65536, 16640, 256)):
+        need = lib.qmlp_workspace_bytes(M, H, I, F)
+        assert need > 0
+        assert lib.qmlp_forward(P(1 << 40), W0, W1, W0, None, P(1 << 42), P(1 << 44), need - 1, M, H, I, F, None) == E_WORKSPACE
+        assert lib.qmlp_forward_rmsnorm(P(1 << 40), W0, 1e-6, W0, W1, W0, P(1 << 42), P(1 << 44), need - 1, M, H, I, F, 0,
+                                        None) == E_WORKSPACE
