@@ -108,8 +108,10 @@ def _quantize(w, fmt, stream):
 def _read_info(pw, stream=None):
     norm = ctypes.c_double(0.0)
     flushed = ctypes.c_uint32(0)
-    _lib.check(_lib.lib().qmlp_packed_info(_lib.ptr(pw.buf), pw.rows, pw.cols, pw.fmt_code, ctypes.byref(norm),
-                                           ctypes.byref(flushed), _lib.stream_handle(stream)), "qmlp_packed_info")
+    with _lib.on_device(pw.buf.device, stream):
+        _lib.check(_lib.lib().qmlp_packed_info(_lib.ptr(pw.buf), pw.rows, pw.cols, pw.fmt_code, ctypes.byref(norm),
+                                               ctypes.byref(flushed), _lib.device_stream(pw.buf.device, stream)),
+                   "qmlp_packed_info")
     pw.max_row_norm = float(norm.value)
     pw.flushed_groups = int(flushed.value)
     return pw
@@ -202,9 +204,10 @@ def _pack_weight_begin(w, fmt, stream):
     nbytes = _lib.lib().qmlp_packed_bytes(rows, cols, code)
     if nbytes == 0:
         raise _unsupported_shape(rows, cols, fmt)
-    buf = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
-    _lib.check(_lib.lib().qmlp_quantize_pack(_lib.ptr(w), rows, cols, code, _lib.ptr(buf), nbytes,
-                                             _lib.stream_handle(stream)), "qmlp_quantize_pack")
+    with _lib.on_device(w.device, stream):
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
+        _lib.check(_lib.lib().qmlp_quantize_pack(_lib.ptr(w), rows, cols, code, _lib.ptr(buf), nbytes,
+                                                 _lib.device_stream(w.device, stream)), "qmlp_quantize_pack")
     return PackedWeight(buf, rows, cols, fmt)
 
 
@@ -212,9 +215,11 @@ def _pack_weight_end(pw, strict, stream):
     """Waits for the conversion and refuses non-finite values and, with ``strict``, flushed groups."""
     norm = ctypes.c_double(0.0)
     flushed, bad = ctypes.c_uint32(0), ctypes.c_uint32(0)
-    _lib.check(_lib.lib().qmlp_quantize_pack_info(_lib.ptr(pw.buf), pw.rows, pw.cols, pw.fmt_code, ctypes.byref(norm),
-                                                  ctypes.byref(flushed), ctypes.byref(bad),
-                                                  _lib.stream_handle(stream)), "qmlp_quantize_pack_info")
+    with _lib.on_device(pw.buf.device, stream):
+        _lib.check(_lib.lib().qmlp_quantize_pack_info(_lib.ptr(pw.buf), pw.rows, pw.cols, pw.fmt_code,
+                                                      ctypes.byref(norm), ctypes.byref(flushed), ctypes.byref(bad),
+                                                      _lib.device_stream(pw.buf.device, stream)),
+                   "qmlp_quantize_pack_info")
     pw.max_row_norm = float(norm.value)
     pw.flushed_groups = int(flushed.value)
     if bad.value:
@@ -226,7 +231,7 @@ def _pack_weight_end(pw, strict, stream):
 
 def pack_weight(w, fmt="bfp8", strict=True, stream=None):
     """bf16 ``[rows, cols]`` GPU tensor (HF layout: [out, in]) -> PackedWeight in the matrix format
-    ``fmt`` ("bf16", "bfp8", "bf4" or "mxfp4")."""
+    ``fmt`` ("bf16", "bfp8", "bf4" or "mxfp4"), on ``w``'s GPU."""
     return _pack_weight_end(_pack_weight_begin(w, fmt, stream), strict, stream)
 
 

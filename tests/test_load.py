@@ -91,3 +91,66 @@ def test_pool_refuses_a_device_that_is_not_a_gpu(pkg, monkeypatch):
     assert pool.reserve(64, "cuda:0").numel() == 64
     with pytest.raises(ValueError, match="cpu"):
         pool.reserve(64, "cpu")
+
+
+class _OnGpu1(torch.Tensor):
+    """Host memory that says it is on the second GPU."""
+
+    @property
+    def device(self):
+        return torch.device("cuda", 1)
+
+
+class _Calls:
+    """A library whose calls succeed; ``made`` holds (name, current GPU, stream) of each."""
+
+    def __init__(self):
+        self.made, self.current = [], 0
+
+    def __getattr__(self, name):
+        def call(*args):
+            if name.endswith("_bytes"):
+                return 64
+            self.made.append((name, self.current, args[-1]))
+            return 0
+
+        return call
+
+
+@pytest.fixture
+def calls(pkg, monkeypatch):
+    """The first GPU is current; GPU i's current stream has the handle 100 + i."""
+    from qwen_mlp_amd import _lib
+
+    c = _Calls()
+
+    class Device:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.before, c.current = c.current, self.index
+
+        def __exit__(self, *exc):
+            c.current = self.before
+
+    empty = torch.empty
+    monkeypatch.setattr(_lib, "lib", lambda: c)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: c.current)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 100 + index)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: c.current)
+    monkeypatch.setattr(torch, "empty", lambda *size, device=None, **kw: empty(*size, **kw).as_subclass(_OnGpu1))
+    return c
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "bfp8", "bf4", "mxfp4"])
+def test_a_weight_is_packed_and_checked_on_its_own_gpu(pkg, calls, fmt):
+    from qwen_mlp_amd import mlp
+
+    w = torch.zeros(16, 256, dtype=torch.bfloat16).as_subclass(_OnGpu1)
+    pw = pkg.pack_weight(w, fmt)
+    mlp._read_info(pw)
+    assert [name for name, *_ in calls.made] == ["qmlp_quantize_pack", "qmlp_quantize_pack_info", "qmlp_packed_info"]
+    assert [(gpu, getattr(stream, "value", stream)) for _, gpu, stream in calls.made] == 3 * [(1, 101)]
+    assert calls.current == 0
