@@ -520,13 +520,14 @@ def mlp_forward(x2d, weights, residual=None, out=None, workspace=None, stream=No
             raise ValueError("out must match x")
     if out.dtype == torch.float32:
         flags |= _lib.OUT_F32
-    if workspace is None:
-        workspace = new_workspace(M, H, I, weights.fmt, x2d.device, stream)
-    rc = _lib.lib().qmlp_forward_ex(_lib.ptr(x2d), _lib.ptr(weights.w1.buf), _lib.ptr(weights.w3.buf),
-                                    _lib.ptr(weights.w2.buf), _lib.ptr(residual), _lib.ptr(out),
-                                    _lib.ptr(workspace), workspace.numel(), M, H, I, weights.w1.fmt_code, flags,
-                                    _lib.stream_handle(stream))
-    _lib.check(rc, "qmlp_forward")
+    with _lib.on_device(x2d.device):
+        if workspace is None:
+            workspace = new_workspace(M, H, I, weights.fmt, x2d.device, stream)
+        rc = _lib.lib().qmlp_forward_ex(_lib.ptr(x2d), _lib.ptr(weights.w1.buf), _lib.ptr(weights.w3.buf),
+                                        _lib.ptr(weights.w2.buf), _lib.ptr(residual), _lib.ptr(out),
+                                        _lib.ptr(workspace), workspace.numel(), M, H, I, weights.w1.fmt_code, flags,
+                                        _lib.device_stream(x2d.device, stream))
+        _lib.check(rc, "qmlp_forward")
     return out
 
 
@@ -553,13 +554,15 @@ def mlp_forward_rmsnorm(h2d, norm_weight, weights, eps=1e-6, out=None, workspace
         if out.dtype not in (torch.bfloat16, torch.float32) or tuple(out.shape) != (M, H):
             raise ValueError("out must be a bf16 or fp32 [M, H] tensor")
     flags = _lib.OUT_F32 if out.dtype == torch.float32 else 0
-    if workspace is None:
-        workspace = new_workspace(M, H, I, weights.fmt, h2d.device, stream)
-    rc = _lib.lib().qmlp_forward_rmsnorm(_lib.ptr(h2d), _lib.ptr(norm_weight), float(eps), _lib.ptr(weights.w1.buf),
-                                         _lib.ptr(weights.w3.buf), _lib.ptr(weights.w2.buf), _lib.ptr(out),
-                                         _lib.ptr(workspace), workspace.numel(), M, H, I, weights.w1.fmt_code, flags,
-                                         _lib.stream_handle(stream))
-    _lib.check(rc, "qmlp_forward_rmsnorm")
+    with _lib.on_device(h2d.device):
+        if workspace is None:
+            workspace = new_workspace(M, H, I, weights.fmt, h2d.device, stream)
+        rc = _lib.lib().qmlp_forward_rmsnorm(_lib.ptr(h2d), _lib.ptr(norm_weight), float(eps),
+                                             _lib.ptr(weights.w1.buf), _lib.ptr(weights.w3.buf),
+                                             _lib.ptr(weights.w2.buf), _lib.ptr(out), _lib.ptr(workspace),
+                                             workspace.numel(), M, H, I, weights.w1.fmt_code, flags,
+                                             _lib.device_stream(h2d.device, stream))
+        _lib.check(rc, "qmlp_forward_rmsnorm")
     return out
 
 

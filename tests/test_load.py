@@ -154,3 +154,22 @@ def test_a_weight_is_packed_and_checked_on_its_own_gpu(pkg, calls, fmt):
     assert [name for name, *_ in calls.made] == ["qmlp_quantize_pack", "qmlp_quantize_pack_info", "qmlp_packed_info"]
     assert [(gpu, getattr(stream, "value", stream)) for _, gpu, stream in calls.made] == 3 * [(1, 101)]
     assert calls.current == 0
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "bfp8", "bf4", "mxfp4"])
+def test_the_block_runs_on_its_input_gpu(pkg, calls, fmt):
+    def tensor(*size, dtype=torch.bfloat16):
+        return torch.zeros(*size, dtype=dtype).as_subclass(_OnGpu1)
+
+    gate_up, down = pkg.matrix_formats(fmt)
+    buf = tensor(64, dtype=torch.uint8)
+    w = pkg.MLPWeights(w1=pkg.PackedWeight(buf, I, H, gate_up), w3=pkg.PackedWeight(buf, I, H, gate_up),
+                       w2=pkg.PackedWeight(buf, H, I, down))
+    x, norm = tensor(4, H), tensor(H)
+    for workspace in (None, buf):
+        pkg.mlp_forward(x, w, residual=x, workspace=workspace)
+        pkg.mlp_forward_rmsnorm(x, norm, w, workspace=workspace)
+    assert [name for name, *_ in calls.made] == ["qmlp_workspace_init", "qmlp_forward_ex", "qmlp_workspace_init",
+                                                 "qmlp_forward_rmsnorm", "qmlp_forward_ex", "qmlp_forward_rmsnorm"]
+    assert [(gpu, getattr(stream, "value", stream)) for _, gpu, stream in calls.made] == 6 * [(1, 101)]
+    assert calls.current == 0
