@@ -210,7 +210,8 @@ int qmlp_mx_quantize(const void* x, int x_type, int64_t x_stride, int rows, int 
 int qmlp_mx_quantize_rmsnorm(const void* h, int64_t h_stride, const void* norm_w, float eps, int rows,
                              int cols, void* packed, size_t packed_bytes, qmlp_stream_t stream);
 
-/* Packed matrix -> bf16 (out_type QMLP_X_BF16) or fp32 (QMLP_X_F32) [rows, cols], exactly. */
+/* Packed matrix -> bf16 (out_type QMLP_X_BF16) or fp32 (QMLP_X_F32) [rows, cols], exactly; magnitudes
+ * from 2^128 on (scales of 253 and 254 in packed checkpoints) become infinities. */
 int qmlp_mx_dequantize(const void* packed, int rows, int cols, void* out, int out_type,
                        qmlp_stream_t stream);
 

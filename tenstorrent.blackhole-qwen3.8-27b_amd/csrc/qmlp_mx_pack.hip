@@ -247,7 +247,8 @@ int launch_mx_unpack(const void* packed, int rows, int cols, void* codes, void* 
 // ---------------------------------------------------------------- dequantisation
 //
 // Packed -> bf16 or fp32 values, exactly: a code has two significant bits, and 2^-128, the smallest
-// magnitude (scale byte 0, which packed checkpoints may hold), is a bf16 number too.  Bound by the
+// magnitude (scale byte 0, which packed checkpoints may hold), is a bf16 number too.  Magnitudes from
+// 2^128 on, which scale bytes 253 and 254 of a checkpoint can name, become infinities.  Bound by the
 // write (2048 x 17408 to bf16 in 16.0-18.4 us, 4.9-5.7 TB/s); the thread mapping is the quantiser's.
 template <bool F32, int R>
 __global__ __launch_bounds__(kQThreads) void mx_dequantize_kernel(const uint8_t* __restrict__ packed, int rows,

@@ -266,7 +266,8 @@ def unpack_canonical(pw, stream=None):
 
 def dequantize(pw, stream=None, dtype=torch.float32):
     """Packed weight -> float32 ``[rows, cols]`` via the kernels' own dequant routine.  mxfp4 (a weight
-    or an ``MxTensor``) also to bfloat16, which holds every value of the format exactly."""
+    or an ``MxTensor``) also to bfloat16.  Both hold every value of the format below 2^128 exactly; from
+    there on (scales of 253 and 254, which only packed checkpoints can hold) it becomes an infinity."""
     if pw.fmt == "mxfp4":
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("dtype must be bf16 or fp32")

@@ -551,3 +551,25 @@ def test_block_beyond_32_bit_offsets(pkg, cuda):
     nw = (torch.randn(H, generator=torch.Generator().manual_seed(5)) * 0.1).bfloat16().to(cuda)
     hn = pkg.mxfp4_swiglu(pkg.quantize_mxfp4(x, norm_weight=nw), w.w1, w.w3, quantize=True)
     assert torch.equal(mlp.forward_rmsnorm(x, nw), pkg.mxfp4_linear(hn, w.w2, residual=x))
+
+
+def test_largest_scales(pkg, cuda):
+    """Scales of 252 to 254: magnitudes from 2^128 on, no fp32 or bf16 numbers, dequantise to infinities, the
+    others exactly.  In a product with small activations they count as what they are: |x| < 2^-90, so that
+    no sum of 288 products reaches 2^(9 + 3 + 127 - 90) = 2^49."""
+    K, N = 288, 96
+    codes = np.random.default_rng(1).integers(0, 16, (N, K), dtype=np.uint8)
+    codes[:, :16] = np.arange(16)
+    scales = np.tile(np.array([252, 253, 254], dtype=np.uint8), (N, 3))
+    w = pkg.pack_canonical(torch.from_numpy(omx.join(codes)).to(cuda), torch.from_numpy(scales).to(cuda), "mxfp4")
+    wd = omx.dequantize(codes, scales)
+    big = np.abs(wd) >= 2.0 ** 128
+    assert big.any() and (np.abs(wd[~big]) > 2.0 ** 127).any()
+    for dt in (torch.float32, torch.bfloat16):
+        d = _np(pkg.dequantize(w, dtype=dt))
+        assert np.array_equal(d[~big], wd[~big]) and np.array_equal(d[big], np.sign(wd[big]) * np.inf)
+    for M in (1, 5, 40):
+        x = (_rows(M, K, torch.float32, M).clamp(-256, 256) * 2.0 ** -98).contiguous()
+        ref, mag = omx.linear(omx.dequantize(*omx.quantize(x.double().numpy())), wd)
+        y = pkg.mxfp4_linear(x.to(cuda), w, out_dtype=torch.float32)
+        assert (np.abs(_np(y) - ref) <= _sum_error(K, mag)).all()
