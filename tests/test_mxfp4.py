@@ -328,3 +328,30 @@ def test_the_block_takes_activations_beyond_32_bit_offsets(pkg):
         assert lib.qmlp_forward(P(1 << 40), W0, W1, W0, None, P(1 << 42), P(1 << 44), need - 1, M, H, I, F, None) == E_WORKSPACE
         assert lib.qmlp_forward_rmsnorm(P(1 << 40), W0, 1e-6, W0, W1, W0, P(1 << 42), P(1 << 44), need - 1, M, H, I, F, 0,
                                         None) == E_WORKSPACE
+
+
+# The tiled kernels, with the last tile of features full and part full (a row length that is not a multiple of
+# 4 among them), whole and in pieces; tests/test_gpu_mxfp4_tiles.py runs them.
+TILE_SHAPES = [(1, 1107, 256, 96), (1, 1107, 65, 96), (1, 1097, 256, 3904), (1, 1097, 66, 3904),
+               (1, 1688, 4608, 96), (1, 2311, 1593, 96), (1, 1392, 256, 33632), (1, 1392, 77, 33632),
+               (1, 2047, 4608, 96), (1, 2047, 4618, 96), (1, 2047, 6144, 96), (1, 1361, 8237, 96),
+               (2, 1025, 256, 96), (2, 1025, 250, 96), (2, 33, 256, 22816), (2, 33, 250, 22816),
+               (2, 1635, 1280, 96), (2, 1635, 1275, 96), (2, 65, 2816, 16352), (2, 777, 2819, 1056),
+               (2, 65, 2803, 16352), (2, 1178, 3328, 96), (2, 1178, 3331, 96), (2, 782, 6912, 96), (2, 782, 6915, 96)]
+
+
+def tile_plan(pkg, nmat, M, N, K):
+    """(tile height in units of 64 tokens, pieces of K) of a product that is planned on tiles."""
+    kind, ks, *_ = _plan(pkg, nmat, M, N, K)
+    assert kind >= 4, f"{nmat} x {M} x {N} x {K} is not planned on tiles"
+    return kind - 3, ks
+
+
+def test_tile_shapes_reach_every_tiled_kernel(pkg):
+    got = {(n, *tile_plan(pkg, n, M, N, K), N % (256 // n) == 0) for n, M, N, K in TILE_SHAPES}
+    got = {(n, h, ks > 1, full) for n, h, ks, full in got}
+    heights = [(h, False) for h in (1, 2, 3, 4)] + [(h, True) for h in (1, 2)]
+    assert got == {(n, h, split, full) for n in (1, 2) for h, split in heights for full in (True, False)}
+    for n in (1, 2):  # rows that start misaligned for vector stores, whole and in pieces
+        odd = {tile_plan(pkg, n, M, N, K)[1] > 1 for m, M, N, K in TILE_SHAPES if m == n and N % 4}
+        assert odd == {True, False}
