@@ -573,3 +573,137 @@ def test_largest_scales(pkg, cuda):
         ref, mag = omx.linear(omx.dequantize(*omx.quantize(x.double().numpy())), wd)
         y = pkg.mxfp4_linear(x.to(cuda), w, out_dtype=torch.float32)
         assert (np.abs(_np(y) - ref) <= _sum_error(K, mag)).all()
+
+
+# ---------------------------------------------------------------- largest sizes, streams, checkpoints
+
+
+@pytest.mark.parametrize("rows,cols", [(1 << 20, 32), (2, 1 << 20)])
+def test_largest_matrices(pkg, cuda, rows, cols):
+    """As activations and as weights, against the oracle on some of their rows and against each other."""
+    print(f"case largest {rows}x{cols}", flush=True)
+    base = _rows(min(rows, 96), cols, torch.bfloat16, 9)
+    x = base.to(cuda).repeat(-(-rows // 96), 1)[:rows].contiguous()
+    t = pkg.quantize_mxfp4(x)
+    codes, scales = pkg.unpack_canonical(t)
+    want, wants = omx.quantize(_np(base))
+    assert np.array_equal(codes[:96].cpu().numpy(), omx.join(want)) and np.array_equal(scales[:96].cpu().numpy(), wants)
+    for at in (range(96, rows - 95, 96 * 1021) if rows > 96 else ()):
+        assert torch.equal(codes[at:at + 96], codes[:96]) and torch.equal(scales[at:at + 96], scales[:96])
+    assert torch.equal(codes[-1], codes[(rows - 1) % 96]) and torch.equal(scales[-1], scales[(rows - 1) % 96])
+    pw = pkg.pack_weight(x, "mxfp4")
+    units = t.nbytes - omx.TRAILER_BYTES  # rows is whole units here, or the rest is zeros in a weight
+    if rows % 32 == 0:
+        assert torch.equal(pw.buf[:units], t.buf[:units])
+    again = pkg.pack_canonical(codes, scales, "mxfp4")
+    assert torch.equal(again.buf, pw.buf)
+    assert torch.equal(pkg.dequantize(pw, dtype=torch.bfloat16), pkg.dequantize(t, dtype=torch.bfloat16))
+    normed = pkg.quantize_mxfp4(x, norm_weight=torch.zeros(cols, dtype=torch.bfloat16, device=cuda))
+    few = pkg.quantize_mxfp4(x[:96], norm_weight=torch.zeros(cols, dtype=torch.bfloat16, device=cuda))
+    for a, b in zip(pkg.unpack_canonical(normed), pkg.unpack_canonical(few)):
+        assert torch.equal(a[:96], b) and torch.equal(a[-1], b[(rows - 1) % 96])
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 1 << 20, 64), (70, 1 << 20, 64), (1, 33, 1 << 20), (40, 33, 1 << 20),
+                                   (1100, 33, 1 << 20)])
+def test_products_at_the_largest_sizes(pkg, cuda, M, N, K):
+    """Every block's scale is the same, so every product is a multiple of 2^-9.  A random sum of 2^20 of them, up
+    to 36 2^-7 = 144 units each, stays below 2^24 units (it has a spread of 2^10 times 40 or so), so that no
+    sum rounds.  For a gate below -87.33 the reciprocal of 1 + exp(-gate) lies below fp32's
+    normal numbers, and the silu may come out as 0, from which it is less than 87.34 e^-87.33 < 1.1e-36 away."""
+    print(f"case largest product {M}x{N}x{K}", flush=True)
+    g = torch.Generator(device=cuda).manual_seed(N)
+    table = torch.tensor([*omx.VALUES, *-omx.VALUES], dtype=torch.float32, device=cuda)
+    x = table[torch.randint(0, 16, (M, K), generator=g, device=cuda)]
+    x[:, ::32] = 4.0
+    t = pkg.quantize_mxfp4(x)
+    assert torch.equal(pkg.dequantize(t), x)
+    scales = torch.full((N, K // 32), 120, device=cuda, dtype=torch.uint8)
+    ws = [pkg.pack_canonical(torch.randint(0, 256, (N, K // 2), generator=g, device=cuda, dtype=torch.uint8), scales,
+                             "mxfp4") for _ in range(2)]
+    some = [0, M // 2, M - 1]
+    gate, up = (x[some].double() @ pkg.dequantize(w).double().T for w in ws)
+    y = pkg.mxfp4_linear(x, ws[0], out_dtype=torch.float32)
+    assert torch.equal(y[some].double(), gate)
+    assert torch.equal(pkg.mxfp4_linear(t, ws[0], out_dtype=torch.float32), y)
+    ref = gate * torch.sigmoid(gate) * up
+    y = pkg.mxfp4_swiglu(x, *ws, out_dtype=torch.float32)
+    err = (8 + gate.abs()) * 2.0 ** -23 * ref.abs() + 1.1e-36 * up.abs() + 1e-37
+    assert ((y[some].double() - ref).abs() <= err).all()
+    assert torch.equal(pkg.mxfp4_swiglu(t, *ws), y.bfloat16())
+
+
+def test_every_call_on_a_given_stream(pkg, cuda):
+    """``stream`` may be another one than the current one; what it returns is ready on that stream."""
+    x, _, w, _ = _product_case(pkg, cuda, 40, 512, 320, torch.bfloat16)
+    w3, _ = _weight(pkg, 512, 320, 5, cuda)
+    plain = torch.randn(512, 256, generator=torch.Generator().manual_seed(1)).bfloat16().to(cuda)
+    norm = torch.zeros(320, dtype=torch.bfloat16, device=cuda)
+    q, e = pkg.unpack_canonical(w)
+    t = pkg.quantize_mxfp4(x)
+    calls = [lambda **k: pkg.quantize_mxfp4(x, **k).buf[:64], lambda **k: pkg.quantize_mxfp4(x, norm_weight=norm, **k).buf[:64],
+             lambda **k: pkg.dequantize(w, **k), lambda **k: pkg.dequantize(t, dtype=torch.bfloat16, **k),
+             lambda **k: pkg.unpack_canonical(t, **k)[0], lambda **k: pkg.pack_canonical(q, e, "mxfp4", **k).buf,
+             lambda **k: pkg.mxfp4_linear(x, w, **k), lambda **k: pkg.mxfp4_swiglu(x, w, w3, **k),
+             lambda **k: pkg.dequantize(pkg.mxfp4_swiglu(x, w, w3, quantize=True, **k), **k)]
+    calls += [lambda f=f, **k: pkg.pack_weight(plain, f, **k).buf for f in ("mxfp4", "bfp8", "bf4", "bf16")]
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    for f, y in zip(calls, want):
+        got = f(stream=s)
+        s.synchronize()
+        assert torch.equal(got, y)
+    assert torch.cuda.current_stream() != s
+
+
+def test_a_block_from_a_checkpoint_in_the_format(pkg, cuda, tmp_path):
+    """Codes and scales become a block through MLPWeights, or a Qwen36MLP through the weight cache, and mean
+    the values that they stand for."""
+    from qwen_mlp_amd import weight_cache
+
+    H, I, M = 256, 512, 7
+    rng = np.random.default_rng(3)
+    made, values = {}, {}
+    for name, (rows, cols) in (("gate_proj", (I, H)), ("up_proj", (I, H)), ("down_proj", (H, I))):
+        codes = rng.integers(0, 16, (rows, cols), dtype=np.uint8)
+        scales = rng.integers(117, 124, (rows, cols // 32), dtype=np.uint8)
+        made[name] = pkg.pack_canonical(torch.from_numpy(omx.join(codes)).to(cuda), torch.from_numpy(scales).to(cuda), "mxfp4")
+        values[name] = omx.dequantize(codes, scales)
+        weight_cache.save(weight_cache.cache_file(tmp_path, name, "mxfp4"), made[name])
+    weights = pkg.MLPWeights(w1=made["gate_proj"], w2=made["down_proj"], w3=made["up_proj"])
+    x = _rows(M, H, torch.bfloat16, 3, 0.05).to(cuda)
+    y = pkg.mlp_forward(x, weights, residual=x, out_dtype=torch.float32)
+    mlp = pkg.Qwen36MLP(cuda, {}, tmp_path, weight_format="mxfp4", max_tokens=M)
+    assert torch.equal(mlp.forward(x, residual=x, out_dtype=torch.float32), y)
+    h = pkg.mxfp4_swiglu(x, made["gate_proj"], made["up_proj"], quantize=True)
+    ref, mag = omx.linear(_np(pkg.dequantize(h)), values["down_proj"])
+    ref, err = ref + _np(x), _sum_error(I, mag)
+    assert (np.abs(_np(y) - ref) <= err + 2.0 ** -24 * (np.abs(ref) + err)).all()
+
+
+def test_verify_arm_on_the_format(pkg, cuda):
+    """The arm's check of each layer's weights and its route take mxfp4 layers."""
+    from qwen_mlp_amd.verify_arm import VerifyArm
+
+    H, I = 256, 512
+
+    class Decoder:
+        def __init__(self, seed):
+            self.sd = _state_dict(H, I, cuda, seed)
+
+        def state_dict(self):
+            return self.sd
+
+        def forward(self, x):
+            return None
+
+    layers = [Decoder(1), Decoder(2)]
+    amd = [pkg.Qwen36MLP(cuda, d.sd, weight_format="mxfp4", max_tokens=16) for d in layers]
+    x = _rows(16, H, torch.bfloat16, 3, 0.05).to(cuda).view(1, 1, 16, H)
+    arm = VerifyArm(layers, amd)
+    with arm.install():
+        got = [d.forward(x) for d in layers]
+    assert all(torch.equal(y, m.forward(x)) for y, m in zip(got, amd)) and arm.audit["hits"] == [1, 1]
+    with pytest.raises(ValueError, match="layer 0"):
+        VerifyArm(layers, amd[::-1]).check_layer_weights()
