@@ -98,8 +98,10 @@ int launch_mx_quantize(const void* x, int type, size_t row_bytes, int rows, int 
 //
 // The decoder's zero-centred norm, n = bf16(x * (1 / sqrt(mean(x^2) + eps)) * (1 + w)), then n's blocks.
 // One workgroup per row, the sums in rows_kernel's order, so that the result is that of the norm pass
-// followed by the quantisation, bit for bit.  Bound by latency (a row's load, a reduction, its store):
-// 3.4-4.5 us at 16 rows of 5120.  REGS: rows of up to 8192 values stay in registers.
+// followed by the quantisation, bit for bit.  Bound by latency (a row's load, a reduction, its store)
+// for few rows: 3.4-4.6 us at 16 of 5120 values.  For many its stores bound it, 4 bytes in runs of 16 and
+// single scale bytes: 7.6 us at 777 rows, 11.0 at 2048 (2.4 TB/s), where the quantisation alone, whose
+// workgroups write whole dwords of eight rows, takes 8.7.  REGS: rows of up to 8192 values stay in registers.
 constexpr int kNormCh = 4;
 template <bool REGS>
 __global__ __launch_bounds__(kQThreads) void mx_norm_quantize_kernel(const uint8_t* __restrict__ x, size_t row_bytes,

@@ -6,11 +6,12 @@ namespace qmlp {
 
 // Every candidate's time in microseconds, linear in what it does, and the cheapest one wins.  The
 // constants were fitted (non-negative least squares, points near the fastest of their sizes weighing
-// most) to 5900 measured (sizes, candidate) points on 256 CUs: 16 shapes from N = 96 to 17408 and K = 512 to
-// 17408 with one and two matrices, 21 token counts from 8 to 2048 (for the streamed kernels the points of
-// matrices beyond 40 million values weigh six times).  The plan they pick was on average 1.9 % (one
-// matrix) and 1.3 % (two) slower than the fastest measured one, at worst 25 % (9.4 against 7.5 us at 96
-// tokens of 3000 x 5120, where streamed and tiled kernels meet).
+// most) to 5900 measured (sizes, candidate) points on 256 CUs with packed activations: 16 shapes from N = 96
+// to 17408 and K = 512 to 17408 with one and two matrices, 21 token counts from 8 to 2048 (for the streamed
+// kernels the points of matrices beyond 40 million values weigh six times).  Measured again on the kernels
+// as they are, up to 1024 tokens the plan is on average 2.1 % (one matrix) and 1.4 % (two) slower than the
+// fastest measured candidate, at worst 25 % (9.4 against 7.5 us at 96 tokens of 3000 x 5120, where streamed
+// and tiled kernels meet).
 //
 // Streamed, per workgroup: launch and tail; units of K a wave takes in turn; all (32 features x token
 // group x unit) products of the launch and all weight units it reads, per CU; rounds of workgroups.
@@ -41,7 +42,9 @@ constexpr TileCost kTileCost[2][4] = {
 // Tiles of more than two heights stay whole: split, they won nowhere.
 constexpr int kMostSplit = 2;
 constexpr int kPieces[] = {1, 2, 3, 4, 6, 8, 12};
-constexpr int kMostStreamed = 1024;  // tokens: beyond, the tiles win at every measured shape
+// Tokens up to which the streamed kernels are candidates.  Beyond, the tiles win at 15 of the 16 measured
+// shapes; at the narrowest, 96 x 5120, streaming took 4.2 us at 2048 tokens and the planned tiles take 10.1.
+constexpr int kMostStreamed = 1024;
 
 MxPlan mx_plan(int M, int N, int K, int nmat, int num_cus) {
   const double cus = num_cus;

@@ -12,9 +12,10 @@
 //     pair of products, in the order written here.
 // Measured (256 tiles of 256 x 256, K = 17408, random codes): 126-131 us, 4.5-4.6 PFLOP/s; without the
 // loads into LDS 110-130, without the LDS reads 105-120, without both 94-104, while the clock goes from
-// 1.70 to 1.81, 1.93 and 2.12 GHz at 64-70 % busy matrix cores: the clock falls as more data moves, so
-// power, and not a unit, bounds it.  Products from registers alone reach 6.1-6.5 PFLOP/s on random codes
-// (8.1-8.8 on constant ones).  Four waves of 128 x 128, which read a third less from LDS, took 127-129 us.
+// 1.70 to 1.81, 1.93 and 2.12 GHz at 64-70 % busy matrix cores: power takes its part through the clock,
+// which falls as more data moves.  What idles the matrix cores a third of the cycles, in all four alike, is
+// not known.  Products from registers alone reach 6.1-6.5 PFLOP/s on random codes (8.1-8.8 on constant
+// ones).  Four waves of 128 x 128, which read a third less from LDS, took 127-129 us.
 #include <atomic>
 #include <type_traits>
 
@@ -140,7 +141,10 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
   const uint32_t lds_scales = lds0 + 4 * T::kHalf;
   const uint32_t lane16 = lane * 16, lane4 = lane * 4;
   // The units this wave brings in.  Unit order: wave column by wave column its matrices one after the
-  // other, then the tokens; units behind the last row tile repeat it (their sums are not stored).
+  // other, then the tokens; units behind the last row tile repeat it (their sums are not stored).  Where
+  // the units do not divide by the waves, the last one is brought in several times (the same bytes to the
+  // same place), so that every wave waits for the same number of loads: 16 for 10 units at 64 tokens, 12
+  // at 128, 14 at 192.
   __amdgpu_buffer_rsrc_t src[T::kMine];
 #pragma unroll
   for (int i = 0; i < T::kMine; ++i) {
