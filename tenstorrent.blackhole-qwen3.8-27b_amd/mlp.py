@@ -79,6 +79,12 @@ def _check_device_tensor(t, name, dtype=None):
         raise ValueError(f"{name} must be contiguous")
 
 
+def _same_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, x on {device}")
+
+
 def quantize_bfp8(w, stream=None):
     """Canonical bfp8 of a bf16 ``[rows, cols]`` GPU tensor -> ``(q int8 [rows, cols], e8 uint8 [rows, cols/16])``."""
     return _quantize(w, "bfp8", stream)
@@ -487,6 +493,14 @@ def check_formats(weights):
                          f"one of {WEIGHT_FORMATS} (bf4 takes a bfp8 down_proj)")
 
 
+def _check_one_gpu(x, weights, out, workspace, other, name):
+    """Refuses a block's tensors of more than one GPU (``other``: the argument ``name``, or None)."""
+    gpu, w1, w2, w3 = x.get_device(), weights.w1.buf, weights.w2.buf, weights.w3.buf
+    if not (w1.get_device() == w2.get_device() == w3.get_device() == out.get_device() == gpu
+            and (workspace is None or workspace.get_device() == gpu) and (other is None or other.get_device() == gpu)):
+        _same_device(x.device, w1=w1, w2=w2, w3=w3, out=out, workspace=workspace, **{name: other})
+
+
 def mlp_forward(x2d, weights, residual=None, out=None, workspace=None, stream=None, out_dtype=None):
     """``out = residual + down(silu(gate(x)) * up(x))`` for a 2-D bf16 ``[M, H]`` GPU tensor.
 
@@ -521,6 +535,7 @@ def mlp_forward(x2d, weights, residual=None, out=None, workspace=None, stream=No
             raise ValueError("out must match x")
     if out.dtype == torch.float32:
         flags |= _lib.OUT_F32
+    _check_one_gpu(x2d, weights, out, workspace, residual, "residual")
     with _lib.on_device(x2d.device):
         if workspace is None:
             workspace = new_workspace(M, H, I, weights.fmt, x2d.device, stream)
@@ -555,6 +570,7 @@ def mlp_forward_rmsnorm(h2d, norm_weight, weights, eps=1e-6, out=None, workspace
         if out.dtype not in (torch.bfloat16, torch.float32) or tuple(out.shape) != (M, H):
             raise ValueError("out must be a bf16 or fp32 [M, H] tensor")
     flags = _lib.OUT_F32 if out.dtype == torch.float32 else 0
+    _check_one_gpu(h2d, weights, out, workspace, norm_weight, "norm_weight")
     with _lib.on_device(h2d.device):
         if workspace is None:
             workspace = new_workspace(M, H, I, weights.fmt, h2d.device, stream)

@@ -26,7 +26,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .mlp import PackedWeight, _check_device_tensor, _check_mxfp4_buffer, _mxfp4_bytes
+from .mlp import PackedWeight, _check_device_tensor, _check_mxfp4_buffer, _mxfp4_bytes, _same_device
 
 _X_TYPES = {torch.bfloat16: _lib.X_BF16, torch.float16: _lib.X_F16, torch.float32: _lib.X_F32}
 
@@ -109,12 +109,6 @@ def quantize_mxfp4(x, norm_weight=None, eps=1e-6, stream=None):
                                                      buf.data_ptr(), nbytes, _lib.device_stream(device, stream))
         _lib.check(rc, "quantize_mxfp4")
     return MxTensor(buf, M, K)
-
-
-def _same_device(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, x on {device}")
 
 
 def _check_buffers(x, **weights):

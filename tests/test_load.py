@@ -100,6 +100,9 @@ class _OnGpu1(torch.Tensor):
     def device(self):
         return torch.device("cuda", 1)
 
+    def get_device(self):
+        return 1
+
 
 class _Calls:
     """A library whose calls succeed; ``made`` holds (name, current GPU, stream) of each."""
@@ -173,3 +176,37 @@ def test_the_block_runs_on_its_input_gpu(pkg, calls, fmt):
                                                  "qmlp_forward_rmsnorm", "qmlp_forward_ex", "qmlp_forward_rmsnorm"]
     assert [(gpu, getattr(stream, "value", stream)) for _, gpu, stream in calls.made] == 6 * [(1, 101)]
     assert calls.current == 0
+
+
+class _OnGpu0(torch.Tensor):
+    @property
+    def device(self):
+        return torch.device("cuda", 0)
+
+    def get_device(self):
+        return 0
+
+
+def test_the_block_refuses_tensors_of_two_gpus(pkg, calls):
+    """A kernel that is given another GPU's pointer may fault; nothing is launched."""
+    def tensor(*size, dtype=torch.bfloat16, gpu=_OnGpu1):
+        return torch.zeros(*size, dtype=dtype).as_subclass(gpu)
+
+    def weights(other=None):
+        bufs = {n: tensor(64, dtype=torch.uint8, gpu=_OnGpu0 if n == other else _OnGpu1) for n in ("w1", "w2", "w3")}
+        return pkg.MLPWeights(**{n: pkg.PackedWeight(b, *((H, I) if n == "w2" else (I, H)), "mxfp4") for n, b in bufs.items()})
+
+    x, norm, there = tensor(4, H), tensor(H), tensor(4, H, gpu=_OnGpu0)
+    for name in ("w1", "w2", "w3"):
+        for f in (lambda w: pkg.mlp_forward(x, w), lambda w: pkg.mlp_forward_rmsnorm(x, norm, w)):
+            with pytest.raises(ValueError, match=f"{name} is on cuda:0, x on cuda:1"):
+                f(weights(name))
+    for kw in (dict(residual=there), dict(out=there), dict(workspace=there)):
+        with pytest.raises(ValueError, match="is on cuda:0"):
+            pkg.mlp_forward(x, weights(), **kw)
+        if "residual" not in kw:
+            with pytest.raises(ValueError, match="is on cuda:0"):
+                pkg.mlp_forward_rmsnorm(x, norm, weights(), **kw)
+    with pytest.raises(ValueError, match="norm_weight"):
+        pkg.mlp_forward_rmsnorm(x, tensor(H, gpu=_OnGpu0), weights())
+    assert calls.made == []
