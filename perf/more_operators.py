@@ -3,9 +3,10 @@ compared.
 
 A server that keeps its projections in MXFP4 (32 consecutive K values share a power-of-two scale) and
 wants more of the activations than 4 bits runs, for each half of a decoder layer: ``norm`` (the
-attention's output added to the residual stream, the zero-centred RMSNorm of the sum, and that in MXFP8:
-e4m3 values, 32 to a power-of-two scale), ``linear`` and ``swiglu`` (products of 8-bit activations and
-4-bit weights), and beside each projection ``lora`` (the low-rank adapters of many requests at once).
+attention's output added to the residual stream, the zero-centred RMSNorm of the sum, and that in
+MXINT8: 8-bit integers, 32 to a power-of-two scale), ``linear`` and ``swiglu`` (products of 8-bit
+activations and 4-bit weights), and beside each projection ``lora`` (the low-rank adapters of many
+requests at once).
 
 Fields of a case: ``kind``; ``tokens`` M; ``k`` (input features); ``n`` (output features; 0 for "norm");
 ``dtype`` of the activations ("bf16", "f16", "f32"); ``residual`` ("bf16", "f32" or "": what is added:
@@ -187,15 +188,12 @@ def prepare(case, seed):
 # ---------------------------------------------------------------- one pass
 
 
-def _mxfp8(x):
-    """The values that MXFP8 makes of x: a block's scale is its maximum's binade less 8, a value is
-    rounded half to even to four significant bits (steps of 2^-9 below 2^-6) and to 448 beyond."""
+def _mxint8(x):
+    """The values that MXINT8 makes of x: 127 steps to either side, the step a 64th of the binade of the
+    block's maximum; rounded half to even, 128 steps to 127."""
     v = x.float().reshape(x.shape[0], -1, 32)
-    e = (torch.frexp(v.abs().amax(dim=2, keepdim=True))[1] - 1).clamp(min=-116) - 8
-    v = torch.ldexp(v, -e)
-    step = (torch.frexp(v)[1] - 1).clamp(min=-6) - 3
-    r = torch.ldexp(torch.round(torch.ldexp(v, -step)), step).clamp(-448.0, 448.0)
-    return torch.ldexp(r, e).reshape(x.shape)
+    e = (torch.frexp(v.abs().amax(dim=2, keepdim=True))[1] - 1).clamp(-120, 126) - 6
+    return torch.ldexp(torch.round(torch.ldexp(v, -e)).clamp(-127.0, 127.0), e).reshape(x.shape)
 
 
 def _weight_values(codes, scales):
@@ -212,7 +210,7 @@ def run(state):
     if own:
         pkg = _package()
         if kind == "norm":
-            h, n = pkg.add_rmsnorm(x, residual, state["norm"], eps=EPS, output="mxfp8")
+            h, n = pkg.add_rmsnorm(x, residual, state["norm"], eps=EPS, output="mxint8")
             return h, pkg.dequantize(n, dtype=torch.bfloat16)
         if kind == "linear":
             return pkg.w4a8_linear(x, state["w"][0], residual=residual, out_dtype=dtype)
@@ -223,14 +221,14 @@ def run(state):
         h = (x.float() + residual.float()).to(residual.dtype)
         f = h.float()
         f = f * torch.rsqrt(f.square().mean(dim=1, keepdim=True) + EPS) * (1 + state["norm"].float())
-        return h, _mxfp8(f.bfloat16()).bfloat16()
+        return h, _mxint8(f.bfloat16()).bfloat16()
     if kind == "lora":
         L, R, K = state["a"].shape
         mine = (state["ids"].unsqueeze(1) == torch.arange(L, device=x.device)) * state["scale"]
         s = (x.float() @ state["a"].float().reshape(L * R, K).T).reshape(-1, L, R) * mine.unsqueeze(2)
         y = s.reshape(-1, L * R) @ state["b"].float().permute(0, 2, 1).reshape(L * R, -1)
     else:
-        v = _mxfp8(x)
+        v = _mxint8(x)
         w = [_weight_values(*q) for q in state["w"]]
         y = v @ w[0].T
         if kind == "swiglu":
@@ -269,13 +267,11 @@ def _exact_mxfp4(w):
     return (torch.sign(v) * r * scale).reshape(w.shape)
 
 
-def _exact_mxfp8(x):
-    """Elements as the e4m3 type defines them, after the block's scale has put its largest into [256, 512)."""
+def _exact_mxint8(x):
     v = x.double().reshape(x.shape[0], -1, 32)
     top = v.abs().amax(dim=2, keepdim=True)
-    scale = torch.exp2(torch.floor(torch.log2(top.clamp(min=2.0 ** -116))) - 8)
-    r = (v / scale).clamp(-448.0, 448.0).to(torch.float8_e4m3fn).double()
-    return (r * scale).reshape(x.shape)
+    step = torch.exp2(torch.floor(torch.log2(top.clamp(min=2.0 ** -120)))) / 64
+    return (torch.round(v / step).clamp(-127.0, 127.0) * step).reshape(x.shape)
 
 
 def exact(case, seed):
@@ -285,7 +281,7 @@ def exact(case, seed):
         h = (x.double() + residual.double()).to(residual.dtype)  # the residual stream keeps its type
         d = h.double()
         d = d / torch.sqrt((d * d).sum(dim=1, keepdim=True) / case["k"] + EPS) * (1 + t["norm"].double())
-        return x.double() + residual.double(), _exact_mxfp8(d.bfloat16())  # the norm hands over bf16 values
+        return x.double() + residual.double(), _exact_mxint8(d.bfloat16())  # the norm hands over bf16 values
     if case["kind"] == "lora":
         y = torch.zeros(case["tokens"], case["n"], dtype=torch.float64, device="cuda")
         for a, (down, up, scale) in enumerate(t["adapters"]):
@@ -293,7 +289,7 @@ def exact(case, seed):
             if len(rows):
                 y[rows] = scale * torch.mm(torch.mm(x[rows].double(), down.double().T), up.double().T)
     else:
-        v = _exact_mxfp8(x)
+        v = _exact_mxint8(x)
         w = [_exact_mxfp4(m) for m in t["w"]]
         y = torch.mm(v, w[0].T)
         if case["kind"] == "swiglu":
