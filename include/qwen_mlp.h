@@ -235,6 +235,65 @@ int qmlp_mx_swiglu(const void* x, int x_type, int64_t x_stride, const void* wg, 
  * range, which the product refuses. */
 size_t qmlp_mx_workspace_bytes(int M, int N, int K, int x_type);
 
+/* ---------------------------------------------------------------- 8-bit activations, 4-bit weights
+ *
+ * The products of the section above with the activations in 8 bits: MXINT8, 32 consecutive K values
+ * share a power-of-two scale and each is an integer q in -127..127.  A block whose largest magnitude
+ * lies in [2^E, 2^(E+1)) has the step 2^(E-6), with E kept in [-120, 126]; values are rounded half to
+ * even, magnitudes beyond 127 steps become 127; a block with an infinity or a NaN becomes NaN as a whole,
+ * and so does every output of its row.  The weights are packed QMLP_FMT_MXFP4.  The products and their
+ * sums are as exact as those of two 4-bit operands.  A packed activation matrix takes
+ * qmlp_mxint8_bytes(rows, cols) bytes (8.25 bits a value) and feeds any number of products. */
+#define QMLP_X_MXINT8 4  /* a packed MXINT8 matrix, as x_type of the qmlp_w4a8_* products */
+#define QMLP_OUT_MXINT8 8 /* flag of qmlp_w4a8_swiglu: out is a packed MXINT8 matrix [M, N] */
+
+/* Bytes of a packed MXINT8 matrix (host only); 0 for sizes that are not supported (cols not a multiple
+ * of 32). */
+size_t qmlp_mxint8_bytes(int rows, int cols);
+
+/* x [rows, cols] (x_type BF16, F16 or F32, as for qmlp_mx_quantize) -> packed. */
+int qmlp_mxint8_quantize(const void* x, int x_type, int64_t x_stride, int rows, int cols, void* packed,
+                         size_t packed_bytes, qmlp_stream_t stream);
+
+/* Packed -> bf16 or fp32 [rows, cols] (out_type QMLP_X_BF16 or QMLP_X_F32), exactly. */
+int qmlp_mxint8_dequantize(const void* packed, int rows, int cols, void* out, int out_type, qmlp_stream_t stream);
+
+/* Packed -> the integers (int8 [rows, cols]) and scale bytes E + 127 (uint8 [rows, cols/32]; 255: not a
+ * number). */
+int qmlp_mxint8_unpack(const void* packed, int rows, int cols, void* q, void* scales, qmlp_stream_t stream);
+
+/* The residual's addition and the decoder's zero-centred RMSNorm of the sum, in one pass
+ * (layer.py:352-357 with the addition in front):
+ *
+ *   h = residual + x,   n = bf16(h / sqrt(mean(h^2) + eps) * (1 + norm_w)),   packed = MXINT8(n)
+ *
+ *   x         bf16 or fp32 [rows, cols]; residual: bf16 or fp32, or null (then h must be null, and the
+ *             norm is that of x)
+ *   norm_w    bf16 [cols]
+ *   h         [rows, cols] of the residual's type, to which the sum is rounded before the norm; may be the
+ *             residual itself (with its stride)
+ *   n         bf16 [rows, cols] contiguous, or null; packed: a packed MXINT8 matrix, or null; not both null
+ * Strides count elements from row to row and are multiples of 16 bytes.  Outputs must not overlap each other
+ * or (but for h on the residual) an input. */
+int qmlp_add_rmsnorm(const void* x, int x_type, int64_t x_stride, const void* residual, int residual_type,
+                     int64_t residual_stride, const void* norm_w, float eps, int rows, int cols, void* h,
+                     int64_t h_stride, void* n, void* packed, size_t packed_bytes, qmlp_stream_t stream);
+
+/* qmlp_mx_linear with 8-bit activations: x BF16, F16 or F32 rows, quantised in the call, or QMLP_X_MXINT8. */
+int qmlp_w4a8_linear(const void* x, int x_type, int64_t x_stride, const void* w, const void* residual,
+                     void* out, void* ws, size_t ws_bytes, int M, int N, int K, int flags,
+                     qmlp_stream_t stream);
+
+/* out[M, N] = silu(x Wg^T + gate_add) * (x Wu^T + up_add): qmlp_mx_swiglu with 8-bit activations.  gate_add
+ * and up_add: fp32 [M, N] or null, what low-rank adapters add to the projections.  flags: QMLP_OUT_F32 or
+ * QMLP_OUT_MXINT8 (N a multiple of 256; quantised from the fp32 values). */
+int qmlp_w4a8_swiglu(const void* x, int x_type, int64_t x_stride, const void* wg, const void* wu,
+                     const float* gate_add, const float* up_add, void* out, void* ws, size_t ws_bytes, int M,
+                     int N, int K, int flags, qmlp_stream_t stream);
+
+/* Workspace bytes of the two products (host only), like qmlp_mx_workspace_bytes; it may hold anything. */
+size_t qmlp_w4a8_workspace_bytes(int M, int N, int K, int x_type);
+
 /* Workspace bytes needed by qmlp_forward for these sizes (host only, no GPU needed).  The size
  * never decreases as M grows, so a workspace sized for M serves every call with fewer tokens, and
  * one workspace serves calls of different shapes as long as it is large enough for each. */
@@ -306,6 +365,9 @@ int qmlp_plan_split(int rows, int K, int nmat, int M, int num_cus, int* out6);
  * per 32 features and 32 tokens, 1 the same with twice the loads under way, 2 of eight waves, 3 per 32
  * features and 64 tokens, 3 + h tiles of 256 features (of both matrices together) x 64 h tokens. */
 int qmlp_mx_plan(int M, int N, int K, int nmat, int num_cus, int* out5);
+
+/* The same for the products with 8-bit activations (tiles of 64 and 128 tokens only: h = 1, 2). */
+int qmlp_w4a8_plan(int M, int N, int K, int nmat, int num_cus, int* out5);
 
 #ifdef __cplusplus
 }

@@ -29,6 +29,7 @@ from .mlp import (
     workspace_pool,
 )
 from .mxfp4 import MxTensor, mxfp4_linear, mxfp4_swiglu, quantize_mxfp4
+from .w4a8 import Mx8Tensor, add_rmsnorm, quantize_mxint8, w4a8_linear, w4a8_swiglu
 
 __all__ = [
     "FMT_BF4", "FMT_BF16", "FMT_BFP8", "FMT_MXFP4", "LIB_PATH", "QmlpError", "lib", "MATRIX_FORMATS", "WEIGHT_FORMATS",
@@ -36,4 +37,5 @@ __all__ = [
     "mlp_forward_rmsnorm", "new_workspace", "pack_canonical", "pack_canonical_bfp8", "pack_weight", "quantize_bf4",
     "quantize_bfp8", "unpack_bfp8", "unpack_canonical", "workspace_bytes", "WorkspacePool", "workspace_pool",
     "MxTensor", "mxfp4_linear", "mxfp4_swiglu", "quantize_mxfp4",
+    "Mx8Tensor", "add_rmsnorm", "quantize_mxint8", "w4a8_linear", "w4a8_swiglu",
 ]

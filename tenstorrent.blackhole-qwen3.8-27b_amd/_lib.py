@@ -21,7 +21,8 @@ QMLP_OK = 0
 OUT_F32 = 1
 RESIDUAL_F32 = 2
 OUT_MXFP4 = 4
-X_BF16, X_F16, X_F32, X_MXFP4 = 0, 1, 2, 3  # QMLP_X_*
+OUT_MXINT8 = 8
+X_BF16, X_F16, X_F32, X_MXFP4, X_MXINT8 = 0, 1, 2, 3, 4  # QMLP_X_*
 WS_COUNTER_BYTES = 524288  # QMLP_WS_COUNTER_BYTES
 SCRATCH_BYTES = 33554432  # QMLP_SCRATCH_BYTES
 E_SHAPE, E_ALIGN, E_FORMAT, E_LAUNCH, E_WORKSPACE, E_NULL, E_DEVICE = -1, -2, -3, -4, -5, -6, -7
@@ -62,6 +63,15 @@ SIGNATURES = {
     "qmlp_mx_swiglu": (_I, [_P, _I, _L, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _P]),
     "qmlp_mx_plan": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(ctypes.c_int)]),
     "qmlp_mx_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
+    "qmlp_mxint8_bytes": (_SZ, [_I, _I]),
+    "qmlp_mxint8_quantize": (_I, [_P, _I, _L, _I, _I, _P, _SZ, _P]),
+    "qmlp_mxint8_dequantize": (_I, [_P, _I, _I, _P, _I, _P]),
+    "qmlp_mxint8_unpack": (_I, [_P, _I, _I, _P, _P, _P]),
+    "qmlp_add_rmsnorm": (_I, [_P, _I, _L, _P, _I, _L, _P, ctypes.c_float, _I, _I, _P, _L, _P, _P, _SZ, _P]),
+    "qmlp_w4a8_linear": (_I, [_P, _I, _L, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _P]),
+    "qmlp_w4a8_swiglu": (_I, [_P, _I, _L, _P, _P, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _P]),
+    "qmlp_w4a8_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
+    "qmlp_w4a8_plan": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(ctypes.c_int)]),
 }
 
 _lib = None

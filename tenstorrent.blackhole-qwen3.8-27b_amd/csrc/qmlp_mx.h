@@ -125,12 +125,15 @@ __device__ __forceinline__ f32x16 mx_product(i32x4 a, i32x4 b, f32x16 c, uint32_
 constexpr int kMxRowsOut = 0;  // out[m, n] = sum (+ residual), bf16 or fp32
 constexpr int kMxGated = 1;    // out[m, n] = silu(gate) * up, bf16 or fp32
 constexpr int kMxPacked = 2;   // the same, quantised into a packed activation matrix
+constexpr int kMxPacked8 = 3;  // the same, as MXINT8 (qmlp_mx8.h)
 
 struct MxOut {
   void* out;
   const void* residual;  // kMxRowsOut only, may be null
   int M, N;
   int out_f32, res_f32;
+  const float* gate_add;  // gated modes of 8-bit activations: fp32 [M, N] added to the matrices' sums in
+  const float* up_add;    // front of the SiLU, may be null
 };
 
 // One product: packed activations x [M, K] times one packed weight matrix [N, K], or two of them.
@@ -144,10 +147,11 @@ struct MxProduct {
   int x_type;        // QMLP_X_*
   size_t row_bytes;  // of unpacked rows
   void* parts;       // kMxPartBytes for the partial tiles of split K ranges (many tokens)
+  bool a8;           // activations in 8 bits (MXINT8) instead of 4
 };
 constexpr size_t kMxPartBytes = 64u << 20;
 constexpr int kMxInside = 4;  // at most this many token rows are quantised inside the streamed product
-bool mx_quantizes_inside(int M, int K);
+bool mx_quantizes_inside(int M, int K, bool a8);
 constexpr int kMxFewTokens = 32;  // up to here every product is streamed
 
 // How a product runs (mx_plan, qmlp_mx_plan.hip).  Streamed: a workgroup of 32 features x 32 tokens, four
@@ -161,7 +165,7 @@ struct MxPlan {
   int workgroups;
   size_t part_bytes;  // of all pieces
 };
-MxPlan mx_plan(int M, int N, int K, int nmat, int num_cus);
+MxPlan mx_plan(int M, int N, int K, int nmat, int num_cus, bool a8);
 int launch_mx_stream(const MxProduct& p, const MxPlan& pl, hipStream_t s);
 int launch_mx_tiled(const MxProduct& p, const MxPlan& pl, hipStream_t s);
 int launch_mx_quantize(const void* x, int type, size_t row_bytes, int rows, int cols, void* packed, hipStream_t s);
@@ -177,6 +181,18 @@ int launch_mx_dequantize(const void* packed, int rows, int cols, void* out, bool
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t mx_bf16x2(float a, float b) {
   return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+}
+
+// Four neighbouring features of an fp32 [M, N] matrix that is added to a product's sums.
+__device__ __forceinline__ f32x4 mx_addend(const float* p, const MxOut& o, int m, int n) {
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (!p || m >= o.M || n >= o.N) return v;
+  p += (size_t)m * o.N + n;
+  if ((o.N & 3) == 0) return *(const f32x4*)p;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < o.N) v[i] = p[i];
+  return v;
 }
 
 // Four neighbouring features n..n+3 of token m.  N may be any number: rows whose length is not a

@@ -46,7 +46,7 @@ constexpr int kPieces[] = {1, 2, 3, 4, 6, 8, 12};
 // shapes; at the narrowest, 96 x 5120, streaming took 4.2 us at 2048 tokens and the planned tiles take 10.1.
 constexpr int kMostStreamed = 1024;
 
-MxPlan mx_plan(int M, int N, int K, int nmat, int num_cus) {
+MxPlan mx_plan(int M, int N, int K, int nmat, int num_cus, bool a8) {
   const double cus = num_cus;
   const long nsb = mx_ksb(K), rows = mx_row_tiles(N);
   auto up = [](long a, long b) { return (a + b - 1) / b; };
@@ -68,8 +68,9 @@ MxPlan mx_plan(int M, int N, int K, int nmat, int num_cus) {
       for (const StreamCost& c : kPairCost) streamed(c);
   }
   if (M <= kMxFewTokens) return best;
-  for (int h = 1; h <= 4; ++h) {
-    const TileCost& c = kTileCost[nmat - 1][h - 1];
+  for (int h = 1; h <= (a8 ? 2 : 4); ++h) {
+    TileCost c = kTileCost[nmat - 1][h - 1];
+    if (a8) c.unit *= 2, c.busy *= 2;
     const long ntt = up(M, 64 * h), tiles = up(N, 256 / nmat) * ntt;
     const double filled = (double)up(M, 32) / (double)(ntt * 2 * h);  // token units that hold tokens
     for (int ks : kPieces) {
@@ -94,6 +95,6 @@ MxPlan mx_plan(int M, int N, int K, int nmat, int num_cus) {
 // leaving it to a launch in front.  Inside / in front, us: one token 12.1 / 13.6 at 5120 x 17408, 10.7 /
 // 13.6 at 17408 x 5120, 19.6 / 21.4 for two such matrices, 4.1 / 5.5 at 2048 x 2048; two tokens of K = 17408
 // 13.5 / 13.6, three 14.9 / 13.6; four tokens of K = 5120 13.7 / 14.9, for two matrices 21.8 / 21.5.
-bool mx_quantizes_inside(int M, int K) { return M <= kMxInside && mx_ksb(K) * M <= 136; }
+bool mx_quantizes_inside(int M, int K, bool a8) { return M <= kMxInside && mx_ksb(K) * M <= (a8 ? 68 : 136); }
 
 }  // namespace qmlp

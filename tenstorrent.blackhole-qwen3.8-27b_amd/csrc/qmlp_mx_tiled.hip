@@ -21,7 +21,7 @@
 
 #include "../../include/qwen_mlp.h"
 #include "qmlp_internal.h"
-#include "qmlp_mx.h"
+#include "qmlp_mx8.h"
 #include "qmlp_xcd.h"
 
 namespace qmlp {
@@ -65,16 +65,23 @@ __device__ __forceinline__ void turn_fence() {
 // 24.5 us; written as the product leaves them, 16 bytes here and there, 34.6.
 constexpr int kMxTurnRow = 36;  // floats of a token's row: 8 lanes' 16-byte accesses meet no bank twice
 constexpr int kMxTurn = 32 * kMxTurnRow;
-template <int NMAT, int MODE>
+template <int NMAT, int MODE, bool A8>
 __device__ __forceinline__ void mx_finish(const MxOut& o, int tok_unit, int feat_unit, int lane, float* turn,
-                                          const f32x4 (&v)[NMAT][4]) {
+                                          f32x4 (&v)[NMAT][4]) {
   const int half = lane >> 5, row = lane & 31, m = tok_unit * 32 + row;
+  if constexpr (A8 && MODE != kMxRowsOut) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[0][k] += mx_addend(o.gate_add, o, m, feat_unit * 32 + 8 * k + 4 * half);
+      v[NMAT - 1][k] += mx_addend(o.up_add, o, m, feat_unit * 32 + 8 * k + 4 * half);
+    }
+  }
   f32x4 y[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k)
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[k][i] = MODE == kMxRowsOut ? v[0][k][i] : silu_mul(v[0][k][i], v[NMAT - 1][k][i]);
-  if constexpr (MODE != kMxPacked) {
+  if constexpr (MODE == kMxRowsOut || MODE == kMxGated) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) *(f32x4*)(turn + row * kMxTurnRow + 8 * k + 4 * half) = y[k];
     turn_fence();
@@ -92,6 +99,26 @@ __device__ __forceinline__ void mx_finish(const MxOut& o, int tok_unit, int feat
 #pragma unroll
       for (int i = 0; i < 4; ++i) mx = max(mx, __float_as_uint(y[k][i]) & 0x7fffffffu);
     mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32));
+    if constexpr (MODE == kMxPacked8) {  // each of the two lanes makes 16 neighbouring values' group
+      const uint32_t s = mx8_scale_byte(mx);
+      float f[16];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float mine = half ? y[2 + k][i] : y[k][i];
+          const float other = __shfl_xor(half ? y[k][i] : y[2 + k][i], 32);
+          f[8 * k + i] = half ? other : mine;
+          f[8 * k + 4 + i] = half ? mine : other;
+        }
+      const i32x4 group = mx8_group(f, s);
+      if (m < o.M && feat_unit * 32 < o.N) {
+        uint8_t* unit = (uint8_t*)o.out + ((size_t)tok_unit * mx_ksb(o.N) + feat_unit / 8) * kMx8Unit;
+        *(i32x4*)(unit + mx8_at(row, feat_unit % 8, half)) = group;
+        if (half == 0) unit[mx8_scale_at(row, feat_unit % 8)] = (uint8_t)s;
+      }
+      return;
+    }
     const uint32_t s = mx_scale_byte(mx);
     u32x4 c;
 #pragma unroll
@@ -108,27 +135,29 @@ __device__ __forceinline__ void mx_finish(const MxOut& o, int tok_unit, int feat
   }
 }
 
-// NF x NT waves, each WF x WT products of 32 features x 32 tokens (WF: of all matrices together).
-template <int NMAT, int WF, int WT, int NF, int NT>
+// NF x NT waves, each WF x WT products of 32 features x 32 tokens (WF: of all matrices together).  8-bit
+// activations (XP = 2): a token unit's two planes are loaded and kept like two units of 4-bit codes, each with
+// the scales, and a product is two, one for each digit.
+template <int NMAT, int WF, int WT, int NF, int NT, int XP>
 struct MxTile {
   static constexpr int kWaves = NF * NT;
   static constexpr int kFeatUnits = WF * NF;
   static constexpr int kTokUnits = WT * NT;
-  static constexpr int kUnits = kFeatUnits + kTokUnits;
+  static constexpr int kUnits = kFeatUnits + kTokUnits * XP;
   static constexpr int kFeatures = 32 * kFeatUnits / NMAT;
   static constexpr int kTokens = 32 * kTokUnits;
   static constexpr int kHalf = kUnits * (kMxCodes / 2);  // codes of 128 K
   static constexpr int kLds = 4 * kHalf + 2 * kUnits * 256;
   static constexpr int kMine = (kUnits + kWaves - 1) / kWaves;  // units a wave brings in
-  static_assert(kLds <= 160 * 1024 && WF * WT % 2 == 0, "tile");
+  static_assert(kLds <= 160 * 1024 && WF * WT * XP % 2 == 0, "tile");
 };
 
-template <int NMAT, int WF, int WT, int NF, int NT, int MODE>
+template <int NMAT, int WF, int WT, int NF, int NT, int MODE, int XP>
 __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t* __restrict__ x,
                                                                   const uint8_t* __restrict__ w0,
                                                                   const uint8_t* __restrict__ w1, int nsb, int ntt,
                                                                   int ks, f32x4* __restrict__ parts, MxOut o) {
-  using T = MxTile<NMAT, WF, WT, NF, NT>;
+  using T = MxTile<NMAT, WF, WT, NF, NT, XP>;
   extern __shared__ __align__(16) uint8_t s_stage[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wf = wave % NF, wt = wave / NF;
@@ -146,19 +175,30 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
   // same place), so that every wave waits for the same number of loads: 16 for 10 units at 64 tokens, 12
   // at 128, 14 at 192.
   __amdgpu_buffer_rsrc_t src[T::kMine];
+  int unit_bytes[T::kMine], scales_at[T::kMine];
 #pragma unroll
   for (int i = 0; i < T::kMine; ++i) {
     const int u = min(wave * T::kMine + i, T::kUnits - 1);  // the last one again where they do not divide
     const uint8_t* p;
+    int extent = n * kMxUnit;
+    unit_bytes[i] = kMxUnit;
+    scales_at[i] = kMxCodes;
     if (u < T::kFeatUnits) {
       constexpr int per = WF / NMAT;
       const int col = u / WF, mat = (u % WF) / per, f = col * per + u % per;
       const int row = min(ft * (T::kFeatUnits / NMAT) + f, ftiles - 1);
       p = (NMAT > 1 && mat ? w1 : w0) + (size_t)row * nsb * kMxUnit;
+      p += (size_t)u0 * kMxUnit;
+    } else if constexpr (XP == 1) {
+      p = x + ((size_t)min(tt * T::kTokUnits + u - T::kFeatUnits, ttiles - 1) * nsb + u0) * kMxUnit;
     } else {
-      p = x + (size_t)min(tt * T::kTokUnits + u - T::kFeatUnits, ttiles - 1) * nsb * kMxUnit;
+      const int v = u - T::kFeatUnits, plane = v % XP * kMx8Plane;
+      p = x + ((size_t)min(tt * T::kTokUnits + v / XP, ttiles - 1) * nsb + u0) * kMx8Unit + plane;
+      unit_bytes[i] = kMx8Unit;
+      scales_at[i] = kMx8Codes - plane;
+      extent = n * kMx8Unit - plane;
     }
-    src[i] = __builtin_amdgcn_make_buffer_rsrc((void*)(p + (size_t)u0 * kMxUnit), 0, n * kMxUnit, kBufferRsrcWord3);
+    src[i] = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, extent, kBufferRsrcWord3);
   }
   // A half of a K unit comes in two parts, half of the wave's units each: load k of part `part` of half h
   // of unit sb.  The codes go to slot 2 (sb % 2) + h, with half 0 the unit's scales.
@@ -168,10 +208,10 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
     if (k >= per * (part ? kPart1 : kPart0)) return;
     const int u = min(wave * T::kMine + i, T::kUnits - 1);
     if (c < 2)
-      load_lds16(src[i], lane16, sb * kMxUnit + 2048 * h + 1024 * c,
+      load_lds16(src[i], lane16, sb * unit_bytes[i] + 2048 * h + 1024 * c,
                    lds0 + (2 * (sb & 1) + h) * T::kHalf + u * 2048 + c * 1024);
     else
-      load_lds4(src[i], lane4, sb * kMxUnit + kMxCodes, lds_scales + ((sb & 1) * T::kUnits + u) * 256);
+      load_lds4(src[i], lane4, sb * unit_bytes[i] + scales_at[i], lds_scales + ((sb & 1) * T::kUnits + u) * 256);
   };
   auto issue_all = [&](int sb, int h, int part) {
 #pragma unroll
@@ -182,24 +222,25 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
   for (int f = 0; f < WF; ++f)
 #pragma unroll
     for (int t = 0; t < WT; ++t) acc[f][t] = f32x16{};
-  i32x4 a[2][WF], b[2][WT];
+  constexpr int kB = WT * XP;  // token operands of a K-step
+  i32x4 a[2][WF], b[2][kB];
   uint32_t fs[WF], xs[WT], fs_next[WF], xs_next[WT];
   const uint8_t* sf = s_stage + wf * WF * 2048 + lane16;
-  const uint8_t* sx = s_stage + (T::kFeatUnits + wt * WT) * 2048 + lane16;
+  const uint8_t* sx = s_stage + (T::kFeatUnits + wt * kB) * 2048 + lane16;
   const uint8_t* sc = s_stage + 4 * T::kHalf + lane4;
   // operand k of one K-step of the wave: its first feature unit, its tokens, its other feature units
   auto fetch = [&](int sb, int h, int j, int k) {
     const uint32_t at = (2 * (sb & 1) + h) * T::kHalf + j * 1024;
-    if (k >= WF + WT) return;
-    if (k >= 1 && k <= WT)
+    if (k >= WF + kB) return;
+    if (k >= 1 && k <= kB)
       b[j][k - 1] = *(const i32x4*)(sx + at + (k - 1) * 2048);
     else
-      a[j][k ? k - WT : 0] = *(const i32x4*)(sf + at + (k ? k - WT : 0) * 2048);
+      a[j][k ? k - kB : 0] = *(const i32x4*)(sf + at + (k ? k - kB : 0) * 2048);
   };
   auto fetch_scale = [&](int sb, int k) {
     const uint8_t* s = sc + (sb & 1) * T::kUnits * 256;
     if (k < WT)
-      xs_next[k] = *(const uint32_t*)(s + (T::kFeatUnits + wt * WT + k) * 256);
+      xs_next[k] = *(const uint32_t*)(s + (T::kFeatUnits + wt * kB + k * XP) * 256);
     else if (k < WF + WT)
       fs_next[k - WT] = *(const uint32_t*)(s + (wf * WF + k - WT) * 256);
   };
@@ -209,12 +250,25 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
   const int nv = max(0, min(mine_f, ttiles - (tt * T::kTokUnits + wt * WT)));
   // One K-step's products, in groups of two; before each group `beside(group)` asks for what comes in
   // beside them (the order is kept as written).
-  constexpr int kGroups = WF * WT / 2;
+  constexpr int kGroups = WF * WT * XP / 2;
+  i32x8 low[XP == 2 ? WT : 1], high[XP == 2 ? WT : 1];  // the digits of a K-step's token operands
   auto multiply = [&](auto jc, auto full, auto beside) {
     constexpr int J = decltype(jc)::value;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       beside(g);
+      if constexpr (XP == 2) {
+        const int f = g / WT, t = g % WT;
+        if (f == 0) {
+          low[t] = high[t] = i32x8{};
+          mx8_digits(b[J & 1][2 * t], 0, low[t], high[t]);
+          mx8_digits(b[J & 1][2 * t + 1], 1, low[t], high[t]);
+        }
+        if (decltype(full)::value || t < nv)
+          acc[f][t] = mx8_product<J>(a[J & 1][f], low[t], high[t], acc[f][t], fs[f], xs[t]);
+        __builtin_amdgcn_sched_barrier(0);
+        continue;
+      }
 #pragma unroll
       for (int k = 2 * g; k < 2 * g + 2; ++k) {
         const int f = k / WT, t = k % WT;
@@ -244,22 +298,22 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
 #pragma unroll
     for (int f = 0; f < WF; ++f) fs[f] = fs_next[f];
     multiply(std::integral_constant<int, 0>{}, full, [&](int g) {
-      spread(g, WF + WT, [&](int k) { fetch(sb, 0, 1, k); });
+      spread(g, WF + kB, [&](int k) { fetch(sb, 0, 1, k); });
       if constexpr (LEFT >= 1) spread(g, 2 * kPart1, [&](int k) { issue(sb + 1, 1, 1, k); });
     });
     stage_barrier<(LEFT >= 1 ? kAhead : 0)>();
     multiply(std::integral_constant<int, 1>{}, full, [&](int g) {
-      spread(g, WF + WT, [&](int k) { fetch(sb, 1, 0, k); });
+      spread(g, WF + kB, [&](int k) { fetch(sb, 1, 0, k); });
       if constexpr (LEFT >= 2) spread(g, 3 * kPart0, [&](int k) { issue(sb + 2, 0, 0, k); });
     });
     multiply(std::integral_constant<int, 2>{}, full, [&](int g) {
-      spread(g, WF + WT, [&](int k) { fetch(sb, 1, 1, k); });
+      spread(g, WF + kB, [&](int k) { fetch(sb, 1, 1, k); });
       if constexpr (LEFT >= 2) spread(g, 3 * kPart1, [&](int k) { issue(sb + 2, 0, 1, k); });
     });
     stage_barrier<(LEFT >= 2 ? kAhead : 0)>();
     multiply(std::integral_constant<int, 3>{}, full, [&](int g) {
       if constexpr (LEFT >= 1) {
-        spread(g, WF + WT, [&](int k) { fetch(sb + 1, 0, 0, k); });
+        spread(g, WF + kB, [&](int k) { fetch(sb + 1, 0, 0, k); });
         spread(g, WF + WT, [&](int k) { fetch_scale(sb + 1, k); });
       }
       if constexpr (LEFT >= 2) spread(g, 2 * kPart0, [&](int k) { issue(sb + 2, 1, 0, k); });
@@ -278,7 +332,7 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
     stage_barrier<T::kMine * 2>();
   }
 #pragma unroll
-  for (int k = 0; k < WF + WT; ++k) {
+  for (int k = 0; k < WF + kB; ++k) {
     fetch_scale(0, k);
     fetch(0, 0, 0, k);
   }
@@ -308,7 +362,7 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
   }
   static_assert(T::kLds >= T::kWaves * kMxTurn * 4);
   float* turn = (float*)s_stage + wave * kMxTurn;
-  if constexpr (MODE != kMxPacked) __syncthreads();  // the stages' readers are done
+  if constexpr (MODE == kMxRowsOut || MODE == kMxGated) __syncthreads();  // the stages' readers are done
 #pragma unroll
   for (int t = 0; t < WT; ++t) {
     if (t >= nv) break;
@@ -321,7 +375,7 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
         for (int m = 0; m < NMAT; ++m)
 #pragma unroll
           for (int i = 0; i < 4; ++i) v[m][k][i] = acc[f + m * per][t][4 * k + i];
-      mx_finish<NMAT, MODE>(o, tt * T::kTokUnits + wt * WT + t, ft * (T::kFeatUnits / NMAT) + wf * per + f, lane,
+      mx_finish<NMAT, MODE, XP == 2>(o, tt * T::kTokUnits + wt * WT + t, ft * (T::kFeatUnits / NMAT) + wf * per + f, lane,
                             turn, v);
     }
   }
@@ -330,10 +384,10 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
 // Adds the pieces of split tiles up, in K order (deterministic), and finishes them: one wave for 32
 // features x 32 tokens.  Bound by its reads and its launch: 4.1-4.8 us for 15.7 MB of pieces (201 tokens of
 // 5120 x 8704).  A launch of its own, so that every CU takes part and no block waits for another.
-template <int NMAT, int WF, int WT, int NF, int NT, int MODE>
+template <int NMAT, int WF, int WT, int NF, int NT, int MODE, int XP>
 __global__ __launch_bounds__(256) void mx_sum_kernel(const f32x4* __restrict__ parts, int tiles, int ntt, int ks,
                                                      MxOut o) {
-  using T = MxTile<NMAT, WF, WT, NF, NT>;
+  using T = MxTile<NMAT, WF, WT, NF, NT, XP>;
   constexpr int per = WF / NMAT, kItems = T::kWaves * per * WT;
   __shared__ __align__(16) float s_turn[4][kMxTurn];
   const int lane = threadIdx.x & 63;
@@ -356,13 +410,13 @@ __global__ __launch_bounds__(256) void mx_sum_kernel(const f32x4* __restrict__ p
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[m][k] += at[(((f + m * per) * WT + t) * 4 + k) * 64];
   }
-  mx_finish<NMAT, MODE>(o, tok, feat, lane, s_turn[threadIdx.x >> 6], v);
+  mx_finish<NMAT, MODE, XP == 2>(o, tok, feat, lane, s_turn[threadIdx.x >> 6], v);
 }
 
-template <typename T, int NMAT, int MODE, int WF, int WT, int NF, int NT>
+template <typename T, int NMAT, int MODE, int WF, int WT, int NF, int NT, int XP>
 static int launch_sum(const MxProduct& p, int tiles, int ntt, int ks, hipStream_t s) {
   constexpr int kItems = T::kWaves * WF / NMAT * WT;
-  launch_timed_part(p.slot, 2, mx_sum_kernel<NMAT, WF, WT, NF, NT, MODE>, dim3((tiles * kItems + 3) / 4), dim3(256), 0, s,
+  launch_timed_part(p.slot, 2, mx_sum_kernel<NMAT, WF, WT, NF, NT, MODE, XP>, dim3((tiles * kItems + 3) / 4), dim3(256), 0, s,
                     (const f32x4*)p.parts, tiles, ntt, ks, p.o);
   return check_launch("mx_sum_kernel");
 }
@@ -381,10 +435,10 @@ static int raise_lds_once(K kern, int bytes, std::atomic<uint64_t>& raised) {
   return 0;
 }
 
-template <int NMAT, int WF, int WT, int NF, int NT, int MODE>
+template <int NMAT, int WF, int WT, int NF, int NT, int MODE, int XP>
 static int launch_tile(const MxProduct& p, int ks, hipStream_t s) {
-  using T = MxTile<NMAT, WF, WT, NF, NT>;
-  auto kern = mx_tiled_kernel<NMAT, WF, WT, NF, NT, MODE>;
+  using T = MxTile<NMAT, WF, WT, NF, NT, XP>;
+  auto kern = mx_tiled_kernel<NMAT, WF, WT, NF, NT, MODE, XP>;
   static std::atomic<uint64_t> raised{0};
   if (int rc = raise_lds_once(kern, T::kLds, raised)) return rc;
   const int nft = (p.o.N + T::kFeatures - 1) / T::kFeatures, ntt = (p.o.M + T::kTokens - 1) / T::kTokens;
@@ -396,7 +450,7 @@ static int launch_tile(const MxProduct& p, int ks, hipStream_t s) {
                     mx_ksb(p.K), ntt, ks, (f32x4*)p.parts, p.o);
   if (int rc = check_launch("mx_tiled_kernel")) return rc;
   if constexpr (WT <= 2) {  // mx_plan splits no higher tile
-    if (ks > 1) return launch_sum<T, NMAT, MODE, WF, WT, NF, NT>(p, tiles, ntt, ks, s);
+    if (ks > 1) return launch_sum<T, NMAT, MODE, WF, WT, NF, NT, XP>(p, tiles, ntt, ks, s);
   }
   return 0;
 }
@@ -404,13 +458,26 @@ static int launch_tile(const MxProduct& p, int ks, hipStream_t s) {
 template <int MODE>
 static int launch_height(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
   constexpr int NMAT = MODE == kMxRowsOut ? 1 : 2;
-  if (pl.height == 1) return launch_tile<NMAT, 2, 1, 4, 2, MODE>(p, pl.ks, s);
-  if (pl.height == 2) return launch_tile<NMAT, 2, 2, 4, 2, MODE>(p, pl.ks, s);
-  if (pl.height == 3) return launch_tile<NMAT, 2, 3, 4, 2, MODE>(p, pl.ks, s);
-  return launch_tile<NMAT, 2, 4, 4, 2, MODE>(p, pl.ks, s);
+  if (pl.height == 1) return launch_tile<NMAT, 2, 1, 4, 2, MODE, 1>(p, pl.ks, s);
+  if (pl.height == 2) return launch_tile<NMAT, 2, 2, 4, 2, MODE, 1>(p, pl.ks, s);
+  if (pl.height == 3) return launch_tile<NMAT, 2, 3, 4, 2, MODE, 1>(p, pl.ks, s);
+  return launch_tile<NMAT, 2, 4, 4, 2, MODE, 1>(p, pl.ks, s);
+}
+
+// 8-bit activations: two heights, as far as LDS goes.
+template <int MODE>
+static int launch_height8(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
+  constexpr int NMAT = MODE == kMxRowsOut ? 1 : 2;
+  if (pl.height == 1) return launch_tile<NMAT, 2, 1, 4, 2, MODE, 2>(p, pl.ks, s);
+  return launch_tile<NMAT, 2, 2, 4, 2, MODE, 2>(p, pl.ks, s);
 }
 
 int launch_mx_tiled(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
+  if (p.a8) {
+    if (p.mode == kMxRowsOut) return launch_height8<kMxRowsOut>(p, pl, s);
+    if (p.mode == kMxGated) return launch_height8<kMxGated>(p, pl, s);
+    return launch_height8<kMxPacked8>(p, pl, s);
+  }
   if (p.mode == kMxRowsOut) return launch_height<kMxRowsOut>(p, pl, s);
   if (p.mode == kMxGated) return launch_height<kMxGated>(p, pl, s);
   return launch_height<kMxPacked>(p, pl, s);

@@ -180,6 +180,23 @@ def _check_mxfp4_buffer(t, name):
         raise ValueError(f"{name}: the buffer does not hold a packed mxfp4 [{t.rows}, {t.cols}]")
 
 
+@functools.lru_cache(maxsize=4096)
+def _mxint8_bytes(rows, cols):
+    n = _lib.lib().qmlp_mxint8_bytes(rows, cols)
+    if n == 0:
+        raise _unsupported_shape(rows, cols, "mxfp4")
+    return n
+
+
+def _check_mxint8_buffer(t, name):
+    """The packed buffer of an ``Mx8Tensor`` is what its shape needs."""
+    buf = t.buf
+    if not (isinstance(buf, torch.Tensor) and buf.is_cuda):
+        raise ValueError(f"{name} must be on the GPU")
+    if buf.dtype != torch.uint8 or not buf.is_contiguous() or buf.numel() < _mxint8_bytes(t.rows, t.cols):
+        raise ValueError(f"{name}: the buffer does not hold a packed mxint8 [{t.rows}, {t.cols}]")
+
+
 def _pack_canonical_mxfp4(codes, scales, stream):
     _check_device_tensor(codes, "q", torch.uint8)
     _check_device_tensor(scales, "e8", torch.uint8)
@@ -250,7 +267,16 @@ def unpack_bfp8(pw, stream=None):
 
 def unpack_canonical(pw, stream=None):
     """Packed bfp8 or bf4 -> canonical (q, e8) (lossless for unflushed groups); packed mxfp4 (a weight
-    or an ``MxTensor``) -> (codes, scales) (lossless)."""
+    or an ``MxTensor``) -> (codes, scales) (lossless); an ``Mx8Tensor`` -> (int8 values ``[rows, cols]`` in
+    steps of 2^(scale - 133), uint8 scales ``[rows, cols/32]``) (lossless)."""
+    if pw.fmt == "mxint8":
+        _check_mxint8_buffer(pw, "the tensor")
+        with _lib.on_device(pw.buf.device, stream):
+            q = torch.empty((pw.rows, pw.cols), dtype=torch.int8, device=pw.buf.device)
+            scales = torch.empty((pw.rows, pw.cols // 32), dtype=torch.uint8, device=pw.buf.device)
+            _lib.check(_lib.lib().qmlp_mxint8_unpack(_lib.ptr(pw.buf), pw.rows, pw.cols, _lib.ptr(q), _lib.ptr(scales),
+                                                     _lib.device_stream(pw.buf.device, stream)), "qmlp_mxint8_unpack")
+        return q, scales
     if pw.fmt == "mxfp4":
         _check_mxfp4_buffer(pw, "the tensor")
         with _lib.on_device(pw.buf.device, stream):
@@ -273,17 +299,23 @@ def unpack_canonical(pw, stream=None):
 def dequantize(pw, stream=None, dtype=torch.float32):
     """Packed weight -> float32 ``[rows, cols]`` via the kernels' own dequant routine.  mxfp4 (a weight
     or an ``MxTensor``) also to bfloat16.  Both hold every value of the format below 2^128 exactly; from
-    there on (scales of 253 and 254, which only packed checkpoints can hold) it becomes an infinity."""
-    if pw.fmt == "mxfp4":
+    there on (scales of 253 and 254, which only packed checkpoints can hold) it becomes an infinity.  An
+    ``Mx8Tensor`` to either, exactly."""
+    if pw.fmt in ("mxfp4", "mxint8"):
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("dtype must be bf16 or fp32")
-        _check_mxfp4_buffer(pw, "the tensor")
+        if pw.fmt == "mxint8":
+            _check_mxint8_buffer(pw, "the tensor")
+            fn = "qmlp_mxint8_dequantize"
+        else:
+            _check_mxfp4_buffer(pw, "the tensor")
+            fn = "qmlp_mx_dequantize"
         with _lib.on_device(pw.buf.device, stream):
             out = torch.empty((pw.rows, pw.cols), dtype=dtype, device=pw.buf.device)
-            rc = _lib.lib().qmlp_mx_dequantize(pw.buf.data_ptr(), pw.rows, pw.cols, out.data_ptr(),
-                                               _lib.X_F32 if dtype == torch.float32 else _lib.X_BF16,
-                                               _lib.device_stream(pw.buf.device, stream))
-            _lib.check(rc, "qmlp_mx_dequantize")
+            rc = getattr(_lib.lib(), fn)(pw.buf.data_ptr(), pw.rows, pw.cols, out.data_ptr(),
+                                         _lib.X_F32 if dtype == torch.float32 else _lib.X_BF16,
+                                         _lib.device_stream(pw.buf.device, stream))
+            _lib.check(rc, fn)
         return out
     if dtype != torch.float32:
         raise ValueError("dtype must be fp32")
