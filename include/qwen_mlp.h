@@ -294,6 +294,37 @@ int qmlp_w4a8_swiglu(const void* x, int x_type, int64_t x_stride, const void* wg
 /* Workspace bytes of the two products (host only), like qmlp_mx_workspace_bytes; it may hold anything. */
 size_t qmlp_w4a8_workspace_bytes(int M, int N, int K, int x_type);
 
+/* ---------------------------------------------------------------- low-rank adapters
+ *
+ * What the adapters of a batch's requests add beside one shared projection:
+ *
+ *   out[m] = base[m] + s_a B_a (A_a x[m]),   a = ids[m];  A_a [rank, K], B_a [N, rank], s_a a number
+ *
+ * for any number of adapters from 1 to 1024 of ranks from 1 to 128, which may differ.  A token whose id is
+ * outside [0, adapters) has none (out[m] = base[m]).
+ *
+ * Layouts (ranks padded to units of 16 with zeros; `first` counts the rank units of the adapters before):
+ *   a     [unit][K / 32][64][8] 16-bit values: lane l of a K-step holds rank l % 16 of the unit, K values
+ *         8 (l / 16)..; adapter after adapter
+ *   b     per adapter [N / 64, rounded up][unit][4][32][8]: in part f lane l holds ranks 8 (l / 16).. of the
+ *         unit for feature 16 (l % 16 / 4) + 4 f + l % 4 of the block (zeros behind N); adapter after adapter
+ *   meta  int32 [adapters][4]: {rank, first, the bits of s_a (fp32), 0}
+ *
+ * A plan groups a batch's tokens by adapter; it serves every projection with the same adapter numbers (all of a
+ * model's layers) until the tokens' adapters change. */
+size_t qmlp_lora_plan_bytes(int M, int adapters); /* host only; 0 for sizes out of range */
+int qmlp_lora_plan(const int32_t* ids, int M, int adapters, void* plan, size_t plan_bytes, qmlp_stream_t stream);
+
+/* x: bf16 or fp16 [M, K] (x_type; x_stride elements from row to row, a multiple of 16 bytes), the type of a and
+ * b; plan: qmlp_lora_plan's for the same M and number of adapters (with another one nothing is written);
+ * base: bf16 or fp32 [M, N] (QMLP_RESIDUAL_F32) or null; out: bf16 or fp32 [M, N] (QMLP_OUT_F32), may be base of
+ * the same type.  Sums are fp32, rounded once.  ws: qmlp_lora_workspace_bytes(M, K, max_rank) bytes that may hold
+ * anything; calls that run at the same time need separate ones. */
+int qmlp_lora_linear(const void* x, int x_type, int64_t x_stride, const void* a, const void* b, const void* meta,
+                     int adapters, int max_rank, const void* plan, const void* base, void* out, void* ws,
+                     size_t ws_bytes, int M, int N, int K, int flags, qmlp_stream_t stream);
+size_t qmlp_lora_workspace_bytes(int M, int K, int max_rank); /* host only; never shrinks as M grows */
+
 /* Workspace bytes needed by qmlp_forward for these sizes (host only, no GPU needed).  The size
  * never decreases as M grows, so a workspace sized for M serves every call with fewer tokens, and
  * one workspace serves calls of different shapes as long as it is large enough for each. */

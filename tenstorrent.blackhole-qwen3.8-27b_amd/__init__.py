@@ -29,6 +29,7 @@ from .mlp import (
     workspace_pool,
 )
 from .mxfp4 import MxTensor, mxfp4_linear, mxfp4_swiglu, quantize_mxfp4
+from .lora import LoraPlan, LoraStack, lora_linear, lora_plan, pack_lora
 from .w4a8 import Mx8Tensor, add_rmsnorm, quantize_mxint8, w4a8_linear, w4a8_swiglu
 
 __all__ = [
@@ -37,5 +38,6 @@ __all__ = [
     "mlp_forward_rmsnorm", "new_workspace", "pack_canonical", "pack_canonical_bfp8", "pack_weight", "quantize_bf4",
     "quantize_bfp8", "unpack_bfp8", "unpack_canonical", "workspace_bytes", "WorkspacePool", "workspace_pool",
     "MxTensor", "mxfp4_linear", "mxfp4_swiglu", "quantize_mxfp4",
+    "LoraPlan", "LoraStack", "lora_linear", "lora_plan", "pack_lora",
     "Mx8Tensor", "add_rmsnorm", "quantize_mxint8", "w4a8_linear", "w4a8_swiglu",
 ]

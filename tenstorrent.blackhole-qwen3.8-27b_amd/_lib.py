@@ -71,6 +71,10 @@ SIGNATURES = {
     "qmlp_w4a8_linear": (_I, [_P, _I, _L, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _P]),
     "qmlp_w4a8_swiglu": (_I, [_P, _I, _L, _P, _P, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _P]),
     "qmlp_w4a8_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
+    "qmlp_lora_plan_bytes": (_SZ, [_I, _I]),
+    "qmlp_lora_plan": (_I, [_P, _I, _I, _P, _SZ, _P]),
+    "qmlp_lora_workspace_bytes": (_SZ, [_I, _I, _I]),
+    "qmlp_lora_linear": (_I, [_P, _I, _L, _P, _P, _P, _I, _I, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _P]),
     "qmlp_w4a8_plan": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(ctypes.c_int)]),
 }
 

@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "qmlp_common.h"
 
 namespace qmlp {
@@ -27,6 +29,19 @@ int current_device_info(DeviceInfo* out);
 
 inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+// Raises a kernel's dynamic LDS limit, once per device (a mask per kernel, bit: device).
+inline int raise_lds_once(const void* kern, int bytes, std::atomic<uint64_t>& raised) {
+  int dev = -1;
+  if (hipGetDevice(&dev) != hipSuccess) return check_launch("hipGetDevice");
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(raised.load(std::memory_order_relaxed) & bit)) {
+    if (hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+      return check_launch("hipFuncSetAttribute");
+    raised.fetch_or(bit, std::memory_order_relaxed);
+  }
+  return 0;
+}
 
 // Optional per-kernel timing of the forward pass (qmlp_set_profile_events): slot 0 is the
 // gate/up kernel, slot 1 the down kernel.  profile_events() hands out the slot's start / stop

@@ -421,26 +421,12 @@ static int launch_sum(const MxProduct& p, int tiles, int ntt, int ks, hipStream_
   return check_launch("mx_sum_kernel");
 }
 
-// Raises a kernel's dynamic LDS limit, once per device (a mask per kernel, bit: device).
-template <typename K>
-static int raise_lds_once(K kern, int bytes, std::atomic<uint64_t>& raised) {
-  int dev = -1;
-  if (hipGetDevice(&dev) != hipSuccess) return check_launch("hipGetDevice");
-  const uint64_t bit = 1ull << (dev & 63);
-  if (!(raised.load(std::memory_order_relaxed) & bit)) {
-    if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
-      return check_launch("hipFuncSetAttribute");
-    raised.fetch_or(bit, std::memory_order_relaxed);
-  }
-  return 0;
-}
-
 template <int NMAT, int WF, int WT, int NF, int NT, int MODE, int XP>
 static int launch_tile(const MxProduct& p, int ks, hipStream_t s) {
   using T = MxTile<NMAT, WF, WT, NF, NT, XP>;
   auto kern = mx_tiled_kernel<NMAT, WF, WT, NF, NT, MODE, XP>;
   static std::atomic<uint64_t> raised{0};
-  if (int rc = raise_lds_once(kern, T::kLds, raised)) return rc;
+  if (int rc = raise_lds_once((const void*)kern, T::kLds, raised)) return rc;
   const int nft = (p.o.N + T::kFeatures - 1) / T::kFeatures, ntt = (p.o.M + T::kTokens - 1) / T::kTokens;
   const int tiles = nft * ntt;
   const size_t part_bytes = (size_t)tiles * ks * (T::kWaves * WF * WT * 4096);

@@ -1,0 +1,189 @@
+"""Low-rank adapters of many requests at once, beside a shared projection.
+
+* ``pack_lora([(a, b, scale), ...])`` -> ``LoraStack``: the adapters of one projection, laid out once when they
+  are loaded (``a`` ``[rank, K]``, ``b`` ``[N, rank]``, both bf16 or both fp16; ranks from 1 to 128 may differ);
+* ``lora_plan(ids, adapters)`` -> ``LoraPlan``: which tokens share an adapter, made once for a batch and used by
+  every projection of every layer; ``ids`` int32 ``[M]``, the adapter of each token (any other number: none);
+* ``lora_linear(x, stack, plan, base=...)``: ``out[m] = base[m] + scale_a b_a (a_a x[m])``.
+
+``base`` may be the shared projection's output, or what the projection adds itself: with an fp32 ``out`` the
+result is the ``residual`` of ``w4a8_linear`` and ``mxfp4_linear``, and ``gate_add`` / ``up_add`` of
+``w4a8_swiglu``, so that the sum of both is rounded once.  Sums are fp32.  Sizes: any M up to 65536, any N, K a
+multiple of 32, up to 1024 adapters.  The reference's projections have no adapters
+(``docker/qwen-c2-graft/graft/mlp.py:402-423``).
+
+Every call runs on the inputs' GPU, on ``stream`` or that GPU's current stream, may be captured into a HIP
+graph (``pack_lora`` reads its scales from the host and may not) and allocates its output and scratch memory from
+torch's caching allocator there.  A replayed graph with ``lora_plan`` in it follows new ids.  Errors:
+``ValueError`` for wrong shapes, dtypes or devices, ``QmlpError`` for launch failures.
+"""
+import functools
+import struct
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from .mlp import _check_device_tensor, _same_device
+from .mxfp4 import _check_out, _check_rows
+
+MAX_RANK = 128
+MAX_ADAPTERS = 1024
+
+
+@dataclass(frozen=True)
+class LoraStack:
+    """The adapters of one projection in the kernels' layout."""
+
+    a: torch.Tensor     # [rank units, K / 32, 64, 8], all adapters in turn
+    b: torch.Tensor     # flat, per adapter [N / 64, rank units, 4, 32, 8]
+    meta: torch.Tensor  # int32 [adapters, 4]: rank, rank units before, scale's bits, 0
+    ranks: tuple
+    n: int
+    k: int
+
+    @property
+    def adapters(self):
+        return len(self.ranks)
+
+    @property
+    def max_rank(self):
+        return max(self.ranks)
+
+    @property
+    def device(self):
+        return self.a.device
+
+    @property
+    def nbytes(self):
+        return sum(t.numel() * t.element_size() for t in (self.a, self.b, self.meta))
+
+
+@dataclass(frozen=True)
+class LoraPlan:
+    """A batch's tokens grouped by adapter."""
+
+    buf: torch.Tensor  # int32, qmlp_lora_plan_bytes(tokens, adapters) bytes
+    tokens: int
+    adapters: int
+
+
+def _units(rank):
+    return -(-rank // 16)
+
+
+def pack_lora(adapters, stream=None):
+    """``[(a [rank, K], b [N, rank], scale), ...]`` (GPU tensors, a number) -> ``LoraStack``.  ``scale`` is what the
+    adapter's product is multiplied by (``alpha / rank`` as a rule)."""
+    adapters = list(adapters)
+    if not 1 <= len(adapters) <= MAX_ADAPTERS:
+        raise ValueError(f"need 1 to {MAX_ADAPTERS} adapters, got {len(adapters)}")
+    first = adapters[0][0]
+    for i, (a, b, scale) in enumerate(adapters):
+        for name, t in (("a", a), ("b", b)):
+            _check_device_tensor(t, f"adapter {i}: {name}")
+            if t.dtype not in (torch.bfloat16, torch.float16) or t.dtype != first.dtype:
+                raise ValueError(f"adapter {i}: {name} must be bf16 or fp16, all adapters alike, got {t.dtype}")
+            if t.dim() != 2:
+                raise ValueError(f"adapter {i}: {name} must be 2-D")
+            if t.device != first.device:
+                raise ValueError(f"adapter {i}: {name} is on {t.device}, the first adapter on {first.device}")
+        rank, K = a.shape
+        if not 1 <= rank <= MAX_RANK or b.shape[1] != rank:
+            raise ValueError(f"adapter {i}: a is {tuple(a.shape)}, b {tuple(b.shape)}: ranks from 1 to {MAX_RANK}, alike")
+        if K != first.shape[1] or b.shape[0] != adapters[0][1].shape[0]:
+            raise ValueError(f"adapter {i}: a is {tuple(a.shape)}, b {tuple(b.shape)}, the first ones are "
+                             f"{tuple(first.shape)} and {tuple(adapters[0][1].shape)}")
+        if K == 0 or K % 32 or b.shape[0] == 0:
+            raise ValueError(f"a must have a multiple of 32 columns and b rows, got {K} and {b.shape[0]}")
+        if not abs(float(scale)) < float("inf"):
+            raise ValueError(f"adapter {i}: the scale must be finite, got {scale}")
+    N, K = adapters[0][1].shape[0], first.shape[1]
+    blocks = -(-N // 64)
+    units = [_units(a.shape[0]) for a, _, _ in adapters]
+    before = [sum(units[:i]) for i in range(len(units))]
+    with _lib.on_device(first.device, stream):
+        pa = torch.zeros((sum(units) * 16, K), dtype=first.dtype, device=first.device)
+        pb = torch.empty((sum(units) * 16 * blocks * 64,), dtype=first.dtype, device=first.device)
+        for (a, b, _), u, at in zip(adapters, units, before):
+            pa[16 * at:16 * at + a.shape[0]] = a
+            wide = torch.zeros((blocks * 64, 16 * u), dtype=first.dtype, device=first.device)
+            wide[:N, :a.shape[0]] = b
+            # feature 16 g + 4 f + e of a block, rank 16 u + 8 h + i -> [block][u][f][lane 16 h + 4 g + e][i]
+            wide = wide.reshape(blocks, 4, 4, 4, u, 2, 8).permute(0, 4, 2, 5, 1, 3, 6)
+            pb[16 * at * blocks * 64:16 * (at + u) * blocks * 64] = wide.reshape(-1)
+        pa = pa.reshape(sum(units), 16, K // 32, 4, 8).permute(0, 2, 3, 1, 4).contiguous()
+        bits = [struct.unpack("<i", struct.pack("<f", float(s)))[0] for _, _, s in adapters]
+        meta = torch.tensor([[a.shape[0], at, s, 0] for (a, _, _), at, s in zip(adapters, before, bits)],
+                            dtype=torch.int32).to(first.device)
+    return LoraStack(pa, pb, meta, tuple(a.shape[0] for a, _, _ in adapters), N, K)
+
+
+@functools.lru_cache(maxsize=4096)
+def _plan_bytes(M, adapters):
+    return _lib.lib().qmlp_lora_plan_bytes(M, adapters)
+
+
+def lora_plan(ids, adapters, stream=None):
+    """``ids`` int32 ``[M]`` on the GPU and the number of adapters that they name -> ``LoraPlan``."""
+    _check_device_tensor(ids, "ids", torch.int32)
+    if ids.dim() != 1 or not 1 <= ids.shape[0] <= 65536:
+        raise ValueError(f"ids must hold 1 to 65536 tokens, got {tuple(ids.shape)}")
+    if not 1 <= adapters <= MAX_ADAPTERS:
+        raise ValueError(f"need 1 to {MAX_ADAPTERS} adapters, got {adapters}")
+    M, device = ids.shape[0], ids.device
+    nbytes = _plan_bytes(M, adapters)
+    with _lib.on_device(device, stream):
+        buf = torch.empty(nbytes // 4, dtype=torch.int32, device=device)
+        _lib.check(_lib.lib().qmlp_lora_plan(ids.data_ptr(), M, adapters, buf.data_ptr(), nbytes,
+                                             _lib.device_stream(device, stream)), "lora_plan")
+    return LoraPlan(buf, M, adapters)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(M, K, max_rank):
+    return _lib.lib().qmlp_lora_workspace_bytes(M, K, max_rank)
+
+
+def lora_linear(x, stack, plan, base=None, out=None, out_dtype=None, stream=None):
+    """``out[m] = base[m] + scale_a b_a (a_a x[m])`` for the adapter ``a`` of each token.
+
+    ``x``: bf16 or fp16 ``[M, K]`` of the adapters' dtype, rows may be strided; ``base`` bf16 or fp32 ``[M, N]`` or
+    None (zeros); ``out`` (or ``out_dtype`` when ``out`` is None) bf16, rounded once to nearest-even, or fp32.
+    ``out`` may be the base itself.
+    """
+    if not isinstance(stack, LoraStack) or not isinstance(plan, LoraPlan):
+        raise ValueError("stack must be a LoraStack (pack_lora) and plan a LoraPlan (lora_plan)")
+    x_type, stride = _check_rows(x)
+    M, K = x.shape
+    N = stack.n
+    if x.dtype != stack.a.dtype:
+        raise ValueError(f"x is {x.dtype}, the adapters {stack.a.dtype}")
+    if K != stack.k:
+        raise ValueError(f"x has {K} columns, the adapters {stack.k}")
+    if plan.tokens != M or plan.adapters != stack.adapters:
+        raise ValueError(f"the plan is for {plan.tokens} tokens and {plan.adapters} adapters, x has {M} rows and the "
+                         f"stack {stack.adapters} adapters")
+    dtype = _check_out(out, out_dtype, (M, N))
+    flags = _lib.OUT_F32 if dtype == torch.float32 else 0
+    if base is not None:
+        _check_device_tensor(base, "base")
+        if base.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError("base must be bf16 or fp32")
+        if tuple(base.shape) != (M, N):
+            raise ValueError(f"base must have shape ({M}, {N})")
+        if base.dtype == torch.float32:
+            flags |= _lib.RESIDUAL_F32
+    device = x.device
+    _same_device(device, stack=stack.a, plan=plan.buf, base=base, out=out)
+    with _lib.on_device(device, stream):
+        if out is None:
+            out = torch.empty((M, N), dtype=dtype, device=device)
+        nbytes = _workspace_bytes(M, K, stack.max_rank)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        rc = _lib.lib().qmlp_lora_linear(x.data_ptr(), x_type, stride, stack.a.data_ptr(), stack.b.data_ptr(),
+                                         stack.meta.data_ptr(), stack.adapters, stack.max_rank, plan.buf.data_ptr(),
+                                         None if base is None else base.data_ptr(), out.data_ptr(), ws.data_ptr(),
+                                         nbytes, M, N, K, flags, _lib.device_stream(device, stream))
+        _lib.check(rc, "lora_linear")
+    return out
