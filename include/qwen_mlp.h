@@ -307,7 +307,7 @@ size_t qmlp_w4a8_workspace_bytes(int M, int N, int K, int x_type);
  *   a     [unit][K / 32][64][8] 16-bit values: lane l of a K-step holds rank l % 16 of the unit, K values
  *         8 (l / 16)..; adapter after adapter
  *   b     per adapter [N / 64, rounded up][unit][4][32][8]: in part f lane l holds ranks 8 (l / 16).. of the
- *         unit for feature 16 (l % 16 / 4) + 4 f + l % 4 of the block (zeros behind N); adapter after adapter
+ *         unit for feature 16 f + l % 16 of the block (zeros behind N); adapter after adapter
  *   meta  int32 [adapters][4]: {rank, first, the bits of s_a (fp32), 0}
  *
  * A plan groups a batch's tokens by adapter; it serves every projection with the same adapter numbers (all of a

@@ -5,8 +5,7 @@
 // An adapter's matrices are used in the order of the 16x16x32 product's operands, ranks padded to units of 16:
 //   A: units of 16 ranks x 32 K, [rank unit][K / 32][lane][8]: lane l holds rank l % 16, K 8 (l / 16)..;
 //   B: blocks of 64 features, [block][rank unit][4][lane 0..31][8]: in part f lane l holds ranks 8 (l / 16).. of
-//      feature 16 (l % 16 / 4) + 4 f + l % 4, so that the four parts' sums leave a lane with 16 neighbouring
-//      features of a token (features behind N: zeros).
+//      feature 16 f + l % 16 (features behind N: zeros).
 // Adapters follow each other; adapter a starts rank unit `first` in both.  The meta table holds {rank, first,
 // s_a's bits, 0} of each.
 //
@@ -21,7 +20,7 @@ namespace qmlp {
 constexpr int kLoraMaxRank = 128;
 constexpr int kLoraMaxAdapters = 1024;
 constexpr int kLoraMagic = 0x41524f4c;
-constexpr int kLoraMaxPieces = 32;
+constexpr int kLoraMaxPieces = 8;
 
 // Tokens of a tile.  One unit of 16 for few tokens (as a rule of as many requests); four share what they read
 // of the adapters for many.
@@ -51,7 +50,7 @@ struct LoraArgs {
 };
 
 // The K range is cut into this many pieces, a workgroup each.
-int lora_pieces(int M, int K, int adapters, int num_cus);
+int lora_pieces(int M, int K);
 size_t lora_parts_bytes(int M, int K, int max_rank);
 int launch_lora_plan(const int* ids, int M, int adapters, int* plan, hipStream_t s);
 int launch_lora(const LoraArgs& a, int num_cus, hipStream_t s);

@@ -97,19 +97,22 @@ __device__ __forceinline__ f32x4 lora_product(u32x4 a, u32x4 b, f32x4 c) {
 
 // ---------------------------------------------------------------- A x
 //
-// One workgroup of 8 waves per (tile, K piece); the waves share the piece's K-steps of 32 out in turn and add
-// their sums up in a fixed order through LDS.  TU: units of 16 tokens of a tile; RU: rank units at most.
-constexpr int kDownWaves = 8;
+// One workgroup of 8 (few tokens: 16) waves per (K piece, tile): with eight pieces each XCD reads one of them
+// of every adapter, which its L2 holds; the waves share the piece's K-steps of 32 out in turn, two
+// neighbouring ones (a line of a 16-bit row) at a time, and add their sums up in a fixed order through LDS.  TU: units of 16 tokens of a tile; RU: rank units at most.
+template <int TU>
+constexpr int kDownWaves = TU == 1 ? 16 : 8;
 template <bool F16, int TU, int RU>
-__global__ __launch_bounds__(kDownWaves * 64, 1) void lora_down_kernel(LoraArgs p, int max_tiles, int ranks) {
-  extern __shared__ __align__(16) float s_sum[];  // [kDownWaves / 2][TU][RU][64 lanes][4]
-  const LoraTile t = lora_tile_of(p.plan, blockIdx.x, p.M, p.adapters);
+__global__ __launch_bounds__(kDownWaves<TU> * 64, 1) void lora_down_kernel(LoraArgs p, int max_tiles, int ranks) {
+  constexpr int kWaves = kDownWaves<TU>;
+  extern __shared__ __align__(16) float s_sum[];  // [kWaves / 2][TU][RU][64 lanes][4]
+  const LoraTile t = lora_tile_of(p.plan, blockIdx.y, p.M, p.adapters);
   if (t.adapter < 0 || t.rows == 0) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int* meta = p.stack.meta + 4 * t.adapter;
-  const int rank = meta[0], steps = p.K / 32, pieces = gridDim.y;
+  const int rank = meta[0], steps = p.K / 32, pieces = gridDim.x;
   const int ru = min((rank + 15) / 16, RU), tu = (t.rows + 15) / 16;
-  const int s0 = blockIdx.y * steps / pieces, s1 = (blockIdx.y + 1) * steps / pieces;
+  const int s0 = blockIdx.x * steps / pieces, s1 = (blockIdx.x + 1) * steps / pieces;
   const uint8_t* a = p.stack.a + ((size_t)meta[1] * steps * 64 + lane) * 16;
   const int* order = p.plan + 4 + 4 * max_tiles + t.first;
   const uint8_t* x[TU];
@@ -124,25 +127,31 @@ __global__ __launch_bounds__(kDownWaves * 64, 1) void lora_down_kernel(LoraArgs 
   for (int u = 0; u < TU; ++u)
 #pragma unroll
     for (int r = 0; r < RU; ++r) acc[u][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-  for (int s = s0 + wave; s < s1; s += kDownWaves) {
-    u32x4 av[RU], xv[TU];
+  for (int s = s0 + 2 * wave; s < s1; s += 2 * kWaves) {
+    u32x4 av[2][RU], xv[2][TU];
 #pragma unroll
-    for (int r = 0; r < RU; ++r)
-      av[r] = mine[r] ? *(const u32x4*)(a + ((size_t)r * steps + s) * 1024) : u32x4{0u, 0u, 0u, 0u};
+    for (int d = 0; d < 2; ++d) {
+      const bool in = s + d < s1;  // a step behind the piece multiplies by zeros
+      const int at = in ? s + d : s;
 #pragma unroll
-    for (int u = 0; u < TU; ++u)
-      if (u < tu) xv[u] = *(const u32x4*)(x[u] + (size_t)s * 64);
+      for (int u = 0; u < TU; ++u)
+        if (u < tu) xv[d][u] = in ? *(const u32x4*)(x[u] + (size_t)at * 64) : u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int u = 0; u < TU; ++u)
-      if (u < tu) {
+      for (int r = 0; r < RU; ++r)
+        av[d][r] = mine[r] && in ? *(const u32x4*)(a + ((size_t)r * steps + at) * 1024) : u32x4{0u, 0u, 0u, 0u};
+    }
 #pragma unroll
-        for (int r = 0; r < RU; ++r)
-          if (r < ru) acc[u][r] = lora_product<F16>(av[r], xv[u], acc[u][r]);
-      }
+    for (int d = 0; d < 2; ++d)
+#pragma unroll
+      for (int u = 0; u < TU; ++u)
+        if (u < tu) {
+#pragma unroll
+          for (int r = 0; r < RU; ++r)
+            if (r < ru) acc[u][r] = lora_product<F16>(av[d][r], xv[d][u], acc[u][r]);
+        }
   }
 #pragma unroll
-  for (int half = kDownWaves / 2; half > 0; half >>= 1) {
+  for (int half = kWaves / 2; half > 0; half >>= 1) {
     if (wave >= half && wave < 2 * half) {
       f32x4* at = (f32x4*)s_sum + (size_t)(wave - half) * TU * RU * 64 + lane;
 #pragma unroll
@@ -166,7 +175,7 @@ __global__ __launch_bounds__(kDownWaves * 64, 1) void lora_down_kernel(LoraArgs 
   for (int u = 0; u < TU; ++u) {
     const int row = u * 16 + (lane & 15);
     if (row >= t.rows) continue;
-    float* o = p.parts + ((size_t)blockIdx.y * p.M + t.first + row) * ranks + 4 * (lane >> 4);
+    float* o = p.parts + ((size_t)blockIdx.x * p.M + t.first + row) * ranks + 4 * (lane >> 4);
 #pragma unroll
     for (int r = 0; r < RU; ++r)
       if (r < ru) *(f32x4*)(o + 16 * r) = acc[u][r];
@@ -175,12 +184,12 @@ __global__ __launch_bounds__(kDownWaves * 64, 1) void lora_down_kernel(LoraArgs 
 
 // ---------------------------------------------------------------- base + s B t
 //
-// One workgroup of 4 waves per (tile, run of feature blocks).  It adds the pieces of t up in order, scales them
-// and splits each fp32 sum into three 16-bit numbers whose sum it is but for 2^-24 of it (bf16), or of the
+// One workgroup of 4 waves per (16 tokens of a tile, run of feature blocks).  It adds the pieces of t up, scales
+// them and splits each fp32 sum into three 16-bit numbers whose sum it is but for 2^-24 of it (bf16), or of the
 // token's largest (fp16: over a power of two that brings the largest near the type's), so the products keep
-// fp32's accuracy; they are laid out in LDS as the products' operands.  An operand of 32 holds 16 ranks twice: the
-// first parts beside the second ones; a second product adds the third parts.
-constexpr int kUpWaves = 4;
+// fp32's accuracy; they are laid out in LDS as the products' operands.  An operand of 32 holds 16 ranks twice:
+// the first parts beside the second ones; a second product adds the third parts.
+constexpr int kUpWaves = 4, kUpThreads = kUpWaves * 64;
 template <bool F16>
 __device__ __forceinline__ uint32_t lora_round(float v) {  // to the adapters' type
   if constexpr (F16) return f32_to_f16_bits(v);
@@ -192,17 +201,43 @@ __device__ __forceinline__ float lora_value(uint32_t b) {
   return bf16_to_f32((uint16_t)b);
 }
 
-template <bool F16, int TU>
-__global__ __launch_bounds__(kUpWaves * 64) void lora_up_kernel(LoraArgs p, int max_tiles, int ranks, int pieces,
-                                                               int blocks_each) {
-  extern __shared__ __align__(16) uint8_t s_t[];  // [rank unit][token unit][2][lane][8] 16-bit numbers
-  __shared__ float s_scale[TU * 16];               // fp16: what a token's sums are multiplied by
-  const LoraTile t = lora_tile_of(p.plan, blockIdx.x, p.M, p.adapters);
-  if (t.rows == 0 || (t.adapter < 0 && p.base == p.out)) return;
+// Four ranks' sum over the pieces, in order.
+__device__ __forceinline__ f32x4 lora_sum(const float* at, size_t piece, int pieces) {
+  f32x4 v[kLoraMaxPieces];
+#pragma unroll
+  for (int q = 0; q < kLoraMaxPieces; ++q) v[q] = *(const f32x4*)(at + min(q, pieces - 1) * piece);
+#pragma unroll
+  for (int q = 1; q < kLoraMaxPieces; ++q)
+    if (q < pieces) v[0] += v[q];
+  return v[0];
+}
+
+// What a lane finishes of a block of 16 tokens x 64 features.  Rows of a multiple of 8 features (WHOLE): 8
+// neighbouring features of tokens lane / 8 and 8 more, so that 8 lanes touch 64 features of a token together.
+// Others, which start anywhere: feature `lane` of all 16 tokens.
+template <int T, bool WHOLE>  // T: 0 nothing, 1 bf16, 2 fp32
+struct LoraRows {
+  u32x4 w[T == 0 ? 1 : !WHOLE ? 4 : T == 2 ? 4 : 2];
+};
+
+constexpr int kTurnRow = 68;  // floats of a token's row in LDS
+template <bool F16, int BASE, bool OUT32, bool WHOLE>
+__global__ __launch_bounds__(kUpThreads) void lora_up_kernel(LoraArgs p, int max_tiles, int ranks, int pieces,
+                                                            int blocks_each, int tile_units) {
+  extern __shared__ __align__(16) uint8_t s_t[];  // [rank unit][2][lane][8] 16-bit numbers, then t in fp32
+  __shared__ __align__(16) float s_turn[kUpWaves][16 * kTurnRow];
+  __shared__ float s_scale[16];  // fp16: what a token's sums are multiplied by
+  __shared__ int s_order[16];
+  const int unit = blockIdx.x % tile_units * 16;
+  LoraTile t = lora_tile_of(p.plan, blockIdx.x / tile_units, p.M, p.adapters);
+  t.first += unit;
+  t.rows = min(16, t.rows - unit);
+  if (t.rows <= 0 || (t.adapter < 0 && p.base == p.out)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int blocks = (p.N + 63) / 64;
   const int b0 = blockIdx.y * blocks_each, b1 = min(blocks, b0 + blocks_each);
   const int* order = p.plan + 4 + 4 * max_tiles + t.first;
+  if (tid < 16) s_order[tid] = order[min(tid, t.rows - 1)];
   int rank = 0, first = 0;
   float s = 0.f;
   if (t.adapter >= 0) {
@@ -211,51 +246,52 @@ __global__ __launch_bounds__(kUpWaves * 64) void lora_up_kernel(LoraArgs p, int 
     first = meta[1];
     s = __int_as_float(meta[2]);
   }
-  const int ru = (rank + 15) / 16, tu = (t.rows + 15) / 16;
+  const int ru = (rank + 15) / 16;
+  const size_t bblock = (size_t)ru * 2048;
+  const uint8_t* bmat = p.stack.b + (size_t)first * ((size_t)blocks * 2048) + (lane & 31) * 16;
+  u32x4 w[4];
+  auto load_w = [&](int b, int r) {
+    const bool mine = r * 16 + ((lane >> 4) & 1) * 8 < rank;
+#pragma unroll
+    for (int f = 0; f < 4; ++f)
+      w[f] = mine ? *(const u32x4*)(bmat + b * bblock + (r * 4 + f) * 512) : u32x4{0u, 0u, 0u, 0u};
+  };
+  if (b0 + wave < b1 && ru) load_w(b0 + wave, 0);
   if (ru) {
-    // a thread: 8 ranks of a token
-    const int items = tu * 16 * ru * 2;
-    auto sum8 = [&](int row, int r8, float (&v)[8]) {
-      f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
-      const float* at = p.parts + (size_t)(t.first + row) * ranks + r8 * 8;
-      for (int q = 0; q < pieces; ++q, at += (size_t)p.M * ranks) {
-        lo += *(const f32x4*)at;
-        hi += *(const f32x4*)(at + 4);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[i] = lo[i] * s;
-        v[4 + i] = hi[i] * s;
-      }
-    };
+    const int row4 = ru * 4;  // four ranks each
+    f32x4* s_sum = (f32x4*)(s_t + (size_t)ru * 2048);
+    const float* at = p.parts + (size_t)t.first * ranks;
+    for (int e = tid; e < t.rows * row4; e += kUpThreads)
+      s_sum[e] = lora_sum(at + (size_t)(e / row4) * ranks + e % row4 * 4, (size_t)p.M * ranks, pieces) * s;
+    __syncthreads();
     if constexpr (F16) {
-      // the token's power of two: 2 ru items of a row are neighbours in neither wave nor time, so one thread a row
-      for (int row = tid; row < TU * 16; row += kUpWaves * 64) {
-        float m = 0.f;
-        if (row < t.rows)
-          for (int r8 = 0; r8 < 2 * ru; ++r8) {
-            float v[8];
-            sum8(row, r8, v);
+      const int row = tid / 16;
+      float m = 0.f;
+      if (row < t.rows)
+        for (int r = tid % 16; r < row4; r += 16) {
+          const f32x4 v = s_sum[row * row4 + r];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
-          }
-        const int e = (int)(__float_as_uint(m) >> 23);  // the largest becomes one of [2^14, 2^15)
-        s_scale[row] = __uint_as_float((uint32_t)(min(max(e, 16), 254) - 14) << 23);
-      }
+          for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(v[i]));
+        }
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+      const int e = (int)(__float_as_uint(m) >> 23);  // the largest becomes one of [2^14, 2^15)
+      s_scale[row] = __uint_as_float((uint32_t)(min(max(e, 16), 254) - 14) << 23);
       __syncthreads();
     }
-    for (int item = tid; item < items; item += kUpWaves * 64) {
+    for (int item = tid; item < 16 * ru * 2; item += kUpThreads) {
       const int row = item / (2 * ru), r8 = item % (2 * ru);
-      float v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
-      if (row < t.rows) sum8(row, r8, v);
+      f32x4 v[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+      if (row < t.rows) {
+        v[0] = s_sum[row * row4 + 2 * r8];
+        v[1] = s_sum[row * row4 + 2 * r8 + 1];
+      }
       float inv = 1.f;
       if constexpr (F16) inv = 1.0f / s_scale[row];  // a power of two: exact
       u32x4 part[3];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float rest = v[i] * inv;
+        float rest = v[i / 4][i % 4] * inv;
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
           const uint32_t b = lora_round<F16>(rest);
@@ -263,99 +299,124 @@ __global__ __launch_bounds__(kUpWaves * 64) void lora_up_kernel(LoraArgs p, int 
           part[k][i / 2] = i % 2 ? part[k][i / 2] | b << 16 : b;
         }
       }
-      // lane of an operand: token row % 16, K 8 (lane / 16)..: ranks 0..15, then again
-      uint8_t* at = s_t + ((size_t)(r8 / 2) * TU + row / 16) * 2048 + ((r8 & 1) * 16 + row % 16) * 16;
-      *(u32x4*)at = part[0];
-      *(u32x4*)(at + 512) = part[1];
-      *(u32x4*)(at + 1024) = part[2];
-      *(u32x4*)(at + 1536) = u32x4{0u, 0u, 0u, 0u};
+      // lane of an operand: token, K 8 (lane / 16)..: ranks 0..15, then again
+      uint8_t* o = s_t + (size_t)(r8 / 2) * 2048 + ((r8 & 1) * 16 + row) * 16;
+      *(u32x4*)o = part[0];
+      *(u32x4*)(o + 512) = part[1];
+      *(u32x4*)(o + 1024) = part[2];
+      *(u32x4*)(o + 1536) = u32x4{0u, 0u, 0u, 0u};
     }
-    __syncthreads();
   }
-  const bool whole = p.N % 8 == 0;  // rows that vector accesses of 8 features divide
-  const size_t bblock = (size_t)ru * 2048;
-  const uint8_t* bmat = p.stack.b + (size_t)first * ((size_t)blocks * 2048) + (lane & 31) * 16;
-  const int g = lane >> 4;
-  for (int b = b0 + wave; b < b1; b += kUpWaves) {
-    f32x4 acc[TU][4];
+  __syncthreads();
+  // where this lane finishes: WHOLE: rows lane / 8 and 8 behind, features 8 (lane % 8)..
+  const int half = WHOLE ? lane >> 3 : 0, n0 = WHOLE ? (lane & 7) * 8 : lane;
+  const size_t at0 = (size_t)s_order[half] * p.N, at1 = (size_t)s_order[WHOLE ? half + 8 : 0] * p.N;
+  LoraRows<BASE, WHOLE> base;
+  auto load_base = [&](int b) {
+    const int n = b * 64 + n0;
+    if (n >= p.N) return;
+    if constexpr (WHOLE) {
 #pragma unroll
-    for (int u = 0; u < TU; ++u)
-#pragma unroll
-      for (int f = 0; f < 4; ++f) acc[u][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int r = 0; r < ru; ++r) {
-      u32x4 w[4];
-      const bool mine = r * 16 + ((lane >> 4) & 1) * 8 < rank;
-#pragma unroll
-      for (int f = 0; f < 4; ++f)
-        w[f] = mine ? *(const u32x4*)(bmat + b * bblock + (r * 4 + f) * 512) : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-      for (int u = 0; u < TU; ++u)
-        if (u < tu) {
-          const uint8_t* at = s_t + ((size_t)r * TU + u) * 2048 + lane * 16;
-          const u32x4 t01 = *(const u32x4*)at, t2 = *(const u32x4*)(at + 1024);
-#pragma unroll
-          for (int f = 0; f < 4; ++f) {
-            acc[u][f] = lora_product<F16>(w[f], t2, acc[u][f]);
-            acc[u][f] = lora_product<F16>(w[f], t01, acc[u][f]);
-          }
-        }
-    }
-    // lane: token lane % 16 of a unit, features 64 b + 16 g..
-#pragma unroll
-    for (int u = 0; u < TU; ++u) {
-      const int row = u * 16 + (lane & 15);
-      if (row >= t.rows) continue;
-      float m = 1.f;
-      if constexpr (F16)
-        if (ru) m = s_scale[row];
-      const size_t at0 = (size_t)order[row] * p.N;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int n = b * 64 + g * 16 + h * 8;
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = acc[u][2 * h + i / 4][i % 4] * m;
-        if (whole && n < p.N) {
-          const size_t at = at0 + n;
-          if (p.base) {
-            if (p.base_f32) {
-              const f32x4 lo = *(const f32x4*)((const float*)p.base + at), hi = *(const f32x4*)((const float*)p.base + at + 4);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] += i < 4 ? lo[i] : hi[i - 4];
-            } else {
-              const u32x4 w = *(const u32x4*)((const uint16_t*)p.base + at);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                v[2 * i] += __uint_as_float(w[i] << 16);
-                v[2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
-              }
-            }
-          }
-          if (p.out_f32) {
-            *(f32x4*)((float*)p.out + at) = f32x4{v[0], v[1], v[2], v[3]};
-            *(f32x4*)((float*)p.out + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
-          } else {
-            u32x4 w;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              w[i] = (uint32_t)f32_to_bf16(v[2 * i]) | (uint32_t)f32_to_bf16(v[2 * i + 1]) << 16;
-            *(u32x4*)((uint16_t*)p.out + at) = w;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (n + i >= p.N) continue;
-            const size_t at = at0 + n + i;
-            if (p.base)
-              v[i] += p.base_f32 ? ((const float*)p.base)[at] : bf16_to_f32(((const uint16_t*)p.base)[at]);
-            if (p.out_f32)
-              ((float*)p.out)[at] = v[i];
-            else
-              ((uint16_t*)p.out)[at] = f32_to_bf16(v[i]);
-          }
+      for (int i = 0; i < 2; ++i) {
+        const size_t at = (i ? at1 : at0) + n;
+        if constexpr (BASE == 1) {
+          base.w[i] = *(const u32x4*)((const uint16_t*)p.base + at);
+        } else if constexpr (BASE == 2) {
+          base.w[2 * i] = *(const u32x4*)((const float*)p.base + at);
+          base.w[2 * i + 1] = *(const u32x4*)((const float*)p.base + at + 4);
         }
       }
+    } else if constexpr (BASE != 0) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {  // tokens behind the last one read it again
+        const size_t at = (size_t)s_order[i] * p.N + n;
+        base.w[i / 4][i % 4] =
+            BASE == 1 ? (uint32_t)((const uint16_t*)p.base)[at] << 16 : ((const uint32_t*)p.base)[at];
+      }
     }
+  };
+  if (b0 + wave < b1) load_base(b0 + wave);
+  float* turn = s_turn[wave];
+  for (int b = b0 + wave; b < b1; b += kUpWaves) {
+    f32x4 acc[4];
+#pragma unroll
+    for (int f = 0; f < 4; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < ru; ++r) {
+      u32x4 v[4];
+#pragma unroll
+      for (int f = 0; f < 4; ++f) v[f] = w[f];
+      if (r + 1 < ru)
+        load_w(b, r + 1);
+      else if (b + kUpWaves < b1)
+        load_w(b + kUpWaves, 0);
+      const uint8_t* at = s_t + (size_t)r * 2048 + lane * 16;
+      const u32x4 t01 = *(const u32x4*)at, t2 = *(const u32x4*)(at + 1024);
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        acc[f] = lora_product<F16>(v[f], t2, acc[f]);
+        acc[f] = lora_product<F16>(v[f], t01, acc[f]);
+      }
+    }
+    // acc: token lane % 16, features 16 f + 4 (lane / 16)..
+    float m = 1.f;
+    if constexpr (F16)
+      if (ru) m = s_scale[lane & 15];
+#pragma unroll
+    for (int f = 0; f < 4; ++f) *(f32x4*)(turn + (lane & 15) * kTurnRow + 16 * f + 4 * (lane >> 4)) = acc[f] * m;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int n = b * 64 + n0;
+    if constexpr (WHOLE) {
+      float y[2][8];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float* from = turn + (half + 8 * i) * kTurnRow + n0;
+        const f32x4 lo = *(const f32x4*)from, hi = *(const f32x4*)(from + 4);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          y[i][j] = j < 4 ? lo[j] : hi[j - 4];
+          if constexpr (BASE == 1)
+            y[i][j] += __uint_as_float(j % 2 ? base.w[i][j / 2] & 0xffff0000u : base.w[i][j / 2] << 16);
+          else if constexpr (BASE == 2)
+            y[i][j] += __uint_as_float(base.w[2 * i + j / 4][j % 4]);
+        }
+      }
+      if (b + kUpWaves < b1) load_base(b + kUpWaves);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (half + 8 * i >= t.rows || n >= p.N) continue;
+        const size_t at = (i ? at1 : at0) + n;
+        if constexpr (OUT32) {
+          *(f32x4*)((float*)p.out + at) = f32x4{y[i][0], y[i][1], y[i][2], y[i][3]};
+          *(f32x4*)((float*)p.out + at + 4) = f32x4{y[i][4], y[i][5], y[i][6], y[i][7]};
+        } else {
+          u32x4 o;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            o[j] = (uint32_t)f32_to_bf16(y[i][2 * j]) | (uint32_t)f32_to_bf16(y[i][2 * j + 1]) << 16;
+          *(u32x4*)((uint16_t*)p.out + at) = o;
+        }
+      }
+    } else {
+      float y[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        y[i] = turn[i * kTurnRow + n0];
+        if constexpr (BASE != 0) y[i] += __uint_as_float(base.w[i / 4][i % 4]);
+      }
+      if (b + kUpWaves < b1) load_base(b + kUpWaves);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if (i >= t.rows || n >= p.N) continue;
+        const size_t at = (size_t)s_order[i] * p.N + n;
+        if constexpr (OUT32)
+          ((float*)p.out)[at] = y[i];
+        else
+          ((uint16_t*)p.out)[at] = f32_to_bf16(y[i]);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -363,58 +424,67 @@ __global__ __launch_bounds__(kUpWaves * 64) void lora_up_kernel(LoraArgs p, int 
 
 static int up_div(int a, int b) { return (a + b - 1) / b; }
 
-// Enough workgroups for the card at two K-steps a wave or more, as far as the tiles alone are not: the most
-// tiles that M tokens can make are counted as half of them, since an adapter's tokens share tiles as a rule.
-int lora_pieces(int M, int K, int adapters, int num_cus) {
-  const int tiles = std::max(1, lora_max_tiles(M, adapters) / 2);
-  return std::max(1, std::min({kLoraMaxPieces, up_div(K / 32, 2 * kDownWaves),
-                               up_div(std::min(num_cus, kMaxWorkgroups), tiles)}));
+// Eight pieces, as far as each wave has two K-steps: one for each XCD, and few enough for the second launch, each
+// of whose workgroups adds them up.
+template <int TU>
+static int pieces_of(int K) {
+  return std::min(kLoraMaxPieces, up_div(K / 32, 2 * kDownWaves<TU>));
 }
+int lora_pieces(int M, int K) { return lora_tile(M) == 16 ? pieces_of<1>(K) : pieces_of<4>(K); }
 
 static int padded_rank(int rank) { return (rank + 15) / 16 * 16; }
 
-// The most that pieces x M can be, whatever the adapters and the card: there are M / 128 or more of lora_pieces'
-// tiles (of M / 64 + 2 or more, halved), hence at most 512 / (M / 128) + 1 pieces.
 size_t lora_parts_bytes(int M, int K, int max_rank) {
-  const int most = std::max(1, std::min(kLoraMaxPieces, up_div(K / 32, 2 * kDownWaves)));
-  const size_t rows = std::min((size_t)most * M, (size_t)kMaxWorkgroups * 128 + M);
-  return align256(rows * padded_rank(max_rank) * 4);
+  return align256((size_t)pieces_of<4>(K) * M * padded_rank(max_rank) * 4);  // the most of both kinds
 }
 
 template <bool F16, int TU, int RU>
 static int launch_down(const LoraArgs& a, int max_tiles, int pieces, hipStream_t s) {
-  constexpr size_t lds = (size_t)kDownWaves / 2 * TU * RU * 64 * 16;
+  constexpr size_t lds = (size_t)kDownWaves<TU> / 2 * TU * RU * 64 * 16;
   auto kern = lora_down_kernel<F16, TU, RU>;
   if constexpr (lds > 65536) {
     static std::atomic<uint64_t> raised{0};
     if (int rc = raise_lds_once((const void*)kern, (int)lds, raised)) return rc;
   }
-  hipLaunchKernelGGL(kern, dim3(max_tiles, pieces), dim3(kDownWaves * 64), lds, s, a, max_tiles,
+  hipLaunchKernelGGL(kern, dim3(pieces, max_tiles), dim3(kDownWaves<TU> * 64), lds, s, a, max_tiles,
                      padded_rank(a.max_rank));
   return check_launch("lora_down_kernel");
 }
 
+template <bool F16, int BASE, bool OUT32, bool WHOLE>
+static int launch_up(const LoraArgs& a, int max_tiles, int pieces, int num_cus, hipStream_t s) {
+  const int blocks = up_div(a.N, 64), tile_units = lora_tile(a.M) / 16;
+  const int tiles = std::max(1, std::min(max_tiles * tile_units / 2, up_div(a.M, 16)));
+  const int runs = std::max(1, std::min(up_div(blocks, kUpWaves), up_div(4 * num_cus, tiles)));
+  const int each = up_div(blocks, runs), units = padded_rank(a.max_rank) / 16;
+  hipLaunchKernelGGL((lora_up_kernel<F16, BASE, OUT32, WHOLE>), dim3(max_tiles * tile_units, up_div(blocks, each)),
+                     dim3(kUpThreads), (size_t)units * (2048 + 1024), s, a, max_tiles, units * 16, pieces, each,
+                     tile_units);
+  return check_launch("lora_up_kernel");
+}
+template <bool F16, int BASE, bool OUT32>
+static int launch_up_rows(const LoraArgs& a, int max_tiles, int pieces, int num_cus, hipStream_t s) {
+  return a.N % 8 ? launch_up<F16, BASE, OUT32, false>(a, max_tiles, pieces, num_cus, s)
+                 : launch_up<F16, BASE, OUT32, true>(a, max_tiles, pieces, num_cus, s);
+}
+
 template <bool F16, int TU>
 static int launch_tokens(const LoraArgs& a, int num_cus, hipStream_t s) {
-  const int max_tiles = lora_max_tiles(a.M, a.adapters), pieces = lora_pieces(a.M, a.K, a.adapters, num_cus);
+  const int max_tiles = lora_max_tiles(a.M, a.adapters), pieces = lora_pieces(a.M, a.K);
   const int units = padded_rank(a.max_rank) / 16;
   const int rc = units <= 1   ? launch_down<F16, TU, 1>(a, max_tiles, pieces, s)
                  : units <= 2 ? launch_down<F16, TU, 2>(a, max_tiles, pieces, s)
                  : units <= 4 ? launch_down<F16, TU, 4>(a, max_tiles, pieces, s)
                               : launch_down<F16, TU, 8>(a, max_tiles, pieces, s);
   if (rc) return rc;
-  const int blocks = up_div(a.N, 64), tiles = std::max(1, max_tiles / 2);
-  const int runs = std::max(1, std::min(up_div(blocks, kUpWaves), up_div(4 * num_cus, tiles)));
-  const int each = up_div(blocks, runs);
-  const size_t lds = (size_t)units * TU * 2048;
-  auto up = lora_up_kernel<F16, TU>;
-  if constexpr (TU > 1) {  // 64 KB at the largest rank, besides the scales
-    static std::atomic<uint64_t> raised{0};
-    if (int rc = raise_lds_once((const void*)up, kLoraMaxRank / 16 * TU * 2048, raised)) return rc;
-  }
-  hipLaunchKernelGGL(up, dim3(max_tiles, up_div(blocks, each)), dim3(kUpWaves * 64), lds, s, a,
-                     max_tiles, padded_rank(a.max_rank), pieces, each);
-  return check_launch("lora_up_kernel");
+  const int base = !a.base ? 0 : a.base_f32 ? 2 : 1;
+  if (a.out_f32)
+    return base == 0   ? launch_up_rows<F16, 0, true>(a, max_tiles, pieces, num_cus, s)
+           : base == 1 ? launch_up_rows<F16, 1, true>(a, max_tiles, pieces, num_cus, s)
+                       : launch_up_rows<F16, 2, true>(a, max_tiles, pieces, num_cus, s);
+  return base == 0   ? launch_up_rows<F16, 0, false>(a, max_tiles, pieces, num_cus, s)
+         : base == 1 ? launch_up_rows<F16, 1, false>(a, max_tiles, pieces, num_cus, s)
+                     : launch_up_rows<F16, 2, false>(a, max_tiles, pieces, num_cus, s);
 }
 
 int launch_lora(const LoraArgs& a, int num_cus, hipStream_t s) {

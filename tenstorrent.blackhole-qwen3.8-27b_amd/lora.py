@@ -109,8 +109,8 @@ def pack_lora(adapters, stream=None):
             pa[16 * at:16 * at + a.shape[0]] = a
             wide = torch.zeros((blocks * 64, 16 * u), dtype=first.dtype, device=first.device)
             wide[:N, :a.shape[0]] = b
-            # feature 16 g + 4 f + e of a block, rank 16 u + 8 h + i -> [block][u][f][lane 16 h + 4 g + e][i]
-            wide = wide.reshape(blocks, 4, 4, 4, u, 2, 8).permute(0, 4, 2, 5, 1, 3, 6)
+            # feature 16 f + e of a block, rank 16 u + 8 h + i -> [block][u][f][lane 16 h + e][i]
+            wide = wide.reshape(blocks, 4, 16, u, 2, 8).permute(0, 3, 1, 4, 2, 5)
             pb[16 * at * blocks * 64:16 * (at + u) * blocks * 64] = wide.reshape(-1)
         pa = pa.reshape(sum(units), 16, K // 32, 4, 8).permute(0, 2, 3, 1, 4).contiguous()
         bits = [struct.unpack("<i", struct.pack("<f", float(s)))[0] for _, _, s in adapters]
