@@ -303,12 +303,13 @@ size_t qmlp_w4a8_workspace_bytes(int M, int N, int K, int x_type);
  * for any number of adapters from 1 to 1024 of ranks from 1 to 128, which may differ.  A token whose id is
  * outside [0, adapters) has none (out[m] = base[m]).
  *
- * Layouts (ranks padded to units of 16 with zeros; `first` counts the rank units of the adapters before):
+ * Layouts (ranks padded with zeros to units of 16 in a, of 32 in b):
  *   a     [unit][K / 32][64][8] 16-bit values: lane l of a K-step holds rank l % 16 of the unit, K values
  *         8 (l / 16)..; adapter after adapter
- *   b     per adapter [N / 64, rounded up][unit][4][32][8]: in part f lane l holds ranks 8 (l / 16).. of the
+ *   b     per adapter [N / 64, rounded up][unit][4][64][8]: in part f lane l holds ranks 8 (l / 16).. of the
  *         unit for feature 16 f + l % 16 of the block (zeros behind N); adapter after adapter
- *   meta  int32 [adapters][4]: {rank, first, the bits of s_a (fp32), 0}
+ *   meta  int32 [adapters][4]: {rank, units of a in the adapters before, the bits of s_a (fp32), units of b
+ *         before}
  *
  * A plan groups a batch's tokens by adapter; it serves every projection with the same adapter numbers (all of a
  * model's layers) until the tokens' adapters change. */

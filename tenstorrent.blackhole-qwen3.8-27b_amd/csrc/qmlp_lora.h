@@ -2,12 +2,12 @@
 //
 //   out[m] = base[m] + s_a B_a (A_a x[m]),   a = ids[m];  A_a [r, K], B_a [N, r], s_a a number
 //
-// An adapter's matrices are used in the order of the 16x16x32 product's operands, ranks padded to units of 16:
+// An adapter's matrices are used in the order of the 16x16x32 product's operands:
 //   A: units of 16 ranks x 32 K, [rank unit][K / 32][lane][8]: lane l holds rank l % 16, K 8 (l / 16)..;
-//   B: blocks of 64 features, [block][rank unit][4][lane 0..31][8]: in part f lane l holds ranks 8 (l / 16).. of
-//      feature 16 f + l % 16 (features behind N: zeros).
-// Adapters follow each other; adapter a starts rank unit `first` in both.  The meta table holds {rank, first,
-// s_a's bits, 0} of each.
+//   B: blocks of 64 features, [block][32 ranks][4][lane][8]: in part f lane l holds ranks 8 (l / 16).. of feature
+//      16 f + l % 16 (features behind N and ranks behind the adapter's: zeros, the latter never read).
+// Adapters follow each other.  The meta table holds {rank, rank units before in A, s_a's bits, 32s of ranks
+// before in B} of each.
 //
 // A plan groups a batch's tokens by adapter: {magic, M, adapters, tiles}, then one {adapter, first row, rows, 0}
 // per tile (rows: places in the order below, at most lora_tile(M) of one adapter; -1: without), then the tokens
@@ -22,9 +22,9 @@ constexpr int kLoraMaxAdapters = 1024;
 constexpr int kLoraMagic = 0x41524f4c;
 constexpr int kLoraMaxPieces = 8;
 
-// Tokens of a tile.  One unit of 16 for few tokens (as a rule of as many requests); four share what they read
+// Tokens of a tile.  One unit of 16 for few tokens (as a rule of as many requests); two share what they read
 // of the adapters for many.
-__host__ __device__ inline int lora_tile(int M) { return M <= 64 ? 16 : 64; }
+__host__ __device__ inline int lora_tile(int M) { return M <= 64 ? 16 : 32; }
 inline int lora_max_tiles(int M, int adapters) {
   const int groups = M < adapters + 1 ? M : adapters + 1;
   return M / lora_tile(M) + groups;

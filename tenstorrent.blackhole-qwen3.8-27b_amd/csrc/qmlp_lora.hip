@@ -6,6 +6,7 @@
 #include <atomic>
 
 #include "qmlp_lora.h"
+#include "qmlp_mx.h"
 
 namespace qmlp {
 
@@ -81,9 +82,10 @@ struct LoraTile {
 };
 // Tile t of a plan; rows 0 where there is none, or where the plan is not one for these sizes.
 __device__ __forceinline__ LoraTile lora_tile_of(const int* plan, int t, int M, int adapters) {
-  if (plan[0] != kLoraMagic || plan[1] != M || plan[2] != adapters || t >= plan[3]) return LoraTile{-1, 0, 0};
-  const int* p = plan + 4 + 4 * t;
-  return LoraTile{p[0], p[1], p[2]};
+  typedef int i32x4_t __attribute__((ext_vector_type(4)));
+  const i32x4_t head = *(const i32x4_t*)plan, p = *(const i32x4_t*)(plan + 4 + 4 * t);  // on their way together
+  const bool ok = (head.x == kLoraMagic) & (head.y == M) & (head.z == adapters) & (t < head.w);
+  return LoraTile{ok ? p.x : -1, ok ? p.y : 0, ok ? p.z : 0};
 }
 
 template <bool F16>
@@ -97,63 +99,97 @@ __device__ __forceinline__ f32x4 lora_product(u32x4 a, u32x4 b, f32x4 c) {
 
 // ---------------------------------------------------------------- A x
 //
-// One workgroup of 8 (few tokens: 16) waves per (K piece, tile): with eight pieces each XCD reads one of them
-// of every adapter, which its L2 holds; the waves share the piece's K-steps of 32 out in turn, two
-// neighbouring ones (a line of a 16-bit row) at a time, and add their sums up in a fixed order through LDS.  TU: units of 16 tokens of a tile; RU: rank units at most.
+// One workgroup of 8 (few tokens: 16) waves per (K piece, tile): with eight pieces each XCD reads one of them of
+// every adapter, which its L2 holds.  The waves share the piece's K-steps of 32 out in turn, two neighbouring ones
+// (a line of a 16-bit row) at a time, and add their sums up in a fixed order through LDS.  Rows of x come in by
+// whole lines, 8 lanes to a row, and turn through LDS into operands: read as the operands lie, one row a lane,
+// every lane of a load is an access of its own, and those bounded the kernel (27000 of a CU for 2048 x 17408).
+// TU: units of 16 tokens of a tile; RU: rank units at most.
 template <int TU>
 constexpr int kDownWaves = TU == 1 ? 16 : 8;
+template <int TU, int RU>
+constexpr size_t kDownLds = kDownWaves<TU> * TU * (RU > 4 ? RU * 512 : 2048);  // turning, then the waves' sums
+
 template <bool F16, int TU, int RU>
 __global__ __launch_bounds__(kDownWaves<TU> * 64, 1) void lora_down_kernel(LoraArgs p, int max_tiles, int ranks) {
-  constexpr int kWaves = kDownWaves<TU>;
-  extern __shared__ __align__(16) float s_sum[];  // [kWaves / 2][TU][RU][64 lanes][4]
+  constexpr int kWaves = kDownWaves<TU>, kLoads = 2 * TU;
+  extern __shared__ __align__(16) uint8_t s_mem[];
   const LoraTile t = lora_tile_of(p.plan, blockIdx.y, p.M, p.adapters);
   if (t.adapter < 0 || t.rows == 0) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int* meta = p.stack.meta + 4 * t.adapter;
+  const int* order = p.plan + 4 + 4 * max_tiles + t.first;
+  const uint8_t* x[kLoads];  // load i: rows 8 i + lane / 8, 16 bytes at 16 (lane % 8) of the two steps' line
+  bool row_in[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int row = 8 * i + (lane >> 3);
+    row_in[i] = row < t.rows;
+    x[i] = p.x + (size_t)order[min(row, t.rows - 1)] * p.x_bytes + (lane & 7) * 16;
+  }
   const int rank = meta[0], steps = p.K / 32, pieces = gridDim.x;
   const int ru = min((rank + 15) / 16, RU), tu = (t.rows + 15) / 16;
   const int s0 = blockIdx.x * steps / pieces, s1 = (blockIdx.x + 1) * steps / pieces;
   const uint8_t* a = p.stack.a + ((size_t)meta[1] * steps * 64 + lane) * 16;
-  const int* order = p.plan + 4 + 4 * max_tiles + t.first;
-  const uint8_t* x[TU];
-#pragma unroll
-  for (int u = 0; u < TU; ++u)  // rows behind the tile's last one read it again
-    x[u] = p.x + (size_t)order[min(u * 16 + (lane & 15), t.rows - 1)] * p.x_bytes + (lane >> 4) * 16;
   bool mine[RU];  // ranks that the adapter has
 #pragma unroll
   for (int r = 0; r < RU; ++r) mine[r] = r * 16 + (lane & 15) < rank;
+  u32x4 av[2][RU], xv[kLoads];
+  auto load = [&](int s) {  // a step behind the piece multiplies zeros by zeros
+    const bool second = s + 1 < s1;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      xv[i] = row_in[i] && (second || (lane & 4) == 0) ? *(const u32x4*)(x[i] + (size_t)s * 64) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+#pragma unroll
+      for (int r = 0; r < RU; ++r)
+        av[d][r] = mine[r] && (d == 0 || second) ? *(const u32x4*)(a + ((size_t)r * steps + s + d) * 1024)
+                                                 : u32x4{0u, 0u, 0u, 0u};
+  };
   f32x4 acc[TU][RU];
 #pragma unroll
   for (int u = 0; u < TU; ++u)
 #pragma unroll
     for (int r = 0; r < RU; ++r) acc[u][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+  uint8_t* turn = s_mem + wave * TU * 2048;  // a row's 8 pieces of 16 bytes, piece c at c ^ (row % 8)
+  auto turn_fence = [] {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+  if (s0 + 2 * wave < s1) load(s0 + 2 * wave);
   for (int s = s0 + 2 * wave; s < s1; s += 2 * kWaves) {
-    u32x4 av[2][RU], xv[2][TU];
 #pragma unroll
-    for (int d = 0; d < 2; ++d) {
-      const bool in = s + d < s1;  // a step behind the piece multiplies by zeros
-      const int at = in ? s + d : s;
-#pragma unroll
-      for (int u = 0; u < TU; ++u)
-        if (u < tu) xv[d][u] = in ? *(const u32x4*)(x[u] + (size_t)at * 64) : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-      for (int r = 0; r < RU; ++r)
-        av[d][r] = mine[r] && in ? *(const u32x4*)(a + ((size_t)r * steps + at) * 1024) : u32x4{0u, 0u, 0u, 0u};
+    for (int i = 0; i < kLoads; ++i) {
+      const int row = 8 * i + (lane >> 3);
+      *(u32x4*)(turn + row * 128 + (((lane & 7) ^ (row & 7)) * 16)) = xv[i];
     }
+    u32x4 w[2][RU];
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+#pragma unroll
+      for (int r = 0; r < RU; ++r) w[d][r] = av[d][r];
+    if (s + 2 * kWaves < s1) load(s + 2 * kWaves);
+    turn_fence();
 #pragma unroll
     for (int d = 0; d < 2; ++d)
 #pragma unroll
       for (int u = 0; u < TU; ++u)
         if (u < tu) {
+          const int row = u * 16 + (lane & 15);
+          const u32x4 v = *(const u32x4*)(turn + row * 128 + (((d * 4 + (lane >> 4)) ^ (row & 7)) * 16));
 #pragma unroll
           for (int r = 0; r < RU; ++r)
-            if (r < ru) acc[u][r] = lora_product<F16>(av[d][r], xv[d][u], acc[u][r]);
+            if (r < ru) acc[u][r] = lora_product<F16>(w[d][r], v, acc[u][r]);
         }
+    turn_fence();
   }
+  __syncthreads();
+  f32x4* s_sum = (f32x4*)s_mem;  // [kWaves / 2][TU][RU][64 lanes]
 #pragma unroll
   for (int half = kWaves / 2; half > 0; half >>= 1) {
     if (wave >= half && wave < 2 * half) {
-      f32x4* at = (f32x4*)s_sum + (size_t)(wave - half) * TU * RU * 64 + lane;
+      f32x4* at = s_sum + (size_t)(wave - half) * TU * RU * 64 + lane;
 #pragma unroll
       for (int u = 0; u < TU; ++u)
 #pragma unroll
@@ -161,7 +197,7 @@ __global__ __launch_bounds__(kDownWaves<TU> * 64, 1) void lora_down_kernel(LoraA
     }
     __syncthreads();
     if (wave < half) {
-      const f32x4* at = (const f32x4*)s_sum + (size_t)wave * TU * RU * 64 + lane;
+      const f32x4* at = s_sum + (size_t)wave * TU * RU * 64 + lane;
 #pragma unroll
       for (int u = 0; u < TU; ++u)
 #pragma unroll
@@ -184,16 +220,16 @@ __global__ __launch_bounds__(kDownWaves<TU> * 64, 1) void lora_down_kernel(LoraA
 
 // ---------------------------------------------------------------- base + s B t
 //
-// One workgroup of 4 waves per (16 tokens of a tile, run of feature blocks).  It adds the pieces of t up, scales
+// One workgroup of 8 waves per (16 tokens of a tile, run of feature blocks).  It adds the pieces of t up, scales
 // them and splits each fp32 sum into three 16-bit numbers whose sum it is but for 2^-24 of it (bf16), or of the
 // token's largest (fp16: over a power of two that brings the largest near the type's), so the products keep
-// fp32's accuracy; they are laid out in LDS as the products' operands.  An operand of 32 holds 16 ranks twice:
-// the first parts beside the second ones; a second product adds the third parts.
-constexpr int kUpWaves = 4, kUpThreads = kUpWaves * 64;
+// fp32's accuracy; they are laid out in LDS as the products' operands, 32 ranks' parts of one order each.
+constexpr int kUpWaves = 8, kUpThreads = kUpWaves * 64;
+constexpr int kUpParts = 3 * 1024;  // bytes of 32 ranks of 16 tokens
 template <bool F16>
 __device__ __forceinline__ uint32_t lora_round(float v) {  // to the adapters' type
   if constexpr (F16) return f32_to_f16_bits(v);
-  return f32_to_bf16(v);
+  return mx_bf16x2(v, 0.f) & 0xffffu;
 }
 template <bool F16>
 __device__ __forceinline__ float lora_value(uint32_t b) {
@@ -224,10 +260,9 @@ constexpr int kTurnRow = 68;  // floats of a token's row in LDS
 template <bool F16, int BASE, bool OUT32, bool WHOLE>
 __global__ __launch_bounds__(kUpThreads) void lora_up_kernel(LoraArgs p, int max_tiles, int ranks, int pieces,
                                                             int blocks_each, int tile_units) {
-  extern __shared__ __align__(16) uint8_t s_t[];  // [rank unit][2][lane][8] 16-bit numbers, then t in fp32
+  extern __shared__ __align__(16) uint8_t s_t[];  // [32 ranks][3 parts][lane][8] 16-bit numbers, then t in fp32
   __shared__ __align__(16) float s_turn[kUpWaves][16 * kTurnRow];
   __shared__ float s_scale[16];  // fp16: what a token's sums are multiplied by
-  __shared__ int s_order[16];
   const int unit = blockIdx.x % tile_units * 16;
   LoraTile t = lora_tile_of(p.plan, blockIdx.x / tile_units, p.M, p.adapters);
   t.first += unit;
@@ -237,80 +272,27 @@ __global__ __launch_bounds__(kUpThreads) void lora_up_kernel(LoraArgs p, int max
   const int blocks = (p.N + 63) / 64;
   const int b0 = blockIdx.y * blocks_each, b1 = min(blocks, b0 + blocks_each);
   const int* order = p.plan + 4 + 4 * max_tiles + t.first;
-  if (tid < 16) s_order[tid] = order[min(tid, t.rows - 1)];
   int rank = 0, first = 0;
   float s = 0.f;
   if (t.adapter >= 0) {
     const int* meta = p.stack.meta + 4 * t.adapter;
     rank = min(meta[0], ranks);
-    first = meta[1];
     s = __int_as_float(meta[2]);
+    first = meta[3];
   }
-  const int ru = (rank + 15) / 16;
-  const size_t bblock = (size_t)ru * 2048;
-  const uint8_t* bmat = p.stack.b + (size_t)first * ((size_t)blocks * 2048) + (lane & 31) * 16;
+  const int ru = (rank + 31) / 32;
+  const size_t bblock = (size_t)ru * 4096;
+  const uint8_t* bmat = p.stack.b + (size_t)first * ((size_t)blocks * 4096) + lane * 16;
   u32x4 w[4];
   auto load_w = [&](int b, int r) {
-    const bool mine = r * 16 + ((lane >> 4) & 1) * 8 < rank;
+    const bool mine = r * 32 + (lane >> 4) * 8 < rank;
 #pragma unroll
     for (int f = 0; f < 4; ++f)
-      w[f] = mine ? *(const u32x4*)(bmat + b * bblock + (r * 4 + f) * 512) : u32x4{0u, 0u, 0u, 0u};
+      w[f] = mine ? *(const u32x4*)(bmat + b * bblock + (r * 4 + f) * 1024) : u32x4{0u, 0u, 0u, 0u};
   };
-  if (b0 + wave < b1 && ru) load_w(b0 + wave, 0);
-  if (ru) {
-    const int row4 = ru * 4;  // four ranks each
-    f32x4* s_sum = (f32x4*)(s_t + (size_t)ru * 2048);
-    const float* at = p.parts + (size_t)t.first * ranks;
-    for (int e = tid; e < t.rows * row4; e += kUpThreads)
-      s_sum[e] = lora_sum(at + (size_t)(e / row4) * ranks + e % row4 * 4, (size_t)p.M * ranks, pieces) * s;
-    __syncthreads();
-    if constexpr (F16) {
-      const int row = tid / 16;
-      float m = 0.f;
-      if (row < t.rows)
-        for (int r = tid % 16; r < row4; r += 16) {
-          const f32x4 v = s_sum[row * row4 + r];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(v[i]));
-        }
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-      const int e = (int)(__float_as_uint(m) >> 23);  // the largest becomes one of [2^14, 2^15)
-      s_scale[row] = __uint_as_float((uint32_t)(min(max(e, 16), 254) - 14) << 23);
-      __syncthreads();
-    }
-    for (int item = tid; item < 16 * ru * 2; item += kUpThreads) {
-      const int row = item / (2 * ru), r8 = item % (2 * ru);
-      f32x4 v[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-      if (row < t.rows) {
-        v[0] = s_sum[row * row4 + 2 * r8];
-        v[1] = s_sum[row * row4 + 2 * r8 + 1];
-      }
-      float inv = 1.f;
-      if constexpr (F16) inv = 1.0f / s_scale[row];  // a power of two: exact
-      u32x4 part[3];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float rest = v[i / 4][i % 4] * inv;
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          const uint32_t b = lora_round<F16>(rest);
-          rest = __builtin_isfinite(rest) ? rest - lora_value<F16>(b) : 0.f;
-          part[k][i / 2] = i % 2 ? part[k][i / 2] | b << 16 : b;
-        }
-      }
-      // lane of an operand: token, K 8 (lane / 16)..: ranks 0..15, then again
-      uint8_t* o = s_t + (size_t)(r8 / 2) * 2048 + ((r8 & 1) * 16 + row) * 16;
-      *(u32x4*)o = part[0];
-      *(u32x4*)(o + 512) = part[1];
-      *(u32x4*)(o + 1024) = part[2];
-      *(u32x4*)(o + 1536) = u32x4{0u, 0u, 0u, 0u};
-    }
-  }
-  __syncthreads();
   // where this lane finishes: WHOLE: rows lane / 8 and 8 behind, features 8 (lane % 8)..
   const int half = WHOLE ? lane >> 3 : 0, n0 = WHOLE ? (lane & 7) * 8 : lane;
-  const size_t at0 = (size_t)s_order[half] * p.N, at1 = (size_t)s_order[WHOLE ? half + 8 : 0] * p.N;
+  const size_t at0 = (size_t)order[min(half, t.rows - 1)] * p.N, at1 = (size_t)order[min(WHOLE ? half + 8 : 0, t.rows - 1)] * p.N;
   LoraRows<BASE, WHOLE> base;
   auto load_base = [&](int b) {
     const int n = b * 64 + n0;
@@ -329,13 +311,62 @@ __global__ __launch_bounds__(kUpThreads) void lora_up_kernel(LoraArgs p, int max
     } else if constexpr (BASE != 0) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {  // tokens behind the last one read it again
-        const size_t at = (size_t)s_order[i] * p.N + n;
+        const size_t at = (size_t)order[min(i, t.rows - 1)] * p.N + n;
         base.w[i / 4][i % 4] =
             BASE == 1 ? (uint32_t)((const uint16_t*)p.base)[at] << 16 : ((const uint32_t*)p.base)[at];
       }
     }
   };
   if (b0 + wave < b1) load_base(b0 + wave);
+  if (b0 + wave < b1 && ru) load_w(b0 + wave, 0);
+  if (ru) {
+    const int row4 = (rank + 15) / 16 * 4;  // four ranks each
+    f32x4* s_sum = (f32x4*)(s_t + (size_t)ru * kUpParts);
+    const float* at = p.parts + (size_t)t.first * ranks;
+    for (int e = tid; e < t.rows * row4; e += kUpThreads)
+      s_sum[e] = lora_sum(at + (size_t)(e / row4) * ranks + e % row4 * 4, (size_t)p.M * ranks, pieces) * s;
+    __syncthreads();
+    if constexpr (F16) if (tid < 256) {
+      const int row = tid / 16;
+      float m = 0.f;
+      if (row < t.rows)
+        for (int r = tid % 16; r < row4; r += 16) {
+          const f32x4 v = s_sum[row * row4 + r];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(v[i]));
+        }
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+      const int e = (int)(__float_as_uint(m) >> 23);  // the largest becomes one of [2^14, 2^15)
+      s_scale[row] = __uint_as_float((uint32_t)(min(max(e, 16), 254) - 14) << 23);
+    }
+    if constexpr (F16) __syncthreads();
+    for (int item = tid; item < 16 * ru * 4; item += kUpThreads) {
+      const int row = item / (4 * ru), r8 = item % (4 * ru);
+      f32x4 v[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+      if (row < t.rows && 2 * r8 < row4) {
+        v[0] = s_sum[row * row4 + 2 * r8];
+        v[1] = s_sum[row * row4 + 2 * r8 + 1];
+      }
+      float inv = 1.f;
+      if constexpr (F16) inv = 1.0f / s_scale[row];  // a power of two: exact
+      u32x4 part[3];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float rest = v[i / 4][i % 4] * inv;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          const uint32_t b = lora_round<F16>(rest);
+          rest = __builtin_isfinite(rest) ? rest - lora_value<F16>(b) : 0.f;
+          part[k][i / 2] = i % 2 ? part[k][i / 2] | b << 16 : b;
+        }
+      }
+      uint8_t* o = s_t + (size_t)(r8 / 4) * kUpParts + ((r8 & 3) * 16 + row) * 16;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *(u32x4*)(o + 1024 * k) = part[k];
+    }
+  }
+  __syncthreads();
   float* turn = s_turn[wave];
   for (int b = b0 + wave; b < b1; b += kUpWaves) {
     f32x4 acc[4];
@@ -349,12 +380,12 @@ __global__ __launch_bounds__(kUpThreads) void lora_up_kernel(LoraArgs p, int max
         load_w(b, r + 1);
       else if (b + kUpWaves < b1)
         load_w(b + kUpWaves, 0);
-      const uint8_t* at = s_t + (size_t)r * 2048 + lane * 16;
-      const u32x4 t01 = *(const u32x4*)at, t2 = *(const u32x4*)(at + 1024);
+      const uint8_t* at = s_t + (size_t)r * kUpParts + lane * 16;
 #pragma unroll
-      for (int f = 0; f < 4; ++f) {
-        acc[f] = lora_product<F16>(v[f], t2, acc[f]);
-        acc[f] = lora_product<F16>(v[f], t01, acc[f]);
+      for (int k = 2; k >= 0; --k) {  // the smallest parts first
+        const u32x4 part = *(const u32x4*)(at + 1024 * k);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) acc[f] = lora_product<F16>(v[f], part, acc[f]);
       }
     }
     // acc: token lane % 16, features 16 f + 4 (lane / 16)..
@@ -393,7 +424,7 @@ __global__ __launch_bounds__(kUpThreads) void lora_up_kernel(LoraArgs p, int max
           u32x4 o;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            o[j] = (uint32_t)f32_to_bf16(y[i][2 * j]) | (uint32_t)f32_to_bf16(y[i][2 * j + 1]) << 16;
+            o[j] = mx_bf16x2(y[i][2 * j], y[i][2 * j + 1]);
           *(u32x4*)((uint16_t*)p.out + at) = o;
         }
       }
@@ -408,11 +439,11 @@ __global__ __launch_bounds__(kUpThreads) void lora_up_kernel(LoraArgs p, int max
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         if (i >= t.rows || n >= p.N) continue;
-        const size_t at = (size_t)s_order[i] * p.N + n;
+        const size_t at = (size_t)order[min(i, t.rows - 1)] * p.N + n;
         if constexpr (OUT32)
           ((float*)p.out)[at] = y[i];
         else
-          ((uint16_t*)p.out)[at] = f32_to_bf16(y[i]);
+          ((uint16_t*)p.out)[at] = (uint16_t)mx_bf16x2(y[i], 0.f);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -430,17 +461,17 @@ template <int TU>
 static int pieces_of(int K) {
   return std::min(kLoraMaxPieces, up_div(K / 32, 2 * kDownWaves<TU>));
 }
-int lora_pieces(int M, int K) { return lora_tile(M) == 16 ? pieces_of<1>(K) : pieces_of<4>(K); }
+int lora_pieces(int M, int K) { return lora_tile(M) == 16 ? pieces_of<1>(K) : pieces_of<2>(K); }
 
 static int padded_rank(int rank) { return (rank + 15) / 16 * 16; }
 
 size_t lora_parts_bytes(int M, int K, int max_rank) {
-  return align256((size_t)pieces_of<4>(K) * M * padded_rank(max_rank) * 4);  // the most of both kinds
+  return align256((size_t)pieces_of<2>(K) * M * padded_rank(max_rank) * 4);  // the most of both kinds
 }
 
 template <bool F16, int TU, int RU>
 static int launch_down(const LoraArgs& a, int max_tiles, int pieces, hipStream_t s) {
-  constexpr size_t lds = (size_t)kDownWaves<TU> / 2 * TU * RU * 64 * 16;
+  constexpr size_t lds = kDownLds<TU, RU>;
   auto kern = lora_down_kernel<F16, TU, RU>;
   if constexpr (lds > 65536) {
     static std::atomic<uint64_t> raised{0};
@@ -455,11 +486,13 @@ template <bool F16, int BASE, bool OUT32, bool WHOLE>
 static int launch_up(const LoraArgs& a, int max_tiles, int pieces, int num_cus, hipStream_t s) {
   const int blocks = up_div(a.N, 64), tile_units = lora_tile(a.M) / 16;
   const int tiles = std::max(1, std::min(max_tiles * tile_units / 2, up_div(a.M, 16)));
-  const int runs = std::max(1, std::min(up_div(blocks, kUpWaves), up_div(4 * num_cus, tiles)));
+  // about a workgroup a CU, as far as each wave has a block: 44.1 us at 2048 tokens of 17408 -> 5120 and rank 64,
+  // 48.9 with two (each adds the pieces up again), 48.4 and 45.8 in workgroups of four waves
+  const int runs = std::max(1, std::min(up_div(blocks, kUpWaves), up_div(num_cus, tiles)));
   const int each = up_div(blocks, runs), units = padded_rank(a.max_rank) / 16;
   hipLaunchKernelGGL((lora_up_kernel<F16, BASE, OUT32, WHOLE>), dim3(max_tiles * tile_units, up_div(blocks, each)),
-                     dim3(kUpThreads), (size_t)units * (2048 + 1024), s, a, max_tiles, units * 16, pieces, each,
-                     tile_units);
+                     dim3(kUpThreads), (size_t)(units + 1) / 2 * kUpParts + (size_t)units * 1024, s, a, max_tiles,
+                     units * 16, pieces, each, tile_units);
   return check_launch("lora_up_kernel");
 }
 template <bool F16, int BASE, bool OUT32>
@@ -489,7 +522,7 @@ static int launch_tokens(const LoraArgs& a, int num_cus, hipStream_t s) {
 
 int launch_lora(const LoraArgs& a, int num_cus, hipStream_t s) {
   if (lora_tile(a.M) == 16) return a.f16 ? launch_tokens<true, 1>(a, num_cus, s) : launch_tokens<false, 1>(a, num_cus, s);
-  return a.f16 ? launch_tokens<true, 4>(a, num_cus, s) : launch_tokens<false, 4>(a, num_cus, s);
+  return a.f16 ? launch_tokens<true, 2>(a, num_cus, s) : launch_tokens<false, 2>(a, num_cus, s);
 }
 
 }  // namespace qmlp

@@ -36,8 +36,8 @@ class LoraStack:
     """The adapters of one projection in the kernels' layout."""
 
     a: torch.Tensor     # [rank units, K / 32, 64, 8], all adapters in turn
-    b: torch.Tensor     # flat, per adapter [N / 64, rank units, 4, 32, 8]
-    meta: torch.Tensor  # int32 [adapters, 4]: rank, rank units before, scale's bits, 0
+    b: torch.Tensor     # flat, per adapter [N / 64, rank / 32, 4, 64, 8]
+    meta: torch.Tensor  # int32 [adapters, 4]: rank, rank units before, scale's bits, 32s of ranks before
     ranks: tuple
     n: int
     k: int
@@ -68,8 +68,10 @@ class LoraPlan:
     adapters: int
 
 
-def _units(rank):
-    return -(-rank // 16)
+def _units(ranks, size):
+    """Units of ``size`` ranks of each adapter, and of those before it."""
+    units = [-(-r // size) for r in ranks]
+    return units, [sum(units[:i]) for i in range(len(units))]
 
 
 def pack_lora(adapters, stream=None):
@@ -100,23 +102,23 @@ def pack_lora(adapters, stream=None):
             raise ValueError(f"adapter {i}: the scale must be finite, got {scale}")
     N, K = adapters[0][1].shape[0], first.shape[1]
     blocks = -(-N // 64)
-    units = [_units(a.shape[0]) for a, _, _ in adapters]
-    before = [sum(units[:i]) for i in range(len(units))]
+    ranks = tuple(a.shape[0] for a, _, _ in adapters)
+    units, before = _units(ranks, 16)
+    units32, before32 = _units(ranks, 32)
     with _lib.on_device(first.device, stream):
         pa = torch.zeros((sum(units) * 16, K), dtype=first.dtype, device=first.device)
-        pb = torch.empty((sum(units) * 16 * blocks * 64,), dtype=first.dtype, device=first.device)
-        for (a, b, _), u, at in zip(adapters, units, before):
-            pa[16 * at:16 * at + a.shape[0]] = a
-            wide = torch.zeros((blocks * 64, 16 * u), dtype=first.dtype, device=first.device)
-            wide[:N, :a.shape[0]] = b
-            # feature 16 f + e of a block, rank 16 u + 8 h + i -> [block][u][f][lane 16 h + e][i]
-            wide = wide.reshape(blocks, 4, 16, u, 2, 8).permute(0, 3, 1, 4, 2, 5)
-            pb[16 * at * blocks * 64:16 * (at + u) * blocks * 64] = wide.reshape(-1)
+        pb = torch.empty((sum(units32), 32 * blocks * 64), dtype=first.dtype, device=first.device)
+        for i, (a, b, _) in enumerate(adapters):
+            pa[16 * before[i]:16 * before[i] + ranks[i]] = a
+            wide = torch.zeros((blocks * 64, 32 * units32[i]), dtype=first.dtype, device=first.device)
+            wide[:N, :ranks[i]] = b
+            # feature 16 f + e of a block, rank 32 u + 8 h + j -> [block][u][f][lane 16 h + e][j]
+            wide = wide.reshape(blocks, 4, 16, units32[i], 4, 8).permute(0, 3, 1, 4, 2, 5)
+            pb[before32[i]:before32[i] + units32[i]] = wide.reshape(units32[i], -1)
         pa = pa.reshape(sum(units), 16, K // 32, 4, 8).permute(0, 2, 3, 1, 4).contiguous()
         bits = [struct.unpack("<i", struct.pack("<f", float(s)))[0] for _, _, s in adapters]
-        meta = torch.tensor([[a.shape[0], at, s, 0] for (a, _, _), at, s in zip(adapters, before, bits)],
-                            dtype=torch.int32).to(first.device)
-    return LoraStack(pa, pb, meta, tuple(a.shape[0] for a, _, _ in adapters), N, K)
+        meta = torch.tensor(list(zip(ranks, before, bits, before32)), dtype=torch.int32).to(first.device)
+    return LoraStack(pa, pb, meta, ranks, N, K)
 
 
 @functools.lru_cache(maxsize=4096)

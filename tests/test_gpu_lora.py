@@ -146,7 +146,7 @@ def test_plan_groups_every_token_once(pkg, cuda):
         ids = torch.randint(-2, L + 2, (M,), generator=g, dtype=torch.int32)
         plan = pkg.lora_plan(ids.to(cuda), L)
         w = plan.buf.cpu().numpy()
-        T = 16 if M <= 64 else 64
+        T = 16 if M <= 64 else 32
         most = M // T + min(M, L + 1)
         tiles = w[4:4 + 4 * w[3]].reshape(-1, 4)
         order = w[4 + 4 * most:]
