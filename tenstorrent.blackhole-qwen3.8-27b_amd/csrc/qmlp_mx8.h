@@ -61,15 +61,14 @@ __device__ __forceinline__ void mx8_digits(i32x4 p, int g, i32x8& low, i32x8& hi
   }
 }
 
-// D += A B for 4-bit A and 8-bit B on 32 rows x 32 columns x 64 K (mx_product's counterpart); sb: the packed
-// scale bytes.  A block that is not a number has scale 255, which makes the low digit's product one; its high
-// digit's scale byte carries into the next block of the same row then, whose outputs are lost already.
+// D += A B for 4-bit A and one digit of an 8-bit B on 32 rows x 32 columns x 64 K (mx_product's counterpart); sb:
+// the digit's scale bytes, the packed ones for the low digit, kMx8HighDigit more for the high one.  A block that is
+// not a number has scale 255, which makes the low digit's product one; its high digit's scale byte carries into the
+// next block of the same row then, whose outputs are lost already.
 template <int J>
-__device__ __forceinline__ f32x16 mx8_product(i32x4 a, const i32x8& low, const i32x8& high, f32x16 c, uint32_t sa,
-                                              uint32_t sb) {
+__device__ __forceinline__ f32x16 mx8_digit_product(i32x4 a, const i32x8& digit, f32x16 c, uint32_t sa, uint32_t sb) {
   const i32x8 a8 = __builtin_shufflevector(a, i32x4{0, 0, 0, 0}, 0, 1, 2, 3, 4, 5, 6, 7);
-  c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a8, high, c, 4, 2, J, (int)sa, J, (int)(sb + kMx8HighDigit));
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a8, low, c, 4, 2, J, (int)sa, J, (int)sb);
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a8, digit, c, 4, 2, J, (int)sa, J, (int)sb);
 }
 
 // The packed scale byte from a block's largest |x| bits (fp32).

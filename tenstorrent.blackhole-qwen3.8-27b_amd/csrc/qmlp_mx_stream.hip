@@ -121,7 +121,10 @@ __global__ __launch_bounds__(WAVES * 64) void mx_stream_kernel(const uint8_t* __
         mx8_digits(b.plane[g][J][1], 1, low, high);
 #pragma unroll
         for (int n = 0; n < NMAT; ++n)
-          acc[n][g] = mx8_product<J>(a.code[n][J], low, high, acc[n][g], a.scale[n], b.scale[g]);
+          acc[n][g] = mx8_digit_product<J>(a.code[n][J], high, acc[n][g], a.scale[n], b.scale[g] + kMx8HighDigit);
+#pragma unroll
+        for (int n = 0; n < NMAT; ++n)
+          acc[n][g] = mx8_digit_product<J>(a.code[n][J], low, acc[n][g], a.scale[n], b.scale[g]);
       }
     }
   };

@@ -232,6 +232,13 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
   auto fetch = [&](int sb, int h, int j, int k) {
     const uint32_t at = (2 * (sb & 1) + h) * T::kHalf + j * 1024;
     if (k >= WF + kB) return;
+    if constexpr (XP == 2) {  // the tokens first: their digits take time
+      if (k < kB)
+        b[j][k] = *(const i32x4*)(sx + at + k * 2048);
+      else
+        a[j][k - kB] = *(const i32x4*)(sf + at + (k - kB) * 2048);
+      return;
+    }
     if (k >= 1 && k <= kB)
       b[j][k - 1] = *(const i32x4*)(sx + at + (k - 1) * 2048);
     else
@@ -251,21 +258,33 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
   // One K-step's products, in groups of two; before each group `beside(group)` asks for what comes in
   // beside them (the order is kept as written).
   constexpr int kGroups = WF * WT * XP / 2;
-  i32x8 low[XP == 2 ? WT : 1], high[XP == 2 ? WT : 1];  // the digits of a K-step's token operands
-  auto multiply = [&](auto jc, auto full, auto beside) {
-    constexpr int J = decltype(jc)::value;
+  // 8-bit: the digits of a K-step's token operands and of the next one's, which are made plane by plane in front
+  // of the last two groups' products
+  i32x8 low[2][XP == 2 ? WT : 1], high[2][XP == 2 ? WT : 1];
+  auto digits = [&](int j, int plane) {
+    if constexpr (XP == 2) {
+#pragma unroll
+      for (int t = 0; t < WT; ++t) mx8_digits(b[j][2 * t + plane], plane, low[j][t], high[j][t]);
+    }
+  };
+  auto multiply = [&](auto jc, auto full, auto next, auto beside) {
+    constexpr int J = decltype(jc)::value, j = J & 1;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       beside(g);
       if constexpr (XP == 2) {
-        const int f = g / WT, t = g % WT;
-        if (f == 0) {
-          low[t] = high[t] = i32x8{};
-          mx8_digits(b[J & 1][2 * t], 0, low[t], high[t]);
-          mx8_digits(b[J & 1][2 * t + 1], 1, low[t], high[t]);
+        if (decltype(next)::value) {
+          if (g == (kGroups > 2 ? kGroups - 2 : 1)) digits(1 - j, 0);
+          if (g == kGroups - 1) digits(1 - j, 1);
         }
-        if (decltype(full)::value || t < nv)
-          acc[f][t] = mx8_product<J>(a[J & 1][f], low[t], high[t], acc[f][t], fs[f], xs[t]);
+        // two products' high digits, then their low ones: none waits for the sum before it
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int i = g / 2 * 2 + k, f = i / WT, t = i % WT;
+          if (decltype(full)::value || t < nv)
+            acc[f][t] = mx8_digit_product<J>(a[j][f], g % 2 ? low[j][t] : high[j][t], acc[f][t], fs[f],
+                                             xs[t] + (g % 2 ? 0u : kMx8HighDigit));
+        }
         __builtin_amdgcn_sched_barrier(0);
         continue;
       }
@@ -297,21 +316,21 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
     for (int t = 0; t < WT; ++t) xs[t] = xs_next[t];
 #pragma unroll
     for (int f = 0; f < WF; ++f) fs[f] = fs_next[f];
-    multiply(std::integral_constant<int, 0>{}, full, [&](int g) {
+    multiply(std::integral_constant<int, 0>{}, full, std::true_type{}, [&](int g) {
       spread(g, WF + kB, [&](int k) { fetch(sb, 0, 1, k); });
       if constexpr (LEFT >= 1) spread(g, 2 * kPart1, [&](int k) { issue(sb + 1, 1, 1, k); });
     });
     stage_barrier<(LEFT >= 1 ? kAhead : 0)>();
-    multiply(std::integral_constant<int, 1>{}, full, [&](int g) {
+    multiply(std::integral_constant<int, 1>{}, full, std::true_type{}, [&](int g) {
       spread(g, WF + kB, [&](int k) { fetch(sb, 1, 0, k); });
       if constexpr (LEFT >= 2) spread(g, 3 * kPart0, [&](int k) { issue(sb + 2, 0, 0, k); });
     });
-    multiply(std::integral_constant<int, 2>{}, full, [&](int g) {
+    multiply(std::integral_constant<int, 2>{}, full, std::true_type{}, [&](int g) {
       spread(g, WF + kB, [&](int k) { fetch(sb, 1, 1, k); });
       if constexpr (LEFT >= 2) spread(g, 3 * kPart1, [&](int k) { issue(sb + 2, 0, 1, k); });
     });
     stage_barrier<(LEFT >= 2 ? kAhead : 0)>();
-    multiply(std::integral_constant<int, 3>{}, full, [&](int g) {
+    multiply(std::integral_constant<int, 3>{}, full, std::bool_constant<LEFT >= 1>{}, [&](int g) {
       if constexpr (LEFT >= 1) {
         spread(g, WF + kB, [&](int k) { fetch(sb + 1, 0, 0, k); });
         spread(g, WF + WT, [&](int k) { fetch_scale(sb + 1, k); });
@@ -336,6 +355,8 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
     fetch_scale(0, k);
     fetch(0, 0, 0, k);
   }
+  digits(0, 0);
+  digits(0, 1);
   auto units = [&](auto full) {
     int sb = 0;
     for (; sb + 2 < n; ++sb) unit(sb, std::integral_constant<int, 2>{}, full);
@@ -450,12 +471,13 @@ static int launch_height(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
   return launch_tile<NMAT, 2, 4, 4, 2, MODE, 1>(p, pl.ks, s);
 }
 
-// 8-bit activations: two heights, as far as LDS goes.
+// 8-bit activations: two heights, as far as LDS goes; the higher one in waves of 128 features x 32 tokens, which make
+// half the digits of 64 x 64 for as many reads from LDS.
 template <int MODE>
 static int launch_height8(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
   constexpr int NMAT = MODE == kMxRowsOut ? 1 : 2;
   if (pl.height == 1) return launch_tile<NMAT, 2, 1, 4, 2, MODE, 2>(p, pl.ks, s);
-  return launch_tile<NMAT, 2, 2, 4, 2, MODE, 2>(p, pl.ks, s);
+  return launch_tile<NMAT, 4, 1, 2, 4, MODE, 2>(p, pl.ks, s);
 }
 
 int launch_mx_tiled(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
