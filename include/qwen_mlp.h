@@ -398,7 +398,9 @@ int qmlp_plan_split(int rows, int K, int nmat, int M, int num_cus, int* out6);
  * features and 64 tokens, 3 + h tiles of 256 features (of both matrices together) x 64 h tokens. */
 int qmlp_mx_plan(int M, int N, int K, int nmat, int num_cus, int* out5);
 
-/* The same for the products with 8-bit activations (tiles of 64 and 128 tokens only: h = 1, 2). */
+/* The same for the products with 8-bit activations: 0 to 3 as there with one unit's loads under way (1: two), 3 + h
+ * for h = 1, 2, of which full rounds may run whole and the rest in pieces of the K range, 8 the kernel of up to 16
+ * tokens. */
 int qmlp_w4a8_plan(int M, int N, int K, int nmat, int num_cus, int* out5);
 
 #ifdef __cplusplus

@@ -157,13 +157,15 @@ constexpr int kMxFewTokens = 32;  // up to here every product is streamed
 // How a product runs (mx_plan, qmlp_mx_plan.hip).  Streamed: a workgroup of 32 features x 32 tokens, four
 // waves with one unit of K under way (kMxStream) or two (kMxStreamDeep, one matrix only), or eight with
 // two (kMxStreamLong); or of 32 features x 64 tokens (kMxStreamWide).  Tiled (kMxTiles): 256 features (128
-// of gate and up each) x 64 height tokens a workgroup, the K range in ks pieces.
-enum MxKind { kMxStream, kMxStreamDeep, kMxStreamLong, kMxStreamWide, kMxTiles };
+// of gate and up each) x 64 height tokens a workgroup, the K range in ks pieces but for the first `whole` tiles.
+// Up to 16 tokens of 8-bit activations have a kernel of their own (kMxFew, height: its waves where it quantises rows).
+enum MxKind { kMxStream, kMxStreamDeep, kMxStreamLong, kMxStreamWide, kMxTiles, kMxFew };
 struct MxPlan {
   MxKind kind;
   int height, ks;
   int workgroups;
   size_t part_bytes;  // of all pieces
+  int whole;
 };
 MxPlan mx_plan(int M, int N, int K, int nmat, int num_cus, bool a8);
 int launch_mx_stream(const MxProduct& p, const MxPlan& pl, hipStream_t s);

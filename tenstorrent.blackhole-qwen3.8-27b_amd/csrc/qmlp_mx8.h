@@ -175,6 +175,53 @@ __device__ __forceinline__ uint32_t abs_max16(const float (&f)[16]) {
   return m;
 }
 
+// Finishes four neighbouring features n0.. of token t of row tile tt from the matrices' sums.  Packed outputs: a
+// block's 32 features are eight neighbouring lanes' (item: the lane's place, item % 8 in the block).
+template <int NMAT, int MODE, bool A8>
+__device__ __forceinline__ void mx_finish4(const MxOut& o, int tt, int t, int n0, int item, f32x4 (&sum)[NMAT]) {
+  const int m = tt * 32 + t;
+  if constexpr (MODE == kMxRowsOut) {
+    mx_store4(o, m, n0, sum[0]);
+  } else {
+    if constexpr (A8) {
+      sum[0] += mx_addend(o.gate_add, o, m, n0);
+      sum[NMAT - 1] += mx_addend(o.up_add, o, m, n0);
+    }
+    f32x4 h;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = silu_mul(sum[0][i], sum[NMAT - 1][i]);
+    if constexpr (MODE == kMxGated) {
+      mx_store4(o, m, n0, h);
+    } else {
+      uint32_t mx = 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = max(mx, __float_as_uint(h[i]) & 0x7fffffffu);
+#pragma unroll
+      for (int d = 1; d < 8; d <<= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, d));
+      const int kb = (n0 % kMxK) / kMxBlock;
+      const size_t u = (size_t)tt * mx_ksb(o.N) + n0 / kMxK;
+      if constexpr (MODE == kMxPacked8) {
+        const uint32_t s = mx8_scale_byte(mx);
+        const i32x4 group = mx8_join(h, item & 3, s);
+        if (m < o.M) {
+          uint8_t* unit = (uint8_t*)o.out + u * kMx8Unit;
+          if ((item & 3) == 0) *(i32x4*)(unit + mx8_at(t, kb, (item >> 2) & 1)) = group;
+          if ((item & 7) == 0) unit[mx8_scale_at(t, kb)] = (uint8_t)s;
+        }
+      } else {
+        const uint32_t s = mx_scale_byte(mx);
+        const uint32_t c = mx_codes4(h, s);
+        const uint32_t hi = (uint32_t)__shfl_xor((int)c, 1);
+        if (m < o.M) {
+          uint8_t* unit = (uint8_t*)o.out + u * kMxUnit;
+          if ((item & 1) == 0) *(uint32_t*)(unit + (kb * 32 + t) * 16 + (n0 % kMxBlock) / 2) = c | (hi << 16);
+          if ((item & 7) == 0) unit[kMxCodes + 4 * (t + 32 * (kb & 1)) + (kb >> 1)] = (uint8_t)s;
+        }
+      }
+    }
+  }
+}
+
 // 16 neighbouring values of type T (0 bf16, 1 fp16, 2 fp32; QMLP_X_*) as fp32.
 template <int T>
 __device__ __forceinline__ void mx8_load(const uint8_t* p, MxWords<T> (&w)[2]) {
@@ -193,6 +240,8 @@ __device__ __forceinline__ void mx8_floats(const MxWords<T> (&w)[2], float (&f)[
   }
 }
 
+constexpr int kMx8FewTokens = 16;
+int launch_mx8_few(const MxProduct& p, const MxPlan& pl, hipStream_t s);
 int launch_mx8_quantize(const void* x, int type, size_t row_bytes, int rows, int cols, void* packed, hipStream_t s);
 int launch_mx8_dequantize(const void* packed, int rows, int cols, void* out, bool f32, hipStream_t s);
 int launch_mx8_unpack(const void* packed, int rows, int cols, void* q, void* scales, hipStream_t s);

@@ -54,6 +54,7 @@ static int run_product(MxProduct p, void* packed_x, int num_cus, hipStream_t s) 
     p.x_type = packed;
   }
   if (p.x_type == packed) p.x_type = kMxPackedX;  // the kernels know one packed type, that of their format
+  if (plan.kind == kMxFew) return launch_mx8_few(p, plan, s);
   return plan.kind == kMxTiles ? launch_mx_tiled(p, plan, s) : launch_mx_stream(p, plan, s);
 }
 
@@ -168,7 +169,7 @@ static int plan_impl(const char* fn, bool a8, int M, int N, int K, int nmat, int
   if (!mx_tokens_ok(M) || !mx_shape_ok(N, K) || nmat < 1 || nmat > 2 || num_cus < 1)
     return set_error(QMLP_E_SHAPE, "%s: M=%d N=%d K=%d, %d matrices on %d CUs", fn, M, N, K, nmat, num_cus);
   const MxPlan p = mx_plan(M, N, K, nmat, num_cus, a8);
-  out5[0] = p.kind == kMxTiles ? kMxStreamWide + p.height : (int)p.kind;
+  out5[0] = p.kind == kMxTiles ? kMxStreamWide + p.height : p.kind == kMxFew ? 8 : (int)p.kind;
   out5[1] = p.ks;
   out5[2] = p.workgroups;
   out5[3] = (int)(p.part_bytes >> 10);

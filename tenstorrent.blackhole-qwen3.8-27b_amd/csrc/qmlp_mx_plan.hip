@@ -1,6 +1,6 @@
 // qmlp_mx_plan.hip -- how an MXFP4 product runs for its sizes (host code).
 #include "qmlp_internal.h"
-#include "qmlp_mx.h"
+#include "qmlp_mx8.h"
 
 namespace qmlp {
 
@@ -46,11 +46,14 @@ constexpr int kPieces[] = {1, 2, 3, 4, 6, 8, 12};
 // shapes; at the narrowest, 96 x 5120, streaming took 4.2 us at 2048 tokens and the planned tiles take 10.1.
 constexpr int kMostStreamed = 1024;
 
+static MxPlan plan_a8(int M, int N, int K, int nmat, int num_cus);
+
 MxPlan mx_plan(int M, int N, int K, int nmat, int num_cus, bool a8) {
+  if (a8) return plan_a8(M, N, K, nmat, num_cus);
   const double cus = num_cus;
   const long nsb = mx_ksb(K), rows = mx_row_tiles(N);
   auto up = [](long a, long b) { return (a + b - 1) / b; };
-  MxPlan best{kMxStream, 0, 1, 0, 0};
+  MxPlan best{kMxStream, 0, 1, 0, 0, 0};
   double best_us = 1e30;
   auto streamed = [&](const StreamCost& c) {
     const long ty = up(M, 32 * c.groups);
@@ -58,7 +61,7 @@ MxPlan mx_plan(int M, int N, int K, int nmat, int num_cus, bool a8) {
                       c.weight * (double)(rows * nsb) / cus + c.round * up(rows * ty, num_cus);
     if (us < best_us && M > 32 * (c.groups - 1)) {
       best_us = us;
-      best = MxPlan{c.kind, 0, 1, (int)(rows * ty), 0};
+      best = MxPlan{c.kind, 0, 1, (int)(rows * ty), 0, 0};
     }
   };
   if (M <= kMostStreamed) {
@@ -68,9 +71,8 @@ MxPlan mx_plan(int M, int N, int K, int nmat, int num_cus, bool a8) {
       for (const StreamCost& c : kPairCost) streamed(c);
   }
   if (M <= kMxFewTokens) return best;
-  for (int h = 1; h <= (a8 ? 2 : 4); ++h) {
-    TileCost c = kTileCost[nmat - 1][h - 1];
-    if (a8) c.unit *= 2, c.busy *= 2;
+  for (int h = 1; h <= 4; ++h) {
+    const TileCost& c = kTileCost[nmat - 1][h - 1];
     const long ntt = up(M, 64 * h), tiles = up(N, 256 / nmat) * ntt;
     const double filled = (double)up(M, 32) / (double)(ntt * 2 * h);  // token units that hold tokens
     for (int ks : kPieces) {
@@ -84,7 +86,72 @@ MxPlan mx_plan(int M, int N, int K, int nmat, int num_cus, bool a8) {
                         (ks > 1 ? c.sum + c.mbyte * (double)bytes * 1e-6 * filled : 0.0);
       if (us < best_us) {
         best_us = us;
-        best = MxPlan{kMxTiles, h, ks, (int)pieces, bytes};
+        best = MxPlan{kMxTiles, h, ks, (int)pieces, bytes, 0};
+      }
+    }
+  }
+  return best;
+}
+
+// The same for 8-bit activations and more than 16 tokens, in tiles of two heights (the streamed kernels with one unit
+// of K under way, but for kMxStreamDeep with two), fitted the same way to 5366 points of 10 shapes from N = 96 to 17408
+// and K = 512 to 17408 at 22 token counts: 0.9 % slower on average than the fastest measured candidate, at worst 17 %
+// (11.9 against 10.1 us at 777 tokens of 1000 x 2976).  What full rounds of tiles leave over may run in pieces by
+// itself: 2048 tokens of 17408 -> 5120, 320 tiles on 256 CUs, took 218.6 us in whole tiles and take 178.7 with 64 tiles
+// in four pieces behind 256 whole ones.
+constexpr StreamCost kStreamCost8[] = {{kMxStream, 4, 1, 3.389, 0.609, 0.138, 0.127, 0.119},
+                                       {kMxStreamDeep, 4, 1, 3.597, 0.409, 0.174, 0.050, 0.551},
+                                       {kMxStreamLong, 8, 1, 3.615, 0.676, 0.171, 0.098, 0.101},
+                                       {kMxStreamWide, 8, 2, 3.225, 1.142, 0.244, 0.143, 0.633}};
+constexpr StreamCost kPairCost8[] = {{kMxStream, 4, 1, 2.747, 1.494, 0.181, 0.181, 0.353},
+                                     {kMxStreamLong, 8, 1, 3.185, 1.359, 0.222, 0.155, 0.785}};
+constexpr TileCost kTileCost8[2][2] = {
+    {{3.55, 2.655, 0.581, 0.528, 0.609, 2.44, 0.152}, {3.83, 3.971, 0.683, 1.108, 0.311, 1.68, 0.208}},
+    {{3.98, 2.667, 0.608, 0.516, 0.318, 3.54, 0.163}, {3.83, 4.025, 0.712, 1.105, 0.115, 3.18, 0.192}}};
+
+static MxPlan plan_a8(int M, int N, int K, int nmat, int num_cus) {
+  const double cus = num_cus;
+  const long nsb = mx_ksb(K), rows = mx_row_tiles(N);
+  auto up = [](long a, long b) { return (a + b - 1) / b; };
+  if (M <= kMx8FewTokens) return MxPlan{kMxFew, rows > num_cus ? 4 : 8, 1, (int)rows, 0, 0};
+  MxPlan best{kMxStream, 0, 1, 0, 0, 0};
+  double best_us = 1e30;
+  auto streamed = [&](const StreamCost& c) {
+    const long ty = up(M, 32 * c.groups);
+    const double us = c.start + c.unit * up(nsb, c.waves) + c.product * (double)(rows * ty * nsb) / cus +
+                      c.weight * (double)(rows * nsb) / cus + c.round * up(rows * ty, num_cus);
+    if (us < best_us && M > 32 * (c.groups - 1)) {
+      best_us = us;
+      best = MxPlan{c.kind, 0, 1, (int)(rows * ty), 0, 0};
+    }
+  };
+  if (M <= kMostStreamed) {
+    if (nmat == 1)
+      for (const StreamCost& c : kStreamCost8) streamed(c);
+    else
+      for (const StreamCost& c : kPairCost8) streamed(c);
+  }
+  if (M <= kMxFewTokens) return best;
+  for (int h = 1; h <= 2; ++h) {
+    const TileCost& c = kTileCost8[nmat - 1][h - 1];
+    const long ntt = up(M, 64 * h), tiles = up(N, 256 / nmat) * ntt;
+    const double filled = (double)up(M, 32) / (double)(ntt * 2 * h);  // token units that hold tokens
+    const long most = tiles / num_cus * num_cus;
+    for (long whole : {0l, most}) {
+      for (int ks : kPieces) {
+        if (whole && (whole == tiles || ks == 1)) continue;  // the same as none
+        if (ks > nsb) break;
+        const long pieces = (tiles - whole) * ks, rest = pieces % num_cus, units = up(nsb, ks);
+        const size_t bytes = ks > 1 ? (size_t)pieces * 256 * 64 * h * 4 : 0;
+        if (bytes > kMxPartBytes) break;
+        const double first = whole / cus, turns = up(pieces, num_cus), busy = pieces / num_cus + rest / cus;
+        const double unit_turns = units * turns + nsb * first, unit_busy = units * busy + nsb * first;
+        const double us = c.start + c.round * (turns + first) + c.unit * unit_turns + c.busy * unit_busy * filled +
+                          c.weight * unit_busy / ntt + (ks > 1 ? c.sum + c.mbyte * (double)bytes * 1e-6 * filled : 0.0);
+        if (us < best_us) {
+          best_us = us;
+          best = MxPlan{kMxTiles, h, ks, (int)(whole + pieces), bytes, (int)whole};
+        }
       }
     }
   }

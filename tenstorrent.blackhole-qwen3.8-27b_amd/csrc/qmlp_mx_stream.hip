@@ -60,10 +60,10 @@ __global__ __launch_bounds__(WAVES * 64) void mx_stream_kernel(const uint8_t* __
     boff[g] = half * 32 + min(lane & 31, o.M - 1 - tt * 32);
   }
   constexpr bool kInside = XT != kMxPackedX;
-  constexpr int kBlockBytes = A8 ? 32 : 16;
+  static_assert(!(kInside && A8), "few rows in 8 bits are the few-token kernel's");
   using Tokens = std::conditional_t<A8, Mx8Stage<MG>, MxStage<MG>>;
   extern __shared__ __align__(16) uint8_t s_x[];  // kInside: codes [block][token], scales [unit][half][token]
-  uint8_t* s_scale = s_x + (size_t)nsb * 8 * o.M * kBlockBytes;
+  uint8_t* s_scale = s_x + (size_t)nsb * 8 * o.M * 16;
   auto load = [&](int sb, MxStage<NMAT>& a, Tokens& b) {
     const size_t u = (size_t)sb * kMxUnit;
 #pragma unroll
@@ -93,15 +93,8 @@ __global__ __launch_bounds__(WAVES * 64) void mx_stream_kernel(const uint8_t* __
     }
   };
   // kInside: the token operands of one unit from LDS
-  auto fetch = [&](int sb, Tokens& b) {
+  auto fetch = [&](int sb, MxStage<MG>& b) {
     const int tok = min(lane & 31, o.M - 1);
-    if constexpr (A8) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-          b.plane[0][j][p] = *(const i32x4*)(s_x + ((sb * 8 + 2 * j + half) * o.M + tok) * 32 + 16 * p);
-    } else
 #pragma unroll
     for (int j = 0; j < 4; ++j) b.code[0][j] = *(const i32x4*)(s_x + ((sb * 8 + 2 * j + half) * o.M + tok) * 16);
     b.scale[0] = *(const uint32_t*)(s_scale + ((sb * 2 + half) * o.M + tok) * 4);
@@ -147,12 +140,12 @@ __global__ __launch_bounds__(WAVES * 64) void mx_stream_kernel(const uint8_t* __
   };
   MxStage<NMAT> a[D];
   Tokens b[kInside ? 1 : D];
-  // kInside: the token rows are requested before the first weights and quantised, kXAhead chunks of 8 (A8: 16)
+  // kInside: the token rows are requested before the first weights and quantised, kXAhead chunks of 8
   // values a thread at a time, while those are on their way.  Every lane takes part in each chunk (four
-  // lanes, or two, share a block); a row has nch chunks, those behind K are the padding.
-  constexpr int kXAhead = A8 ? 2 : 4, kXT = kInside ? XT : 0, kXWords = A8 ? 2 : 1, kXValues = 8 * kXWords;
-  MxWords<kXT> chunk[kXAhead][kXWords];
-  const int nch = nsb * (kMxK / kXValues), items = nch * o.M;
+  // lanes share a block); a row has nch chunks, those behind K are the padding.
+  constexpr int kXAhead = 4, kXT = kInside ? XT : 0;
+  MxWords<kXT> chunk[kXAhead];
+  const int nch = nsb * 32, items = nch * o.M;
   auto x_row = [&](int item) {  // item / nch, for up to kMxInside rows
     int r = 0;
 #pragma unroll
@@ -162,34 +155,17 @@ __global__ __launch_bounds__(WAVES * 64) void mx_stream_kernel(const uint8_t* __
   auto x_load = [&](int first) {
 #pragma unroll
     for (int i = 0; i < kXAhead; ++i) {
-      const int item = first + i * WAVES * 64 + (int)threadIdx.x, row = x_row(item), k = (item - row * nch) * kXValues;
-#pragma unroll
-      for (int w = 0; w < kXWords; ++w)
-        chunk[i][w] = item < items && k < K
-                          ? mx_load8<kXT>(x + (size_t)row * row_bytes + (size_t)(k + 8 * w) * (XT == 2 ? 4 : 2))
-                          : MxWords<kXT>{};
+      const int item = first + i * WAVES * 64 + (int)threadIdx.x, row = x_row(item), k = (item - row * nch) * 8;
+      chunk[i] = item < items && k < K ? mx_load8<kXT>(x + (size_t)row * row_bytes + (size_t)k * (XT == 2 ? 4 : 2))
+                                       : MxWords<kXT>{};
     }
   };
   auto x_quantise = [&](int first) {
 #pragma unroll
     for (int i = 0; i < kXAhead; ++i) {
-      const int item = first + i * WAVES * 64 + (int)threadIdx.x, row = x_row(item), c = item - row * nch;
-      if constexpr (A8) {
-        const int kb = c >> 1;
-        float f[16];
-        mx8_floats<kXT>(chunk[i], f);
-        uint32_t top = abs_max16(f);
-        top = max(top, (uint32_t)__shfl_xor((int)top, 1));
-        const uint32_t s = mx8_scale_byte(top);
-        const i32x4 group = mx8_group(f, s);
-        if (item >= items) continue;
-        *(i32x4*)(s_x + (kb * o.M + row) * 32 + (c & 1) * 16) = group;
-        if ((c & 1) == 0) s_scale[(((kb >> 3) * 2 + (kb & 1)) * o.M + row) * 4 + ((kb >> 1) & 3)] = (uint8_t)s;
-        continue;
-      }
-      const int kb = c >> 2;
+      const int item = first + i * WAVES * 64 + (int)threadIdx.x, row = x_row(item), c = item - row * nch, kb = c >> 2;
       float f[8];
-      mx_floats<kXT>(chunk[i][0], f);
+      mx_floats<kXT>(chunk[i], f);
       const uint32_t s = mx_scale_byte(max4(abs_max8(f)));
       const uint32_t code = mx_codes8(f, s);
       if (item >= items) continue;
@@ -247,47 +223,7 @@ __global__ __launch_bounds__(WAVES * 64) void mx_stream_kernel(const uint8_t* __
 #pragma unroll
       for (int w = 1; w < kHalfWaves; ++w) sum[n] += *(const f32x4*)&s_part[n][g][w][t * kRow + f];
     }
-    const int m = tt * 32 + t, n0 = ft * 32 + f;
-    if constexpr (MODE == kMxRowsOut) {
-      mx_store4(o, m, n0, sum[0]);
-    } else {
-      if constexpr (A8) {
-        sum[0] += mx_addend(o.gate_add, o, m, n0);
-        sum[NMAT - 1] += mx_addend(o.up_add, o, m, n0);
-      }
-      f32x4 h;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = silu_mul(sum[0][i], sum[NMAT - 1][i]);
-      if constexpr (MODE == kMxGated) {
-        mx_store4(o, m, n0, h);
-      } else {  // the 32 features of a token are one block, in 8 neighbouring lanes
-        uint32_t mx = 0u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = max(mx, __float_as_uint(h[i]) & 0x7fffffffu);
-#pragma unroll
-        for (int d = 1; d < 8; d <<= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, d));
-        if constexpr (MODE == kMxPacked8) {
-          const uint32_t s = mx8_scale_byte(mx);
-          const i32x4 group = mx8_join(h, item & 3, s);
-          if (m < o.M) {
-            uint8_t* unit = (uint8_t*)o.out + ((size_t)tt * mx_ksb(o.N) + n0 / kMxK) * kMx8Unit;
-            const int kb = (n0 % kMxK) / kMxBlock;
-            if ((item & 3) == 0) *(i32x4*)(unit + mx8_at(t, kb, (item >> 2) & 1)) = group;
-            if ((item & 7) == 0) unit[mx8_scale_at(t, kb)] = (uint8_t)s;
-          }
-          continue;
-        }
-        const uint32_t s = mx_scale_byte(mx);
-        const uint32_t c = mx_codes4(h, s);
-        const uint32_t hi = (uint32_t)__shfl_xor((int)c, 1);
-        if (m < o.M) {
-          uint8_t* unit = (uint8_t*)o.out + ((size_t)tt * mx_ksb(o.N) + n0 / kMxK) * kMxUnit;
-          const int kb = (n0 % kMxK) / kMxBlock;
-          if ((item & 1) == 0) *(uint32_t*)(unit + (kb * 32 + t) * 16 + f / 2) = c | (hi << 16);
-          if ((item & 7) == 0) unit[kMxCodes + 4 * (t + 32 * (kb & 1)) + (kb >> 1)] = (uint8_t)s;
-        }
-      }
-    }
+    mx_finish4<NMAT, MODE, A8>(o, tt, t, ft * 32 + f, item, sum);
   }
 }
 
@@ -295,7 +231,7 @@ template <int NMAT, int WAVES, int MG, int D, int MODE, int XT, bool A8>
 static int launch_stream(const MxProduct& p, hipStream_t s) {
   const dim3 grid(mx_row_tiles(p.o.N), (mx_row_tiles(p.o.M) + MG - 1) / MG);
   const int nsb = mx_ksb(p.K);
-  const size_t lds = XT == kMxPackedX ? 0 : (size_t)nsb * p.o.M * (8 * (A8 ? 32 : 16) + 8);
+  const size_t lds = XT == kMxPackedX ? 0 : (size_t)nsb * p.o.M * (8 * 16 + 8);
   auto kern = mx_stream_kernel<NMAT, WAVES, MG, D, MODE, XT, A8>;
   launch_timed(p.slot, kern, grid, dim3(WAVES * 64), lds, s, p.x, p.w0, p.w1, nsb, p.o, p.K, p.row_bytes);
   return check_launch("mx_stream_kernel");
@@ -304,33 +240,33 @@ static int launch_stream(const MxProduct& p, hipStream_t s) {
 template <int MODE, int XT, bool A8>
 static int launch_mode(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
   constexpr int NMAT = MODE == kMxRowsOut ? 1 : 2;
-  if constexpr (XT == kMxPackedX) {
-    if (pl.kind == kMxStreamWide) return launch_stream<NMAT, NMAT == 1 ? 8 : 4, 2, 2, MODE, XT, A8>(p, s);
+  if constexpr (XT == kMxPackedX && !(A8 && NMAT == 2)) {
+    if (pl.kind == kMxStreamWide) return launch_stream<NMAT, NMAT == 1 ? 8 : 4, 2, A8 ? 1 : 2, MODE, XT, A8>(p, s);
   }
   if constexpr (NMAT == 1) {
     if (pl.kind == kMxStreamDeep) return launch_stream<1, 4, 1, 2, MODE, XT, A8>(p, s);
   }
-  if (pl.kind == kMxStreamLong) return launch_stream<NMAT, 8, 1, 2, MODE, XT, A8>(p, s);
+  if (pl.kind == kMxStreamLong) return launch_stream<NMAT, 8, 1, A8 ? 1 : 2, MODE, XT, A8>(p, s);
   return launch_stream<NMAT, 4, 1, 1, MODE, XT, A8>(p, s);
 }
 
-template <int MODE, bool A8>
+template <int MODE>
 static int launch_few(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
-  if (p.x_type == 0) return launch_mode<MODE, 0, A8>(p, pl, s);
-  if (p.x_type == 1) return launch_mode<MODE, 1, A8>(p, pl, s);
-  if (p.x_type == 2) return launch_mode<MODE, 2, A8>(p, pl, s);
-  return launch_mode<MODE, kMxPackedX, A8>(p, pl, s);
+  if (p.x_type == 0) return launch_mode<MODE, 0, false>(p, pl, s);
+  if (p.x_type == 1) return launch_mode<MODE, 1, false>(p, pl, s);
+  if (p.x_type == 2) return launch_mode<MODE, 2, false>(p, pl, s);
+  return launch_mode<MODE, kMxPackedX, false>(p, pl, s);
 }
 
 int launch_mx_stream(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
   if (p.a8) {
-    if (p.mode == kMxRowsOut) return launch_few<kMxRowsOut, true>(p, pl, s);
-    if (p.mode == kMxGated) return launch_few<kMxGated, true>(p, pl, s);
-    return launch_few<kMxPacked8, true>(p, pl, s);
+    if (p.mode == kMxRowsOut) return launch_mode<kMxRowsOut, kMxPackedX, true>(p, pl, s);
+    if (p.mode == kMxGated) return launch_mode<kMxGated, kMxPackedX, true>(p, pl, s);
+    return launch_mode<kMxPacked8, kMxPackedX, true>(p, pl, s);
   }
-  if (p.mode == kMxRowsOut) return launch_few<kMxRowsOut, false>(p, pl, s);
-  if (p.mode == kMxGated) return launch_few<kMxGated, false>(p, pl, s);
-  return launch_few<kMxPacked, false>(p, pl, s);
+  if (p.mode == kMxRowsOut) return launch_few<kMxRowsOut>(p, pl, s);
+  if (p.mode == kMxGated) return launch_few<kMxGated>(p, pl, s);
+  return launch_few<kMxPacked>(p, pl, s);
 }
 
 }  // namespace qmlp

@@ -156,15 +156,19 @@ template <int NMAT, int WF, int WT, int NF, int NT, int MODE, int XP>
 __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t* __restrict__ x,
                                                                   const uint8_t* __restrict__ w0,
                                                                   const uint8_t* __restrict__ w1, int nsb, int ntt,
-                                                                  int ks, f32x4* __restrict__ parts, MxOut o) {
+                                                                  int whole, int ks, f32x4* __restrict__ parts,
+                                                                  MxOut o) {
   using T = MxTile<NMAT, WF, WT, NF, NT, XP>;
   extern __shared__ __align__(16) uint8_t s_stage[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wf = wave % NF, wt = wave / NF;
-  // the tile, and the piece q of its K units
-  const int piece = xcd_run(blockIdx.x, gridDim.x), tile = piece / ks, q = piece - tile * ks;
+  // the tile, and the piece q of its K units: the first `whole` tiles run whole, the others in ks pieces
+  const bool split = (int)blockIdx.x >= whole && ks > 1;
+  const int piece = (int)blockIdx.x < whole ? xcd_run(blockIdx.x, whole) : xcd_run(blockIdx.x - whole, gridDim.x - whole);
+  const int pieces = split ? ks : 1;
+  const int tile = (int)blockIdx.x < whole ? piece : whole + piece / pieces, q = split ? piece % pieces : 0;
   const int ft = tile / ntt, tt = tile % ntt;
-  const int u0 = q * nsb / ks, n = (q + 1) * nsb / ks - u0;
+  const int u0 = q * nsb / pieces, n = (q + 1) * nsb / pieces - u0;
   const int ftiles = mx_row_tiles(o.N), ttiles = mx_row_tiles(o.M);
   const uint32_t lds0 = lds_address(s_stage);
   const uint32_t lds_scales = lds0 + 4 * T::kHalf;
@@ -368,7 +372,7 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
   else
     units(std::false_type{});
   constexpr int per = WF / NMAT;
-  if (WT <= 2 && ks > 1) {  // the sums as the lanes hold them; mx_sum_kernel adds the pieces up
+  if (WT <= 2 && split) {  // the sums as the lanes hold them; mx_sum_kernel adds the pieces up
     f32x4* at = parts + ((size_t)piece * T::kWaves + wave) * (WF * WT * 4 * 64) + lane;
 #pragma unroll
     for (int f = 0; f < WF; ++f)
@@ -406,13 +410,13 @@ __global__ __launch_bounds__(NF* NT * 64, 1) void mx_tiled_kernel(const uint8_t*
 // features x 32 tokens.  Bound by its reads and its launch: 4.1-4.8 us for 15.7 MB of pieces (201 tokens of
 // 5120 x 8704).  A launch of its own, so that every CU takes part and no block waits for another.
 template <int NMAT, int WF, int WT, int NF, int NT, int MODE, int XP>
-__global__ __launch_bounds__(256) void mx_sum_kernel(const f32x4* __restrict__ parts, int tiles, int ntt, int ks,
-                                                     MxOut o) {
+__global__ __launch_bounds__(256) void mx_sum_kernel(const f32x4* __restrict__ parts, int whole, int tiles, int ntt,
+                                                     int ks, MxOut o) {
   using T = MxTile<NMAT, WF, WT, NF, NT, XP>;
   constexpr int per = WF / NMAT, kItems = T::kWaves * per * WT;
   __shared__ __align__(16) float s_turn[4][kMxTurn];
   const int lane = threadIdx.x & 63;
-  const int item = blockIdx.x * 4 + (threadIdx.x >> 6), tile = item / kItems, r = item % kItems;
+  const int item = blockIdx.x * 4 + (threadIdx.x >> 6), tile = whole + item / kItems, r = item % kItems;
   if (tile >= tiles) return;
   const int wave = r / (per * WT), f = r / WT % per, t = r % WT;
   const int wf = wave % NF, wt = wave / NF, ft = tile / ntt, tt = tile % ntt;
@@ -425,7 +429,7 @@ __global__ __launch_bounds__(256) void mx_sum_kernel(const f32x4* __restrict__ p
     for (int k = 0; k < 4; ++k) v[m][k] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 2
   for (int q = 0; q < ks; ++q) {
-    const f32x4* at = parts + ((size_t)(tile * ks + q) * T::kWaves + wave) * (WF * WT * 4 * 64) + lane;
+    const f32x4* at = parts + ((size_t)((tile - whole) * ks + q) * T::kWaves + wave) * (WF * WT * 4 * 64) + lane;
 #pragma unroll
     for (int m = 0; m < NMAT; ++m)
 #pragma unroll
@@ -435,29 +439,29 @@ __global__ __launch_bounds__(256) void mx_sum_kernel(const f32x4* __restrict__ p
 }
 
 template <typename T, int NMAT, int MODE, int WF, int WT, int NF, int NT, int XP>
-static int launch_sum(const MxProduct& p, int tiles, int ntt, int ks, hipStream_t s) {
+static int launch_sum(const MxProduct& p, int whole, int tiles, int ntt, int ks, hipStream_t s) {
   constexpr int kItems = T::kWaves * WF / NMAT * WT;
-  launch_timed_part(p.slot, 2, mx_sum_kernel<NMAT, WF, WT, NF, NT, MODE, XP>, dim3((tiles * kItems + 3) / 4), dim3(256), 0, s,
-                    (const f32x4*)p.parts, tiles, ntt, ks, p.o);
+  launch_timed_part(p.slot, 2, mx_sum_kernel<NMAT, WF, WT, NF, NT, MODE, XP>, dim3(((tiles - whole) * kItems + 3) / 4),
+                    dim3(256), 0, s, (const f32x4*)p.parts, whole, tiles, ntt, ks, p.o);
   return check_launch("mx_sum_kernel");
 }
 
 template <int NMAT, int WF, int WT, int NF, int NT, int MODE, int XP>
-static int launch_tile(const MxProduct& p, int ks, hipStream_t s) {
+static int launch_tile(const MxProduct& p, int whole, int ks, hipStream_t s) {
   using T = MxTile<NMAT, WF, WT, NF, NT, XP>;
   auto kern = mx_tiled_kernel<NMAT, WF, WT, NF, NT, MODE, XP>;
   static std::atomic<uint64_t> raised{0};
   if (int rc = raise_lds_once((const void*)kern, T::kLds, raised)) return rc;
   const int nft = (p.o.N + T::kFeatures - 1) / T::kFeatures, ntt = (p.o.M + T::kTokens - 1) / T::kTokens;
   const int tiles = nft * ntt;
-  const size_t part_bytes = (size_t)tiles * ks * (T::kWaves * WF * WT * 4096);
-  if (ks > mx_ksb(p.K) || (ks > 1 && (WT > 2 || part_bytes > kMxPartBytes)))  // never planned
+  const size_t part_bytes = (size_t)(tiles - whole) * ks * (T::kWaves * WF * WT * 4096);
+  if (ks > mx_ksb(p.K) || whole < 0 || whole > tiles || (ks > 1 && (WT > 2 || part_bytes > kMxPartBytes)))  // never planned
     return set_error(QMLP_E_WORKSPACE, "mx_tiled_kernel: %d tiles in %d pieces", tiles, ks);
-  launch_timed_part(p.slot, ks > 1 ? 1 : 3, kern, dim3(tiles * ks), dim3(T::kWaves * 64), T::kLds, s, p.x, p.w0, p.w1,
-                    mx_ksb(p.K), ntt, ks, (f32x4*)p.parts, p.o);
+  launch_timed_part(p.slot, ks > 1 ? 1 : 3, kern, dim3(whole + (tiles - whole) * ks), dim3(T::kWaves * 64), T::kLds, s, p.x, p.w0, p.w1,
+                    mx_ksb(p.K), ntt, whole, ks, (f32x4*)p.parts, p.o);
   if (int rc = check_launch("mx_tiled_kernel")) return rc;
   if constexpr (WT <= 2) {  // mx_plan splits no higher tile
-    if (ks > 1) return launch_sum<T, NMAT, MODE, WF, WT, NF, NT, XP>(p, tiles, ntt, ks, s);
+    if (ks > 1) return launch_sum<T, NMAT, MODE, WF, WT, NF, NT, XP>(p, whole, tiles, ntt, ks, s);
   }
   return 0;
 }
@@ -465,10 +469,10 @@ static int launch_tile(const MxProduct& p, int ks, hipStream_t s) {
 template <int MODE>
 static int launch_height(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
   constexpr int NMAT = MODE == kMxRowsOut ? 1 : 2;
-  if (pl.height == 1) return launch_tile<NMAT, 2, 1, 4, 2, MODE, 1>(p, pl.ks, s);
-  if (pl.height == 2) return launch_tile<NMAT, 2, 2, 4, 2, MODE, 1>(p, pl.ks, s);
-  if (pl.height == 3) return launch_tile<NMAT, 2, 3, 4, 2, MODE, 1>(p, pl.ks, s);
-  return launch_tile<NMAT, 2, 4, 4, 2, MODE, 1>(p, pl.ks, s);
+  if (pl.height == 1) return launch_tile<NMAT, 2, 1, 4, 2, MODE, 1>(p, pl.whole, pl.ks, s);
+  if (pl.height == 2) return launch_tile<NMAT, 2, 2, 4, 2, MODE, 1>(p, pl.whole, pl.ks, s);
+  if (pl.height == 3) return launch_tile<NMAT, 2, 3, 4, 2, MODE, 1>(p, pl.whole, pl.ks, s);
+  return launch_tile<NMAT, 2, 4, 4, 2, MODE, 1>(p, pl.whole, pl.ks, s);
 }
 
 // 8-bit activations: two heights, as far as LDS goes; the higher one in waves of 128 features x 32 tokens, which make
@@ -476,8 +480,8 @@ static int launch_height(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
 template <int MODE>
 static int launch_height8(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
   constexpr int NMAT = MODE == kMxRowsOut ? 1 : 2;
-  if (pl.height == 1) return launch_tile<NMAT, 2, 1, 4, 2, MODE, 2>(p, pl.ks, s);
-  return launch_tile<NMAT, 4, 1, 2, 4, MODE, 2>(p, pl.ks, s);
+  if (pl.height == 1) return launch_tile<NMAT, 2, 1, 4, 2, MODE, 2>(p, pl.whole, pl.ks, s);
+  return launch_tile<NMAT, 4, 1, 2, 4, MODE, 2>(p, pl.whole, pl.ks, s);
 }
 
 int launch_mx_tiled(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
