@@ -81,66 +81,74 @@ __device__ __forceinline__ float mx8_inverse(uint32_t byte) {
   return __uint_as_float((257u - byte) << 23);  // of no use for kMxNan
 }
 
-// 16 values -> one group.  Adding 2^23 to a magnitude of at most 127 rounds it to an integer, half to even.
-__device__ __forceinline__ i32x4 mx8_group(const float (&v)[16], uint32_t byte) {
-  const float inv = mx8_inverse(byte);
-  uint32_t low[4] = {0, 0, 0, 0}, high[4] = {0, 0, 0, 0};  // the last ones take nothing
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const uint32_t q = __float_as_uint(fminf(fabsf(v[i]) * inv, 127.0f) + 8388608.0f) & 127u;
-    const uint32_t l = (q & 15u) | ((__float_as_uint(v[i]) >> 26) & 32u), h = q >> 4;
-    const int d = 6 * i / 32, at = 6 * i % 32;
-    low[d] |= l << at;
-    high[d] |= h << at;
-    if (at > 26) {
-      low[d + 1] |= l >> (32 - at);
-      high[d + 1] |= h >> (32 - at);
-    }
-  }
-  if (byte == kMxNan) return i32x4{0, 0, 0, 0};
+// A value's digits: {s, q's five low bits} as a 6-bit field, and q's two high bits.  Adding 2^23 rounds the scaled
+// magnitude to an integer, half to even, in the sum's low bits; 128 and more (in a block's saturating values) become
+// 127.
+struct Mx8Digits {
+  uint32_t field, high;
+};
+__device__ __forceinline__ Mx8Digits mx8_digits_of(float v, float inv) {
+  const uint32_t q = min(__float_as_uint(fmaf(fabsf(v), inv, 8388608.0f)), 0x4b00007fu);
+  return Mx8Digits{(q & 31u) | ((__float_as_uint(v) >> 26) & ~31u), (q >> 5) & 3u};
+}
+// A group from the 96-bit streams of its fields and of its high bits (from bit 1 of each field on).
+__device__ __forceinline__ i32x4 mx8_assemble(const uint32_t (&f)[3], const uint32_t (&h)[3]) {
+  // the high digit's low bit, bit 4 of a field here, goes to bit 0 of it, 32 bits before that
+  const uint32_t down[3] = {__builtin_amdgcn_alignbit(f[1], f[0], 4), __builtin_amdgcn_alignbit(f[2], f[1], 4), f[2] >> 4};
   i32x4 p;
   uint32_t upper = 0;
 #pragma unroll
   for (int d = 0; d < 3; ++d) {
-    p[d] = (int)(low[d] | (high[(d + 1) % 3] & mx8_first((d + 1) % 3)));
-    upper |= high[d] & mx8_upper(d);
+    const int next = (d + 1) % 3;
+    p[d] = (int)((f[d] & ~mx8_first(next)) | (down[next] & mx8_first(next)));
+    upper |= h[d] & mx8_upper(d);
   }
   p[3] = (int)upper;
   return p;
 }
 
+// 16 values -> one group.
+__device__ __forceinline__ i32x4 mx8_group(const float (&v)[16], uint32_t byte) {
+  const float inv = mx8_inverse(byte);
+  uint32_t f[3] = {0, 0, 0}, h[3] = {0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const Mx8Digits q = mx8_digits_of(v[i], inv);
+    const int d = 6 * i / 32, at = 6 * i % 32, dh = (6 * i + 1) / 32, ah = (6 * i + 1) % 32;
+    f[d] |= q.field << at;
+    h[dh] |= q.high << ah;
+    if (at > 26 && d < 2) f[d + 1] |= q.field >> (32 - at);
+    if (ah > 30 && dh < 2) h[dh + 1] |= q.high >> (32 - ah);
+  }
+  const i32x4 p = mx8_assemble(f, h);
+  return byte == kMxNan ? i32x4{0, 0, 0, 0} : p;
+}
+
 // The same from four neighbouring lanes of four values each (part 0..3 of the group): all four get the group.
 __device__ __forceinline__ i32x4 mx8_join(f32x4 v, int part, uint32_t byte) {
   const float inv = mx8_inverse(byte);
-  uint32_t l = 0, h = 0;  // four fields, 24 bits
+  uint32_t f = 0, h = 0;  // four fields, 24 bits
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t q = __float_as_uint(fminf(fabsf(v[i]) * inv, 127.0f) + 8388608.0f) & 127u;
-    l |= ((q & 15u) | ((__float_as_uint(v[i]) >> 26) & 32u)) << (6 * i);
-    h |= (q >> 4) << (6 * i);
+    const Mx8Digits q = mx8_digits_of(v[i], inv);
+    f |= q.field << (6 * i);
+    h |= q.high << (6 * i + 1);
   }
-  if (byte == kMxNan) l = h = 0;
-  auto place = [&](uint32_t f, uint32_t (&o)[3]) {
-    o[0] = part == 0 ? f : part == 1 ? f << 24 : 0u;
-    o[1] = part == 1 ? f >> 8 : part == 2 ? f << 16 : 0u;
-    o[2] = part == 2 ? f >> 16 : part == 3 ? f << 8 : 0u;
+  auto place = [&](uint32_t v, uint32_t (&o)[3]) {
+    o[0] = part == 0 ? v : part == 1 ? v << 24 : 0u;
+    o[1] = part == 1 ? v >> 8 : part == 2 ? v << 16 : 0u;
+    o[2] = part == 2 ? v >> 16 : part == 3 ? v << 8 : 0u;
+#pragma unroll
+    for (int d = 0; d < 3; ++d) {
+      o[d] |= (uint32_t)__shfl_xor((int)o[d], 1);
+      o[d] |= (uint32_t)__shfl_xor((int)o[d], 2);
+    }
   };
-  uint32_t low[3], high[3];
-  place(l, low);
-  place(h, high);
-  i32x4 p = {0, 0, 0, 0};
-#pragma unroll
-  for (int d = 0; d < 3; ++d) {
-    p[d] |= (int)low[d];
-    p[(d + 2) % 3] |= (int)(high[d] & mx8_first(d));
-    p[3] |= (int)(high[d] & mx8_upper(d));
-  }
-#pragma unroll
-  for (int d = 0; d < 4; ++d) {
-    p[d] |= __shfl_xor(p[d], 1);
-    p[d] |= __shfl_xor(p[d], 2);
-  }
-  return p;
+  uint32_t fields[3], highs[3];
+  place(f, fields);
+  place(h, highs);
+  const i32x4 p = mx8_assemble(fields, highs);
+  return byte == kMxNan ? i32x4{0, 0, 0, 0} : p;
 }
 
 // A group's integers q.
