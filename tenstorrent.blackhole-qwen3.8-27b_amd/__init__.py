@@ -29,8 +29,8 @@ from .mlp import (
     workspace_pool,
 )
 from .mxfp4 import MxTensor, mxfp4_linear, mxfp4_swiglu, quantize_mxfp4
-from .lora import LoraPlan, LoraStack, lora_linear, lora_plan, pack_lora
-from .w4a8 import Mx8Tensor, add_rmsnorm, quantize_mxint8, w4a8_linear, w4a8_swiglu
+from .lora import LoraPlan, LoraStack, MLPAdapters, lora_linear, lora_plan, pack_lora
+from .w4a8 import Mx8Tensor, add_rmsnorm, quantize_mxint8, w4a8_linear, w4a8_mlp, w4a8_swiglu
 
 __all__ = [
     "FMT_BF4", "FMT_BF16", "FMT_BFP8", "FMT_MXFP4", "LIB_PATH", "QmlpError", "lib", "MATRIX_FORMATS", "WEIGHT_FORMATS",
@@ -38,6 +38,7 @@ __all__ = [
     "mlp_forward_rmsnorm", "new_workspace", "pack_canonical", "pack_canonical_bfp8", "pack_weight", "quantize_bf4",
     "quantize_bfp8", "unpack_bfp8", "unpack_canonical", "workspace_bytes", "WorkspacePool", "workspace_pool",
     "MxTensor", "mxfp4_linear", "mxfp4_swiglu", "quantize_mxfp4",
-    "LoraPlan", "LoraStack", "lora_linear", "lora_plan", "pack_lora",
-    "Mx8Tensor", "add_rmsnorm", "quantize_mxint8", "w4a8_linear", "w4a8_swiglu",
+    "LoraPlan", "LoraStack", "MLPAdapters", "lora_linear", "lora_plan", "pack_lora",
+    "Mx8Tensor", "add_rmsnorm", "quantize_mxint8", "w4a8_linear", "w4a8_mlp",
+    "w4a8_swiglu",
 ]

@@ -39,16 +39,10 @@ class LoraStack:
     b: torch.Tensor     # flat, per adapter [N / 64, rank / 32, 4, 64, 8]
     meta: torch.Tensor  # int32 [adapters, 4]: rank, rank units before, scale's bits, 32s of ranks before
     ranks: tuple
+    max_rank: int
+    adapters: int
     n: int
     k: int
-
-    @property
-    def adapters(self):
-        return len(self.ranks)
-
-    @property
-    def max_rank(self):
-        return max(self.ranks)
 
     @property
     def device(self):
@@ -57,6 +51,15 @@ class LoraStack:
     @property
     def nbytes(self):
         return sum(t.numel() * t.element_size() for t in (self.a, self.b, self.meta))
+
+
+@dataclass(frozen=True)
+class MLPAdapters:
+    """The adapters of one feed-forward block, None where a projection has none; fields as in ``MLPWeights``."""
+
+    w1: LoraStack = None  # gate_proj
+    w2: LoraStack = None  # down_proj
+    w3: LoraStack = None  # up_proj
 
 
 @dataclass(frozen=True)
@@ -118,7 +121,7 @@ def pack_lora(adapters, stream=None):
         pa = pa.reshape(sum(units), 16, K // 32, 4, 8).permute(0, 2, 3, 1, 4).contiguous()
         bits = [struct.unpack("<i", struct.pack("<f", float(s)))[0] for _, _, s in adapters]
         meta = torch.tensor(list(zip(ranks, before, bits, before32)), dtype=torch.int32).to(first.device)
-    return LoraStack(pa, pb, meta, ranks, N, K)
+    return LoraStack(pa, pb, meta, ranks, max(ranks), len(ranks), N, K)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -180,9 +183,9 @@ def lora_linear(x, stack, plan, base=None, out=None, out_dtype=None, stream=None
     _same_device(device, stack=stack.a, plan=plan.buf, base=base, out=out)
     with _lib.on_device(device, stream):
         if out is None:
-            out = torch.empty((M, N), dtype=dtype, device=device)
+            out = x.new_empty((M, N), dtype=dtype)
         nbytes = _workspace_bytes(M, K, stack.max_rank)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
         rc = _lib.lib().qmlp_lora_linear(x.data_ptr(), x_type, stride, stack.a.data_ptr(), stack.b.data_ptr(),
                                          stack.meta.data_ptr(), stack.adapters, stack.max_rank, plan.buf.data_ptr(),
                                          None if base is None else base.data_ptr(), out.data_ptr(), ws.data_ptr(),

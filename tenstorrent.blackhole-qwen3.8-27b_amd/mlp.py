@@ -26,8 +26,9 @@ from . import _lib
 # MLP weight formats.  "bf4" is the reference's mixed layout (``mlp.py:17-19,164-169``): gate/up in
 # bf4 (3 magnitude bits), down in bfp8.
 # "mxfp4" is microscaled 4-bit floating point (OCP MX) for all three matrices; the activations are
-# quantised to it in every call.
+# quantised in every call, to the same format or to 8 bits (ACTIVATION_FORMATS).
 WEIGHT_FORMATS = ("bf16", "bfp8", "bf4", "mxfp4")
+ACTIVATION_FORMATS = ("mxfp4", "mxint8")
 MATRIX_FORMATS = ("bf16", "bfp8", "bf4", "mxfp4")
 _MANTISSA_BITS = {"bfp8": 7, "bf4": 3}
 
@@ -626,18 +627,29 @@ class Qwen36MLP:
     default.  ``forward`` allocates nothing but its output (and nothing at all when ``out`` is
     given), so it may run inside a HIP graph capture on a stream that already holds a large enough
     workspace.
+
+    ``activation_format`` (mxfp4 weights only): "mxfp4", the default there, or "mxint8" -- activations in 8 bits
+    (``w4a8_mlp``), whose calls take ``adapters`` and the batch's ``plan`` too and allocate their scratch from
+    torch's caching allocator instead of the pool.
     """
 
     def __init__(self, mesh_device, state_dict, tensor_cache_path=None, args=None, tt_ccl=None,
-                 weight_format="bfp8", max_tokens=2048, pool=None):
+                 weight_format="bfp8", max_tokens=2048, pool=None, activation_format=None):
         self.device = torch.device(mesh_device) if not isinstance(mesh_device, torch.device) else mesh_device
         self.args = args
         self.tt_ccl = tt_ccl
+        if activation_format is not None and activation_format not in ACTIVATION_FORMATS:
+            raise ValueError(f"activation format must be one of {ACTIVATION_FORMATS}, got {activation_format!r}")
         self.weights = load_mlp_weights(self.device, state_dict, tensor_cache_path, args, weight_format)
+        if activation_format is not None and self.weights.fmt != "mxfp4":
+            raise ValueError(f"an activation format belongs to mxfp4 weights, got {self.weights.fmt}")
+        self.activation_format = activation_format or ("mxfp4" if self.weights.fmt == "mxfp4" else None)
         self.max_tokens = int(max_tokens)
         self.pool = workspace_pool if pool is None else pool
         nbytes = self._workspace_bytes(self.max_tokens)
         self._ws_size = (self.max_tokens, nbytes)
+        if self.activation_format == "mxint8":
+            return
         self.pool.reserve(nbytes, self.device)
         # torch.cuda.graph(g) without a stream captures on its own side stream: give it a workspace
         # too, so that the usual warm-up-then-capture pattern needs no stream argument
@@ -662,7 +674,12 @@ class Qwen36MLP:
             size = self._ws_size = (tokens, self._workspace_bytes(tokens))
         return self.pool.reserve(size[1], self.device)
 
-    def forward(self, x, residual=None, out=None, out_dtype=None):
+    def _needs_8_bits(self, adapters, plan):
+        if self.activation_format != "mxint8" and (adapters is not None or plan is not None):
+            raise ValueError('adapters need activation_format="mxint8"')
+
+    def forward(self, x, residual=None, out=None, out_dtype=None, adapters=None, plan=None):
+        self._needs_8_bits(adapters, plan)
         if not isinstance(x, torch.Tensor) or x.dtype != torch.bfloat16:
             raise ValueError("BF16 activation tensor required")
         if x.dim() < 1 or x.shape[-1] != self.weights.hidden:
@@ -688,18 +705,24 @@ class Qwen36MLP:
             if not out.is_contiguous():  # a reshape would write into a copy
                 raise ValueError("out must be contiguous")
             o2d = out.reshape(M, shape[-1])
-        y = mlp_forward(x2d, self.weights, residual=r2d, out=o2d, workspace=self._workspace_for(M),
-                        out_dtype=out_dtype)
+        if self.activation_format == "mxint8":
+            from .w4a8 import w4a8_mlp
+
+            y = w4a8_mlp(x2d, self.weights, residual=r2d, out=o2d, out_dtype=out_dtype, adapters=adapters, plan=plan)
+        else:
+            y = mlp_forward(x2d, self.weights, residual=r2d, out=o2d, workspace=self._workspace_for(M),
+                            out_dtype=out_dtype)
         if out is not None:
             return out
         return y if len(shape) == 2 else y.reshape(shape)
 
     __call__ = forward
 
-    def forward_rmsnorm(self, h, norm_weight, eps=1e-6, out=None, out_dtype=None):
+    def forward_rmsnorm(self, h, norm_weight, eps=1e-6, out=None, out_dtype=None, adapters=None, plan=None):
         """``h + self.forward(rmsnorm(h) * (1 + norm_weight))`` in one call: the decoder's
         ``ffn_norm`` -> MLP -> residual add (``layer.py:352-357``).  ``h`` ``[..., H]`` bf16;
         ``out`` may be ``h`` itself."""
+        self._needs_8_bits(adapters, plan)
         if not isinstance(h, torch.Tensor) or h.dtype != torch.bfloat16 or h.device.type != "cuda":
             raise ValueError("h must be a bf16 GPU tensor")
         if h.dim() < 1 or h.shape[-1] != self.weights.hidden:
@@ -716,8 +739,51 @@ class Qwen36MLP:
             if not out.is_contiguous():  # a reshape would write into a copy
                 raise ValueError("out must be contiguous")
             o2d = out.reshape(M, shape[-1])
-        y = mlp_forward_rmsnorm(h2d, norm_weight, self.weights, eps=eps, out=o2d, workspace=self._workspace_for(M),
-                                out_dtype=out_dtype)
+        if self.activation_format == "mxint8":
+            y = self._normed(h2d, None, norm_weight, eps, o2d, out_dtype, adapters, plan)
+        else:
+            y = mlp_forward_rmsnorm(h2d, norm_weight, self.weights, eps=eps, out=o2d, workspace=self._workspace_for(M),
+                                    out_dtype=out_dtype)
         if out is not None:
             return out
         return y if len(shape) == 2 else y.reshape(shape)
+
+    def _normed(self, x, residual, norm_weight, eps, out, out_dtype, adapters, plan):
+        """The block behind the norm of ``residual + x`` (``x`` without a residual), for 2-D tensors."""
+        from .w4a8 import add_rmsnorm, w4a8_mlp
+
+        if self.activation_format != "mxint8":
+            h, n = add_rmsnorm(x, residual, norm_weight, eps=eps, output="rows")
+            return mlp_forward(n, self.weights, residual=h, out=out, workspace=self._workspace_for(x.shape[0]),
+                               out_dtype=out_dtype)
+        rows = None
+        if adapters is None:
+            h, n = add_rmsnorm(x, residual, norm_weight, eps=eps)
+        else:
+            h, rows, n = add_rmsnorm(x, residual, norm_weight, eps=eps, output="both")
+        return w4a8_mlp(n, self.weights, residual=h, out=out, out_dtype=out_dtype, adapters=adapters, plan=plan, rows=rows)
+
+    def forward_add_rmsnorm(self, x, residual, norm_weight, eps=1e-6, out=None, out_dtype=None, adapters=None, plan=None):
+        """``h + self.forward(rmsnorm(h) * (1 + norm_weight))`` with ``h = residual + x``: the feed-forward half of a
+        decoder layer with the addition of the attention's output ``x`` in front (``layer.py:352-357``).  ``x`` and
+        ``residual`` ``[..., H]``, bf16 or fp32; ``h`` is rounded to the residual's dtype.  ``out`` (or ``out_dtype``)
+        bf16 or fp32; it may be the residual itself."""
+        self._needs_8_bits(adapters, plan)
+        for name, t in (("x", x), ("residual", residual)):
+            if not isinstance(t, torch.Tensor) or t.dtype not in (torch.bfloat16, torch.float32) or t.device.type != "cuda":
+                raise ValueError(f"{name} must be a bf16 or fp32 GPU tensor")
+        H = self.weights.hidden
+        if x.dim() < 1 or x.shape[-1] != H or x.numel() == 0:
+            raise ValueError(f"x must be non-empty and end in hidden size {H}, got {tuple(x.shape)}")
+        if residual.shape != x.shape:
+            raise ValueError("residual must have x's shape")
+        o2d = None
+        if out is not None:
+            if out.shape != x.shape:
+                raise ValueError("out must have x's shape")
+            if not out.is_contiguous():  # a reshape would write into a copy
+                raise ValueError("out must be contiguous")
+            o2d = out.reshape(-1, H)
+        y = self._normed(x.reshape(-1, H).contiguous(), residual.reshape(-1, H).contiguous(), norm_weight, eps, o2d,
+                         out_dtype, adapters, plan)
+        return out if out is not None else y.reshape(x.shape)

@@ -11,7 +11,9 @@ are rounded half to even, 128 steps to 127.  A block that holds an infinity or a
   the sum in one pass, ``n`` as an ``Mx8Tensor``, as bf16 rows, or both;
 * ``w4a8_linear(x, w, residual=...)``: ``out = x w^T (+ residual)``;
 * ``w4a8_swiglu(x, w1, w3)``: ``silu(x w1^T + gate_add) * (x w3^T + up_add)``, the gate/up pair of the block, as
-  rows or (``quantize=True``) as the ``Mx8Tensor`` that the down projection takes.
+  rows or (``quantize=True``) as the ``Mx8Tensor`` that the down projection takes;
+* ``w4a8_mlp(x, weights, ...)``: the block of the two, with the adapters of many requests beside its projections
+  (``Qwen36MLP(..., weight_format="mxfp4", activation_format="mxint8")`` calls it).
 
 ``x`` of the products is an ``Mx8Tensor`` or a bf16, fp16 or fp32 ``[M, K]`` tensor, which the call quantises;
 weights come from ``pack_weight(w, "mxfp4")`` or ``pack_canonical(codes, scales, "mxfp4")``.  Sizes: any M up
@@ -29,6 +31,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
+from .lora import lora_linear
 from .mlp import _check_device_tensor, _check_mxfp4_buffer, _check_mxint8_buffer, _mxint8_bytes, _same_device
 from .mxfp4 import _check_out, _check_rows, _check_weight
 
@@ -65,7 +68,7 @@ def quantize_mxint8(x, stream=None):
     M, K = x.shape
     device, nbytes = x.device, _mxint8_bytes(M, K)
     with _lib.on_device(device, stream):
-        buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        buf = x.new_empty(nbytes, dtype=torch.uint8)
         rc = _lib.lib().qmlp_mxint8_quantize(x.data_ptr(), x_type, stride, M, K, buf.data_ptr(), nbytes,
                                              _lib.device_stream(device, stream))
         _lib.check(rc, "quantize_mxint8")
@@ -75,12 +78,12 @@ def quantize_mxint8(x, stream=None):
 def _check_norm_rows(t, name):
     """(QMLP_X_* code, row stride) of a bf16 or fp32 ``[M, K]`` tensor with contiguous rows."""
     try:
-        x_type, stride = _check_rows(t)
+        rows = _check_rows(t)
     except ValueError as e:
         raise ValueError(f"{name}: {e}") from None
-    if x_type == _lib.X_F16:
+    if rows[0] == _lib.X_F16:
         raise ValueError(f"{name} must be bf16 or fp32, got {t.dtype}")
-    return x_type, stride
+    return rows
 
 
 def add_rmsnorm(x, residual, norm_weight, eps=1e-6, output="mxint8", out=None, stream=None):
@@ -100,13 +103,15 @@ def add_rmsnorm(x, residual, norm_weight, eps=1e-6, output="mxint8", out=None, s
     M, K = x.shape
     device = x.device
     _check_device_tensor(norm_weight, "norm_weight", torch.bfloat16)
-    if tuple(norm_weight.shape) != (K,):
+    if norm_weight.dim() != 1 or norm_weight.shape[0] != K:
         raise ValueError(f"norm_weight must have shape ({K},)")
-    r_type, r_stride, h_stride = x_type, 0, 0
+    rp = hp = n = buf = np = bp = None
+    r_type, r_stride, h_stride, nbytes = x_type, 0, 0, 0
     if residual is not None:
         r_type, r_stride = _check_norm_rows(residual, "residual")
         if residual.shape != x.shape:
             raise ValueError(f"residual must have shape ({M}, {K})")
+        rp = residual.data_ptr()
         if out is not None:
             h_type, h_stride = _check_norm_rows(out, "out")
             if h_type != r_type or out.shape != x.shape:
@@ -119,16 +124,18 @@ def add_rmsnorm(x, residual, norm_weight, eps=1e-6, output="mxint8", out=None, s
         if residual is not None:
             h = out
             if h is None:
-                h = torch.empty((M, K), dtype=residual.dtype, device=device)
-                h_stride = K
-        n = torch.empty((M, K), dtype=torch.bfloat16, device=device) if output != "mxint8" else None
-        nbytes = _mxint8_bytes(M, K) if output != "rows" else 0
-        buf = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        rc = _lib.lib().qmlp_add_rmsnorm(
-            x.data_ptr(), x_type, x_stride, None if residual is None else residual.data_ptr(), r_type, r_stride,
-            norm_weight.data_ptr(), float(eps), M, K, None if residual is None else h.data_ptr(), h_stride,
-            None if n is None else n.data_ptr(), None if buf is None else buf.data_ptr(), nbytes,
-            _lib.device_stream(device, stream))
+                h, h_stride = residual.new_empty((M, K)), K
+            hp = h.data_ptr()
+        if output != "mxint8":
+            n = x.new_empty((M, K), dtype=torch.bfloat16)
+            np = n.data_ptr()
+        if output != "rows":
+            nbytes = _mxint8_bytes(M, K)
+            buf = x.new_empty(nbytes, dtype=torch.uint8)
+            bp = buf.data_ptr()
+        rc = _lib.lib().qmlp_add_rmsnorm(x.data_ptr(), x_type, x_stride, rp, r_type, r_stride, norm_weight.data_ptr(),
+                                         float(eps), M, K, hp, h_stride, np, bp, nbytes,
+                                         _lib.device_stream(device, stream))
         _lib.check(rc, "add_rmsnorm")
     if output == "rows":
         return h, n
@@ -238,3 +245,44 @@ def w4a8_swiglu(x, w1, w3, gate_add=None, up_add=None, out=None, out_dtype=None,
                                          flags, _lib.device_stream(device, stream))
         _lib.check(rc, "w4a8_swiglu")
     return res
+
+
+def w4a8_mlp(x, weights, residual=None, out=None, out_dtype=None, adapters=None, plan=None, rows=None, stream=None):
+    """``out = residual + down(silu(gate(x)) * up(x))`` with 8-bit activations and mxfp4 ``MLPWeights``.
+
+    ``x`` as in ``w4a8_linear``, ``residual`` / ``out`` / ``out_dtype`` as its.  ``adapters`` (``MLPAdapters``) and the
+    batch's ``plan``: low-rank adapters beside the projections; those of gate and up read ``x`` as rows (``rows`` where
+    ``x`` is an ``Mx8Tensor``), those of down the bf16 rows between the projections, which then are what the down
+    projection quantises.
+    """
+    if weights.fmt != "mxfp4":
+        raise ValueError(f"8-bit activations need mxfp4 weights, got {weights.fmt}")
+    gate_add = up_add = None
+    w2 = None
+    if adapters is not None:
+        if plan is None:
+            raise ValueError("adapters need the batch's plan (lora_plan)")
+        if rows is None and not isinstance(x, Mx8Tensor):
+            rows = x
+        for name, stack, n, k in (("w1", adapters.w1, weights.intermediate, weights.hidden),
+                                  ("w3", adapters.w3, weights.intermediate, weights.hidden),
+                                  ("w2", adapters.w2, weights.hidden, weights.intermediate)):
+            if stack is not None and (stack.n, stack.k) != (n, k):
+                raise ValueError(f"adapters.{name} is for [{stack.n}, {stack.k}], the projection is [{n}, {k}]")
+        if rows is None and (adapters.w1 is not None or adapters.w3 is not None):
+            raise ValueError("rows must hold the block's input where x is an Mx8Tensor")
+        if adapters.w1 is not None:
+            gate_add = lora_linear(rows, adapters.w1, plan, out_dtype=torch.float32, stream=stream)
+        if adapters.w3 is not None:
+            up_add = lora_linear(rows, adapters.w3, plan, out_dtype=torch.float32, stream=stream)
+        w2 = adapters.w2
+    elif plan is not None or rows is not None:
+        raise ValueError("plan and rows belong to adapters")
+    if residual is not None and tuple(residual.shape) != (x.shape[0], weights.hidden):
+        raise ValueError(f"residual must have shape ({x.shape[0]}, {weights.hidden})")
+    if w2 is None:
+        h = w4a8_swiglu(x, weights.w1, weights.w3, gate_add, up_add, quantize=True, stream=stream)
+    else:
+        h = w4a8_swiglu(x, weights.w1, weights.w3, gate_add, up_add, stream=stream)
+        residual = lora_linear(h, w2, plan, base=residual, out_dtype=torch.float32, stream=stream)
+    return w4a8_linear(h, weights.w2, residual=residual, out=out, out_dtype=out_dtype, stream=stream)
