@@ -127,8 +127,8 @@ __global__ __launch_bounds__(kDownWaves<TU> * 64, 1) void lora_down_kernel(LoraA
     row_in[i] = row < t.rows;
     x[i] = p.x + (size_t)order[min(row, t.rows - 1)] * p.x_bytes + (lane & 7) * 16;
   }
-  const int rank = meta[0], steps = p.K / 32, pieces = gridDim.x;
-  const int ru = min((rank + 15) / 16, RU), tu = (t.rows + 15) / 16;
+  const int rank = min(meta[0], ranks), steps = p.K / 32, pieces = gridDim.x;
+  const int ru = min((rank + 15) / 16, ranks / 16), tu = (t.rows + 15) / 16;
   const int s0 = blockIdx.x * steps / pieces, s1 = (blockIdx.x + 1) * steps / pieces;
   const uint8_t* a = p.stack.a + ((size_t)meta[1] * steps * 64 + lane) * 16;
   bool mine[RU];  // ranks that the adapter has
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(kUpThreads) void lora_up_kernel(LoraArgs p, int max
         for (int r = tid % 16; r < row4; r += 16) {
           const f32x4 v = s_sum[row * row4 + r];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(v[i]));
+          for (int i = 0; i < 4; ++i) m = r * 4 + i < rank ? fmaxf(m, fabsf(v[i])) : m;
         }
 #pragma unroll
       for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
@@ -348,6 +348,9 @@ __global__ __launch_bounds__(kUpThreads) void lora_up_kernel(LoraArgs p, int max
         v[0] = s_sum[row * row4 + 2 * r8];
         v[1] = s_sum[row * row4 + 2 * r8 + 1];
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)  // ranks behind the adapter's: not a number where x is not finite
+        if (r8 * 8 + i >= rank) v[i / 4][i % 4] = 0.f;
       float inv = 1.f;
       if constexpr (F16) inv = 1.0f / s_scale[row];  // a power of two: exact
       u32x4 part[3];

@@ -300,3 +300,39 @@ def test_widest_scales(pkg, cuda):
     y = _np(pkg.w4a8_linear(t, w, out_dtype=torch.float32))
     tiny = 2.0 ** -126  # below it a result may be flushed
     assert (np.abs(y - ref) <= _sum_error(64, mag) + tiny).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_products_of_strided_rows(pkg, cuda, dtype):
+    """Rows apart in memory, quantised by the product and in front of it."""
+    for M in (1, 2, 4, 16, 40):
+        wide = _rows(M, 544, dtype, M).to(cuda)
+        x = wide[:, :320]
+        w, _ = _weight(pkg, 256, 320, 6, cuda)
+        assert M == 1 or not x.is_contiguous()
+        assert torch.equal(pkg.w4a8_linear(x, w), pkg.w4a8_linear(x.contiguous(), w))
+        assert torch.equal(pkg.w4a8_swiglu(x, w, w), pkg.w4a8_swiglu(pkg.quantize_mxint8(x), w, w))
+
+
+def test_offsets_beyond_32_bits(pkg, cuda):
+    """A packed matrix of more than 2^32 bytes, its rows more than 2^32 bytes from the first: the last rows and columns,
+    against the same rows by themselves."""
+    rows, cols = 65536, 81920
+    g = torch.Generator(device=cuda).manual_seed(2)
+    x = torch.randn(rows, cols, generator=g, device=cuda, dtype=torch.bfloat16)
+    t, last = pkg.quantize_mxint8(x), x[-96:]
+    few = pkg.quantize_mxint8(last)
+    assert t.nbytes > 1 << 32 and torch.equal(t.buf[-few.nbytes:], few.buf)
+    n = torch.randn(cols, generator=g, device=cuda, dtype=torch.bfloat16)
+    h, q = pkg.add_rmsnorm(x, x, n)
+    h2, q2 = pkg.add_rmsnorm(last, last, n)
+    assert torch.equal(h[-96:], h2) and torch.equal(q.buf[-few.nbytes:], q2.buf)
+    del h, q
+    codes = torch.randint(0, 256, (40, cols // 2), generator=g, device=cuda, dtype=torch.uint8)
+    w = pkg.pack_canonical(codes, torch.full((40, cols // 32), 120, dtype=torch.uint8, device=cuda), "mxfp4")
+    y = pkg.w4a8_linear(t, w, out_dtype=torch.float32)
+    xd = pkg.dequantize(few).double()
+    ref = (xd @ pkg.dequantize(w).double().T).cpu().numpy()
+    mag = (xd.abs() @ pkg.dequantize(w).double().abs().T).cpu().numpy()
+    assert (np.abs(_np(y[-96:]) - ref) <= _sum_error(cols, mag)).all()
+    assert torch.equal(pkg.dequantize(t, dtype=torch.bfloat16)[-96:], pkg.dequantize(few, dtype=torch.bfloat16))
