@@ -1,12 +1,13 @@
 // qmlp_lora.hip -- low-rank adapters of many requests at once (layouts: qmlp_lora.h).
 //
-// Two launches: lora_down_kernel makes t = A_a x of every token, lora_up_kernel adds s_a B_a t to the base.
-// Both go by tiles of tokens that share an adapter, so that an adapter is read once a tile.
+// Two launches: lora_down_kernel makes t = A_a x of every token, lora_up_kernel adds s_a B_a t to the base; or one,
+// where A and a few tokens' rows are little to read again.  Both go by tiles of tokens that share an adapter.
 #include <algorithm>
 #include <atomic>
 
 #include "qmlp_lora.h"
 #include "qmlp_mx.h"
+#include "qmlp_xcd.h"
 
 namespace qmlp {
 
@@ -105,20 +106,18 @@ __device__ __forceinline__ f32x4 lora_product(u32x4 a, u32x4 b, f32x4 c) {
 // whole lines, 8 lanes to a row, and turn through LDS into operands: read as the operands lie, one row a lane,
 // every lane of a load is an access of its own, and those bounded the kernel (27000 of a CU for 2048 x 17408).
 // TU: units of 16 tokens of a tile; RU: rank units at most.
-template <int TU>
-constexpr int kDownWaves = TU == 1 ? 16 : 8;
 template <int TU, int RU>
-constexpr size_t kDownLds = kDownWaves<TU> * TU * (RU > 4 ? RU * 512 : 2048);  // turning, then the waves' sums
+constexpr int kDownWaves = TU == 1 && RU <= 4 ? 16 : 8;  // 128 ranks take the registers of two waves
+template <int TU, int RU>
+constexpr size_t kDownLds = kDownWaves<TU, RU> * TU * (RU > 4 ? RU * 512 : 2048);  // turning, then the waves' sums
 
+// The sums of K-steps s0..s1 of one tile, in wave 0 of kDownWaves: lane: token lane % 16 of a unit, ranks 16 r + 4
+// (lane / 16)..
 template <bool F16, int TU, int RU>
-__global__ __launch_bounds__(kDownWaves<TU> * 64, 1) void lora_down_kernel(LoraArgs p, int max_tiles, int ranks) {
-  constexpr int kWaves = kDownWaves<TU>, kLoads = 2 * TU;
-  extern __shared__ __align__(16) uint8_t s_mem[];
-  const LoraTile t = lora_tile_of(p.plan, blockIdx.y, p.M, p.adapters);
-  if (t.adapter < 0 || t.rows == 0) return;
+__device__ __forceinline__ void lora_down_tile(const LoraArgs& p, const LoraTile& t, const int* order, int rank, int first,
+                                               int s0, int s1, uint8_t* s_mem, f32x4 (&acc)[TU][RU]) {
+  constexpr int kWaves = kDownWaves<TU, RU>, kLoads = 2 * TU;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int* meta = p.stack.meta + 4 * t.adapter;
-  const int* order = p.plan + 4 + 4 * max_tiles + t.first;
   const uint8_t* x[kLoads];  // load i: rows 8 i + lane / 8, 16 bytes at 16 (lane % 8) of the two steps' line
   bool row_in[kLoads];
 #pragma unroll
@@ -127,10 +126,8 @@ __global__ __launch_bounds__(kDownWaves<TU> * 64, 1) void lora_down_kernel(LoraA
     row_in[i] = row < t.rows;
     x[i] = p.x + (size_t)order[min(row, t.rows - 1)] * p.x_bytes + (lane & 7) * 16;
   }
-  const int rank = min(meta[0], ranks), steps = p.K / 32, pieces = gridDim.x;
-  const int ru = min((rank + 15) / 16, ranks / 16), tu = (t.rows + 15) / 16;
-  const int s0 = blockIdx.x * steps / pieces, s1 = (blockIdx.x + 1) * steps / pieces;
-  const uint8_t* a = p.stack.a + ((size_t)meta[1] * steps * 64 + lane) * 16;
+  const int steps = p.K / 32, ru = (rank + 15) / 16, tu = (t.rows + 15) / 16;
+  const uint8_t* a = p.stack.a + ((size_t)first * steps * 64 + lane) * 16;
   bool mine[RU];  // ranks that the adapter has
 #pragma unroll
   for (int r = 0; r < RU; ++r) mine[r] = r * 16 + (lane & 15) < rank;
@@ -147,7 +144,6 @@ __global__ __launch_bounds__(kDownWaves<TU> * 64, 1) void lora_down_kernel(LoraA
         av[d][r] = mine[r] && (d == 0 || second) ? *(const u32x4*)(a + ((size_t)r * steps + s + d) * 1024)
                                                  : u32x4{0u, 0u, 0u, 0u};
   };
-  f32x4 acc[TU][RU];
 #pragma unroll
   for (int u = 0; u < TU; ++u)
 #pragma unroll
@@ -205,8 +201,20 @@ __global__ __launch_bounds__(kDownWaves<TU> * 64, 1) void lora_down_kernel(LoraA
     }
     __syncthreads();
   }
-  if (wave != 0) return;
-  // lane: token lane % 16 of a unit, ranks 16 r + 4 (lane / 16)..
+}
+
+template <bool F16, int TU, int RU>
+__global__ __launch_bounds__((kDownWaves<TU, RU> * 64), 1) void lora_down_kernel(LoraArgs p, int max_tiles, int ranks) {
+  extern __shared__ __align__(16) uint8_t s_mem[];
+  const LoraTile t = lora_tile_of(p.plan, blockIdx.y, p.M, p.adapters);
+  if (t.adapter < 0 || t.rows == 0) return;
+  const int* meta = p.stack.meta + 4 * t.adapter;
+  const int rank = min(meta[0], ranks), steps = p.K / 32, pieces = gridDim.x;
+  f32x4 acc[TU][RU];
+  lora_down_tile<F16, TU, RU>(p, t, p.plan + 4 + 4 * max_tiles + t.first, rank, meta[1], blockIdx.x * steps / pieces,
+                              (blockIdx.x + 1) * steps / pieces, s_mem, acc);
+  const int lane = threadIdx.x;
+  if (lane >= 64) return;
 #pragma unroll
   for (int u = 0; u < TU; ++u) {
     const int row = u * 16 + (lane & 15);
@@ -214,7 +222,7 @@ __global__ __launch_bounds__(kDownWaves<TU> * 64, 1) void lora_down_kernel(LoraA
     float* o = p.parts + ((size_t)blockIdx.x * p.M + t.first + row) * ranks + 4 * (lane >> 4);
 #pragma unroll
     for (int r = 0; r < RU; ++r)
-      if (r < ru) *(f32x4*)(o + 16 * r) = acc[u][r];
+      if (r * 16 < rank) *(f32x4*)(o + 16 * r) = acc[u][r];
   }
 }
 
@@ -224,8 +232,20 @@ __global__ __launch_bounds__(kDownWaves<TU> * 64, 1) void lora_down_kernel(LoraA
 // them and splits each fp32 sum into three 16-bit numbers whose sum it is but for 2^-24 of it (bf16), or of the
 // token's largest (fp16: over a power of two that brings the largest near the type's), so the products keep
 // fp32's accuracy; they are laid out in LDS as the products' operands, 32 ranks' parts of one order each.
-constexpr int kUpWaves = 8, kUpThreads = kUpWaves * 64;
+// DOWN: rank units that a workgroup (of up to 16 waves) makes t of by itself, 0 where lora_down_kernel did: one launch
+// instead of two where that reads little.
 constexpr int kUpParts = 3 * 1024;  // bytes of 32 ranks of 16 tokens
+template <int DOWN>
+constexpr int kUpWaves = DOWN ? kDownWaves<1, DOWN> : 8;
+constexpr int kTurnRow = 68;  // floats of a token's row in LDS
+// LDS: what makes t (DOWN), later the rows that turn; then the operands; then t in fp32.
+template <int DOWN>
+constexpr size_t kUpWork = kUpWaves<DOWN> * 16 * kTurnRow * 4;
+template <int DOWN>
+constexpr size_t lora_up_lds(int units) {
+  return kUpWork<DOWN> + (size_t)(units + 1) / 2 * kUpParts + (size_t)units * 1024;
+}
+static_assert(kUpWork<8> >= kDownLds<1, 8> && kUpWork<4> >= kDownLds<1, 4>);
 template <bool F16>
 __device__ __forceinline__ uint32_t lora_round(float v) {  // to the adapters' type
   if constexpr (F16) return f32_to_f16_bits(v);
@@ -248,35 +268,33 @@ __device__ __forceinline__ f32x4 lora_sum(const float* at, size_t piece, int pie
   return v[0];
 }
 
-// What a lane finishes of a block of 16 tokens x 64 features.  Rows of a multiple of 8 features (WHOLE): 8
+// A block of 16 tokens x 64 features is finished by rows.  Rows of a multiple of 8 features (WHOLE): a lane takes 8
 // neighbouring features of tokens lane / 8 and 8 more, so that 8 lanes touch 64 features of a token together.
 // Others, which start anywhere: feature `lane` of all 16 tokens.
-template <int T, bool WHOLE>  // T: 0 nothing, 1 bf16, 2 fp32
-struct LoraRows {
-  u32x4 w[T == 0 ? 1 : !WHOLE ? 4 : T == 2 ? 4 : 2];
-};
-
-constexpr int kTurnRow = 68;  // floats of a token's row in LDS
-template <bool F16, int BASE, bool OUT32, bool WHOLE>
-__global__ __launch_bounds__(kUpThreads) void lora_up_kernel(LoraArgs p, int max_tiles, int ranks, int pieces,
-                                                            int blocks_each, int tile_units) {
-  extern __shared__ __align__(16) uint8_t s_t[];  // [32 ranks][3 parts][lane][8] 16-bit numbers, then t in fp32
-  __shared__ __align__(16) float s_turn[kUpWaves][16 * kTurnRow];
-  __shared__ float s_scale[16];  // fp16: what a token's sums are multiplied by
-  const int unit = blockIdx.x % tile_units * 16;
-  LoraTile t = lora_tile_of(p.plan, blockIdx.x / tile_units, p.M, p.adapters);
+template <bool F16, bool WHOLE, int DOWN>
+__global__ __launch_bounds__(kUpWaves<DOWN> * 64) void lora_up_kernel(LoraArgs p, int max_tiles, int ranks, int pieces,
+                                                                     int runs, int blocks_each, int tile_units) {
+  constexpr int kWaves = kUpWaves<DOWN>, kThreads = kWaves * 64;
+  extern __shared__ __align__(16) uint8_t s_work[];
+  uint8_t* s_t = s_work + kUpWork<DOWN>;  // [32 ranks][3 parts][lane][8] 16-bit numbers, then t in fp32
+  __shared__ float s_scale[16];           // fp16: what a token's sums are multiplied by
+  // a tile's runs follow each other on one XCD, whose L2 keeps what they share
+  const int place = xcd_run(blockIdx.x, gridDim.x), run = place % runs, tile = place / runs;
+  const int unit = tile % tile_units * 16;
+  LoraTile t = lora_tile_of(p.plan, tile / tile_units, p.M, p.adapters);
   t.first += unit;
   t.rows = min(16, t.rows - unit);
   if (t.rows <= 0 || (t.adapter < 0 && p.base == p.out)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int blocks = (p.N + 63) / 64;
-  const int b0 = blockIdx.y * blocks_each, b1 = min(blocks, b0 + blocks_each);
+  const int b0 = run * blocks_each, b1 = min(blocks, b0 + blocks_each);
   const int* order = p.plan + 4 + 4 * max_tiles + t.first;
-  int rank = 0, first = 0;
+  int rank = 0, first = 0, first_a = 0;
   float s = 0.f;
   if (t.adapter >= 0) {
     const int* meta = p.stack.meta + 4 * t.adapter;
     rank = min(meta[0], ranks);
+    first_a = meta[1];
     s = __int_as_float(meta[2]);
     first = meta[3];
   }
@@ -293,27 +311,27 @@ __global__ __launch_bounds__(kUpThreads) void lora_up_kernel(LoraArgs p, int max
   // where this lane finishes: WHOLE: rows lane / 8 and 8 behind, features 8 (lane % 8)..
   const int half = WHOLE ? lane >> 3 : 0, n0 = WHOLE ? (lane & 7) * 8 : lane;
   const size_t at0 = (size_t)order[min(half, t.rows - 1)] * p.N, at1 = (size_t)order[min(WHOLE ? half + 8 : 0, t.rows - 1)] * p.N;
-  LoraRows<BASE, WHOLE> base;
+  u32x4 base[4];
   auto load_base = [&](int b) {
     const int n = b * 64 + n0;
-    if (n >= p.N) return;
+    if (n >= p.N || !p.base) return;
     if constexpr (WHOLE) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const size_t at = (i ? at1 : at0) + n;
-        if constexpr (BASE == 1) {
-          base.w[i] = *(const u32x4*)((const uint16_t*)p.base + at);
-        } else if constexpr (BASE == 2) {
-          base.w[2 * i] = *(const u32x4*)((const float*)p.base + at);
-          base.w[2 * i + 1] = *(const u32x4*)((const float*)p.base + at + 4);
+        if (p.base_f32) {
+          base[2 * i] = *(const u32x4*)((const float*)p.base + at);
+          base[2 * i + 1] = *(const u32x4*)((const float*)p.base + at + 4);
+        } else {
+          base[2 * i] = *(const u32x4*)((const uint16_t*)p.base + at);
         }
       }
-    } else if constexpr (BASE != 0) {
+    } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {  // tokens behind the last one read it again
         const size_t at = (size_t)order[min(i, t.rows - 1)] * p.N + n;
-        base.w[i / 4][i % 4] =
-            BASE == 1 ? (uint32_t)((const uint16_t*)p.base)[at] << 16 : ((const uint32_t*)p.base)[at];
+        base[i / 4][i % 4] =
+            p.base_f32 ? ((const uint32_t*)p.base)[at] : (uint32_t)((const uint16_t*)p.base)[at] << 16;
       }
     }
   };
@@ -322,9 +340,19 @@ __global__ __launch_bounds__(kUpThreads) void lora_up_kernel(LoraArgs p, int max
   if (ru) {
     const int row4 = (rank + 15) / 16 * 4;  // four ranks each
     f32x4* s_sum = (f32x4*)(s_t + (size_t)ru * kUpParts);
-    const float* at = p.parts + (size_t)t.first * ranks;
-    for (int e = tid; e < t.rows * row4; e += kUpThreads)
-      s_sum[e] = lora_sum(at + (size_t)(e / row4) * ranks + e % row4 * 4, (size_t)p.M * ranks, pieces) * s;
+    if constexpr (DOWN) {
+      f32x4 acc[1][DOWN];
+      lora_down_tile<F16, 1, DOWN>(p, t, order, rank, first_a, 0, p.K / 32, s_work, acc);
+      if (wave == 0 && (lane & 15) < t.rows) {
+#pragma unroll
+        for (int r = 0; r < DOWN; ++r)
+          if (r * 16 < rank) s_sum[(lane & 15) * row4 + 4 * r + (lane >> 4)] = acc[0][r] * s;
+      }
+    } else {
+      const float* at = p.parts + (size_t)t.first * ranks;
+      for (int e = tid; e < t.rows * row4; e += kThreads)
+        s_sum[e] = lora_sum(at + (size_t)(e / row4) * ranks + e % row4 * 4, (size_t)p.M * ranks, pieces) * s;
+    }
     __syncthreads();
     if constexpr (F16) if (tid < 256) {
       const int row = tid / 16;
@@ -341,7 +369,7 @@ __global__ __launch_bounds__(kUpThreads) void lora_up_kernel(LoraArgs p, int max
       s_scale[row] = __uint_as_float((uint32_t)(min(max(e, 16), 254) - 14) << 23);
     }
     if constexpr (F16) __syncthreads();
-    for (int item = tid; item < 16 * ru * 4; item += kUpThreads) {
+    for (int item = tid; item < 16 * ru * 4; item += kThreads) {
       const int row = item / (4 * ru), r8 = item % (4 * ru);
       f32x4 v[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
       if (row < t.rows && 2 * r8 < row4) {
@@ -370,8 +398,8 @@ __global__ __launch_bounds__(kUpThreads) void lora_up_kernel(LoraArgs p, int max
     }
   }
   __syncthreads();
-  float* turn = s_turn[wave];
-  for (int b = b0 + wave; b < b1; b += kUpWaves) {
+  float* turn = (float*)s_work + wave * 16 * kTurnRow;
+  for (int b = b0 + wave; b < b1; b += kWaves) {
     f32x4 acc[4];
 #pragma unroll
     for (int f = 0; f < 4; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -381,8 +409,8 @@ __global__ __launch_bounds__(kUpThreads) void lora_up_kernel(LoraArgs p, int max
       for (int f = 0; f < 4; ++f) v[f] = w[f];
       if (r + 1 < ru)
         load_w(b, r + 1);
-      else if (b + kUpWaves < b1)
-        load_w(b + kUpWaves, 0);
+      else if (b + kWaves < b1)
+        load_w(b + kWaves, 0);
       const uint8_t* at = s_t + (size_t)r * kUpParts + lane * 16;
 #pragma unroll
       for (int k = 2; k >= 0; --k) {  // the smallest parts first
@@ -409,18 +437,22 @@ __global__ __launch_bounds__(kUpThreads) void lora_up_kernel(LoraArgs p, int max
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           y[i][j] = j < 4 ? lo[j] : hi[j - 4];
-          if constexpr (BASE == 1)
-            y[i][j] += __uint_as_float(j % 2 ? base.w[i][j / 2] & 0xffff0000u : base.w[i][j / 2] << 16);
-          else if constexpr (BASE == 2)
-            y[i][j] += __uint_as_float(base.w[2 * i + j / 4][j % 4]);
+        }
+        if (p.base && p.base_f32) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[i][j] += __uint_as_float(base[2 * i + j / 4][j % 4]);
+        } else if (p.base) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            y[i][j] += __uint_as_float(j % 2 ? base[2 * i][j / 2] & 0xffff0000u : base[2 * i][j / 2] << 16);
         }
       }
-      if (b + kUpWaves < b1) load_base(b + kUpWaves);
+      if (b + kWaves < b1) load_base(b + kWaves);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (half + 8 * i >= t.rows || n >= p.N) continue;
         const size_t at = (i ? at1 : at0) + n;
-        if constexpr (OUT32) {
+        if (p.out_f32) {
           *(f32x4*)((float*)p.out + at) = f32x4{y[i][0], y[i][1], y[i][2], y[i][3]};
           *(f32x4*)((float*)p.out + at + 4) = f32x4{y[i][4], y[i][5], y[i][6], y[i][7]};
         } else {
@@ -436,14 +468,14 @@ __global__ __launch_bounds__(kUpThreads) void lora_up_kernel(LoraArgs p, int max
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         y[i] = turn[i * kTurnRow + n0];
-        if constexpr (BASE != 0) y[i] += __uint_as_float(base.w[i / 4][i % 4]);
+        if (p.base) y[i] += __uint_as_float(base[i / 4][i % 4]);
       }
-      if (b + kUpWaves < b1) load_base(b + kUpWaves);
+      if (b + kWaves < b1) load_base(b + kWaves);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         if (i >= t.rows || n >= p.N) continue;
         const size_t at = (size_t)order[min(i, t.rows - 1)] * p.N + n;
-        if constexpr (OUT32)
+        if (p.out_f32)
           ((float*)p.out)[at] = y[i];
         else
           ((uint16_t*)p.out)[at] = (uint16_t)mx_bf16x2(y[i], 0.f);
@@ -462,7 +494,7 @@ static int up_div(int a, int b) { return (a + b - 1) / b; }
 // of whose workgroups adds them up.
 template <int TU>
 static int pieces_of(int K) {
-  return std::min(kLoraMaxPieces, up_div(K / 32, 2 * kDownWaves<TU>));
+  return std::min(kLoraMaxPieces, up_div(K / 32, 2 * kDownWaves<TU, 1>));
 }
 int lora_pieces(int M, int K) { return lora_tile(M) == 16 ? pieces_of<1>(K) : pieces_of<2>(K); }
 
@@ -480,47 +512,60 @@ static int launch_down(const LoraArgs& a, int max_tiles, int pieces, hipStream_t
     static std::atomic<uint64_t> raised{0};
     if (int rc = raise_lds_once((const void*)kern, (int)lds, raised)) return rc;
   }
-  hipLaunchKernelGGL(kern, dim3(pieces, max_tiles), dim3(kDownWaves<TU> * 64), lds, s, a, max_tiles,
+  hipLaunchKernelGGL(kern, dim3(pieces, max_tiles), dim3(kDownWaves<TU, RU> * 64), lds, s, a, max_tiles,
                      padded_rank(a.max_rank));
   return check_launch("lora_down_kernel");
 }
 
-template <bool F16, int BASE, bool OUT32, bool WHOLE>
+template <bool F16, bool WHOLE, int DOWN>
 static int launch_up(const LoraArgs& a, int max_tiles, int pieces, int num_cus, hipStream_t s) {
   const int blocks = up_div(a.N, 64), tile_units = lora_tile(a.M) / 16;
   const int tiles = std::max(1, std::min(max_tiles * tile_units / 2, up_div(a.M, 16)));
   // about a workgroup a CU, as far as each wave has a block: 44.1 us at 2048 tokens of 17408 -> 5120 and rank 64,
   // 48.9 with two (each adds the pieces up again), 48.4 and 45.8 in workgroups of four waves
-  const int runs = std::max(1, std::min(up_div(blocks, kUpWaves), up_div(num_cus, tiles)));
-  const int each = up_div(blocks, runs), units = padded_rank(a.max_rank) / 16;
-  hipLaunchKernelGGL((lora_up_kernel<F16, BASE, OUT32, WHOLE>), dim3(max_tiles * tile_units, up_div(blocks, each)),
-                     dim3(kUpThreads), (size_t)(units + 1) / 2 * kUpParts + (size_t)units * 1024, s, a, max_tiles,
-                     units * 16, pieces, each, tile_units);
+  const int most = std::max(1, DOWN ? std::min(up_div(blocks, 4), num_cus / max_tiles)
+                                    : std::min(up_div(blocks, kUpWaves<0>), up_div(num_cus, tiles)));
+  const int each = up_div(blocks, most), runs = up_div(blocks, each), units = padded_rank(a.max_rank) / 16;
+  auto kern = lora_up_kernel<F16, WHOLE, DOWN>;
+  if constexpr (lora_up_lds<DOWN>(kLoraMaxRank / 16) > 65536 - 64) {
+    static std::atomic<uint64_t> raised{0};
+    if (int rc = raise_lds_once((const void*)kern, (int)lora_up_lds<DOWN>(kLoraMaxRank / 16), raised)) return rc;
+  }
+  hipLaunchKernelGGL(kern, dim3(max_tiles * tile_units * runs), dim3(kUpWaves<DOWN> * 64), lora_up_lds<DOWN>(units), s, a,
+                     max_tiles, units * 16, pieces, runs, each, tile_units);
   return check_launch("lora_up_kernel");
 }
-template <bool F16, int BASE, bool OUT32>
+template <bool F16, int DOWN>
 static int launch_up_rows(const LoraArgs& a, int max_tiles, int pieces, int num_cus, hipStream_t s) {
-  return a.N % 8 ? launch_up<F16, BASE, OUT32, false>(a, max_tiles, pieces, num_cus, s)
-                 : launch_up<F16, BASE, OUT32, true>(a, max_tiles, pieces, num_cus, s);
+  return a.N % 8 ? launch_up<F16, false, DOWN>(a, max_tiles, pieces, num_cus, s)
+                 : launch_up<F16, true, DOWN>(a, max_tiles, pieces, num_cus, s);
+}
+
+// Whether t is made by every workgroup that uses it: where that reads at most half a megabyte of A and x, a third of
+// that beyond 32 ranks.  One launch / two, us in a graph (and with the host's time in a loop of calls): one token of
+// 5120 -> 5120 and rank 16, 174 KB: 7.3 / 8.1 (10.3 / 13.0); 16 tokens of 16 adapters of 5120 -> 17408 and rank 32, 492
+// KB: 12.4 / 13.9 (11.7 / 13.2), of one 10.1 / 9.0 (10.3 / 13.1); 2048 -> 2048 and rank 64, 266 KB: 10.7 / 10.0; one
+// token of 17408 -> 5120 and rank 16, 592 KB: 11.5 / 8.4 (11.0 / 13.1); rank 64 of 5120, 666 KB: 15.5 / 10.0.
+static bool lora_one_launch(const LoraArgs& a) {
+  const int ranks = padded_rank(a.max_rank);
+  return lora_tile(a.M) == 16 && (size_t)(ranks + std::min(a.M, 16)) * a.K * 2 <= (ranks <= 32 ? 500000 : 167000);
 }
 
 template <bool F16, int TU>
 static int launch_tokens(const LoraArgs& a, int num_cus, hipStream_t s) {
   const int max_tiles = lora_max_tiles(a.M, a.adapters), pieces = lora_pieces(a.M, a.K);
   const int units = padded_rank(a.max_rank) / 16;
+  if (TU == 1 && lora_one_launch(a))
+    return units <= 1   ? launch_up_rows<F16, 1>(a, max_tiles, pieces, num_cus, s)
+           : units <= 2 ? launch_up_rows<F16, 2>(a, max_tiles, pieces, num_cus, s)
+           : units <= 4 ? launch_up_rows<F16, 4>(a, max_tiles, pieces, num_cus, s)
+                        : launch_up_rows<F16, 8>(a, max_tiles, pieces, num_cus, s);
   const int rc = units <= 1   ? launch_down<F16, TU, 1>(a, max_tiles, pieces, s)
                  : units <= 2 ? launch_down<F16, TU, 2>(a, max_tiles, pieces, s)
                  : units <= 4 ? launch_down<F16, TU, 4>(a, max_tiles, pieces, s)
                               : launch_down<F16, TU, 8>(a, max_tiles, pieces, s);
   if (rc) return rc;
-  const int base = !a.base ? 0 : a.base_f32 ? 2 : 1;
-  if (a.out_f32)
-    return base == 0   ? launch_up_rows<F16, 0, true>(a, max_tiles, pieces, num_cus, s)
-           : base == 1 ? launch_up_rows<F16, 1, true>(a, max_tiles, pieces, num_cus, s)
-                       : launch_up_rows<F16, 2, true>(a, max_tiles, pieces, num_cus, s);
-  return base == 0   ? launch_up_rows<F16, 0, false>(a, max_tiles, pieces, num_cus, s)
-         : base == 1 ? launch_up_rows<F16, 1, false>(a, max_tiles, pieces, num_cus, s)
-                     : launch_up_rows<F16, 2, false>(a, max_tiles, pieces, num_cus, s);
+  return launch_up_rows<F16, 0>(a, max_tiles, pieces, num_cus, s);
 }
 
 int launch_lora(const LoraArgs& a, int num_cus, hipStream_t s) {
