@@ -7,7 +7,6 @@
 
 #include "qmlp_lora.h"
 #include "qmlp_mx.h"
-#include "qmlp_xcd.h"
 
 namespace qmlp {
 
@@ -270,17 +269,22 @@ __device__ __forceinline__ f32x4 lora_sum(const float* at, size_t piece, int pie
 
 // A block of 16 tokens x 64 features is finished by rows.  Rows of a multiple of 8 features (WHOLE): a lane takes 8
 // neighbouring features of tokens lane / 8 and 8 more, so that 8 lanes touch 64 features of a token together.
-// Others, which start anywhere: feature `lane` of all 16 tokens.
-template <bool F16, bool WHOLE, int DOWN>
+// Others, which start anywhere: feature `lane` of all 16 tokens.  BASE: 0 none, 1 bf16, 2 fp32.
+template <bool F16, bool WHOLE, int BASE, int DOWN>
 __global__ __launch_bounds__(kUpWaves<DOWN> * 64) void lora_up_kernel(LoraArgs p, int max_tiles, int ranks, int pieces,
                                                                      int runs, int blocks_each, int tile_units) {
   constexpr int kWaves = kUpWaves<DOWN>, kThreads = kWaves * 64;
   extern __shared__ __align__(16) uint8_t s_work[];
   uint8_t* s_t = s_work + kUpWork<DOWN>;  // [32 ranks][3 parts][lane][8] 16-bit numbers, then t in fp32
   __shared__ float s_scale[16];           // fp16: what a token's sums are multiplied by
-  // a tile's runs follow each other on one XCD, whose L2 keeps what they share
-  const int place = xcd_run(blockIdx.x, gridDim.x), run = place % runs, tile = place / runs;
+  // DOWN: a tile's runs share an XCD (block b runs on XCD b % 8), whose L2 keeps the A that they all read, where there
+  // are tiles for every XCD
+  const int b8 = blockIdx.x / 8, tiles = gridDim.x / runs;
+  const bool grouped = DOWN && tiles % 8 == 0;
+  const int run = !DOWN ? blockIdx.x / tiles : grouped ? b8 % runs : blockIdx.x % runs;
+  const int tile = !DOWN ? blockIdx.x % tiles : grouped ? b8 / runs * 8 + blockIdx.x % 8 : blockIdx.x / runs;
   const int unit = tile % tile_units * 16;
+  if (tile >= max_tiles * tile_units) return;
   LoraTile t = lora_tile_of(p.plan, tile / tile_units, p.M, p.adapters);
   t.first += unit;
   t.rows = min(16, t.rows - unit);
@@ -311,27 +315,23 @@ __global__ __launch_bounds__(kUpWaves<DOWN> * 64) void lora_up_kernel(LoraArgs p
   // where this lane finishes: WHOLE: rows lane / 8 and 8 behind, features 8 (lane % 8)..
   const int half = WHOLE ? lane >> 3 : 0, n0 = WHOLE ? (lane & 7) * 8 : lane;
   const size_t at0 = (size_t)order[min(half, t.rows - 1)] * p.N, at1 = (size_t)order[min(WHOLE ? half + 8 : 0, t.rows - 1)] * p.N;
-  u32x4 base[4];
+  u32x4 base[BASE == 1 && WHOLE ? 2 : 4];
   auto load_base = [&](int b) {
     const int n = b * 64 + n0;
-    if (n >= p.N || !p.base) return;
-    if constexpr (WHOLE) {
+    if (n >= p.N) return;
+    if constexpr (BASE == 1 && WHOLE) {
+      base[0] = *(const u32x4*)((const uint16_t*)p.base + at0 + n);
+      base[1] = *(const u32x4*)((const uint16_t*)p.base + at1 + n);
+    } else if constexpr (BASE == 2 && WHOLE) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const size_t at = (i ? at1 : at0) + n;
-        if (p.base_f32) {
-          base[2 * i] = *(const u32x4*)((const float*)p.base + at);
-          base[2 * i + 1] = *(const u32x4*)((const float*)p.base + at + 4);
-        } else {
-          base[2 * i] = *(const u32x4*)((const uint16_t*)p.base + at);
-        }
-      }
-    } else {
+      for (int i = 0; i < 4; ++i)
+        base[i] = *(const u32x4*)((const float*)p.base + (i < 2 ? at0 : at1) + n + i % 2 * 4);
+    } else if constexpr (BASE != 0) {  // tokens behind the last one read it again
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {  // tokens behind the last one read it again
+      for (int i = 0; i < 16; ++i) {
         const size_t at = (size_t)order[min(i, t.rows - 1)] * p.N + n;
         base[i / 4][i % 4] =
-            p.base_f32 ? ((const uint32_t*)p.base)[at] : (uint32_t)((const uint16_t*)p.base)[at] << 16;
+            BASE == 1 ? (uint32_t)((const uint16_t*)p.base)[at] << 16 : ((const uint32_t*)p.base)[at];
       }
     }
   };
@@ -438,13 +438,13 @@ __global__ __launch_bounds__(kUpWaves<DOWN> * 64) void lora_up_kernel(LoraArgs p
         for (int j = 0; j < 8; ++j) {
           y[i][j] = j < 4 ? lo[j] : hi[j - 4];
         }
-        if (p.base && p.base_f32) {
+        if constexpr (BASE == 2) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) y[i][j] += __uint_as_float(base[2 * i + j / 4][j % 4]);
-        } else if (p.base) {
+        } else if constexpr (BASE == 1) {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            y[i][j] += __uint_as_float(j % 2 ? base[2 * i][j / 2] & 0xffff0000u : base[2 * i][j / 2] << 16);
+            y[i][j] += __uint_as_float(j % 2 ? base[i][j / 2] & 0xffff0000u : base[i][j / 2] << 16);
         }
       }
       if (b + kWaves < b1) load_base(b + kWaves);
@@ -468,17 +468,17 @@ __global__ __launch_bounds__(kUpWaves<DOWN> * 64) void lora_up_kernel(LoraArgs p
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         y[i] = turn[i * kTurnRow + n0];
-        if (p.base) y[i] += __uint_as_float(base[i / 4][i % 4]);
+        if constexpr (BASE != 0) y[i] += __uint_as_float(base[i / 4][i % 4]);
       }
       if (b + kWaves < b1) load_base(b + kWaves);
+      if (p.out_f32) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if (i >= t.rows || n >= p.N) continue;
-        const size_t at = (size_t)order[min(i, t.rows - 1)] * p.N + n;
-        if (p.out_f32)
-          ((float*)p.out)[at] = y[i];
-        else
-          ((uint16_t*)p.out)[at] = (uint16_t)mx_bf16x2(y[i], 0.f);
+        for (int i = 0; i < 16; ++i)
+          if (i < t.rows && n < p.N) ((float*)p.out)[(size_t)order[i] * p.N + n] = y[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (i < t.rows && n < p.N) ((uint16_t*)p.out)[(size_t)order[i] * p.N + n] = (uint16_t)mx_bf16x2(y[i], 0.f);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -517,28 +517,35 @@ static int launch_down(const LoraArgs& a, int max_tiles, int pieces, hipStream_t
   return check_launch("lora_down_kernel");
 }
 
-template <bool F16, bool WHOLE, int DOWN>
+template <bool F16, bool WHOLE, int BASE, int DOWN>
 static int launch_up(const LoraArgs& a, int max_tiles, int pieces, int num_cus, hipStream_t s) {
   const int blocks = up_div(a.N, 64), tile_units = lora_tile(a.M) / 16;
   const int tiles = std::max(1, std::min(max_tiles * tile_units / 2, up_div(a.M, 16)));
   // about a workgroup a CU, as far as each wave has a block: 44.1 us at 2048 tokens of 17408 -> 5120 and rank 64,
   // 48.9 with two (each adds the pieces up again), 48.4 and 45.8 in workgroups of four waves
-  const int most = std::max(1, DOWN ? std::min(up_div(blocks, 4), num_cus / max_tiles)
+  const int slots = DOWN && max_tiles >= 8 ? up_div(max_tiles, 8) * 8 : max_tiles * tile_units;
+  const int most = std::max(1, DOWN ? std::min(up_div(blocks, 4), num_cus / slots)
                                     : std::min(up_div(blocks, kUpWaves<0>), up_div(num_cus, tiles)));
   const int each = up_div(blocks, most), runs = up_div(blocks, each), units = padded_rank(a.max_rank) / 16;
-  auto kern = lora_up_kernel<F16, WHOLE, DOWN>;
+  auto kern = lora_up_kernel<F16, WHOLE, BASE, DOWN>;
   if constexpr (lora_up_lds<DOWN>(kLoraMaxRank / 16) > 65536 - 64) {
     static std::atomic<uint64_t> raised{0};
     if (int rc = raise_lds_once((const void*)kern, (int)lora_up_lds<DOWN>(kLoraMaxRank / 16), raised)) return rc;
   }
-  hipLaunchKernelGGL(kern, dim3(max_tiles * tile_units * runs), dim3(kUpWaves<DOWN> * 64), lora_up_lds<DOWN>(units), s, a,
+  hipLaunchKernelGGL(kern, dim3(slots * runs), dim3(kUpWaves<DOWN> * 64), lora_up_lds<DOWN>(units), s, a,
                      max_tiles, units * 16, pieces, runs, each, tile_units);
   return check_launch("lora_up_kernel");
 }
+template <bool F16, bool WHOLE, int DOWN>
+static int launch_up_base(const LoraArgs& a, int max_tiles, int pieces, int num_cus, hipStream_t s) {
+  if (!a.base) return launch_up<F16, WHOLE, 0, DOWN>(a, max_tiles, pieces, num_cus, s);
+  if (!a.base_f32) return launch_up<F16, WHOLE, 1, DOWN>(a, max_tiles, pieces, num_cus, s);
+  return launch_up<F16, WHOLE, 2, DOWN>(a, max_tiles, pieces, num_cus, s);
+}
 template <bool F16, int DOWN>
 static int launch_up_rows(const LoraArgs& a, int max_tiles, int pieces, int num_cus, hipStream_t s) {
-  return a.N % 8 ? launch_up<F16, false, DOWN>(a, max_tiles, pieces, num_cus, s)
-                 : launch_up<F16, true, DOWN>(a, max_tiles, pieces, num_cus, s);
+  return a.N % 8 ? launch_up_base<F16, false, DOWN>(a, max_tiles, pieces, num_cus, s)
+                 : launch_up_base<F16, true, DOWN>(a, max_tiles, pieces, num_cus, s);
 }
 
 // Whether t is made by every workgroup that uses it: where that reads at most half a megabyte of A and x, a third of
