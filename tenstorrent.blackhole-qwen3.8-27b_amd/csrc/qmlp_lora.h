@@ -50,7 +50,7 @@ struct LoraArgs {
 };
 
 // The K range is cut into this many pieces, a workgroup each.
-int lora_pieces(int M, int K);
+int lora_pieces(int M, int K, int adapters, int num_cus);
 size_t lora_parts_bytes(int M, int K, int max_rank);
 int launch_lora_plan(const int* ids, int M, int adapters, int* plan, hipStream_t s);
 int launch_lora(const LoraArgs& a, int num_cus, hipStream_t s);
