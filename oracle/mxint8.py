@@ -35,8 +35,9 @@ def packed_bytes(rows, cols):
 
 
 def group_bytes(q, negative):
-    """16 integers and the signs of what they were rounded from (zeros keep theirs) -> 16 bytes: 96 bits of 6-bit fields (sign, a bit of another digit, the low digit), then the
-    two high bits of every high digit at their places modulo 32."""
+    """16 integers and the signs of what they were rounded from (zeros keep theirs) -> 16 bytes: 96 bits of 6-bit
+    fields (sign, a bit of another digit, the low digit), then the two high bits of every high digit at their places
+    modulo 32."""
     low = high = 0
     for i, v in enumerate(int(a) for a in q):
         low |= ((abs(v) & 15) | (32 if negative[i] else 0)) << 6 * i

@@ -92,6 +92,15 @@ def test_lora_linear(pkg, cuda, case, dtype):
     _check(pkg, cuda, ids, ranks, N, K, dtype, seed=case)
 
 
+@pytest.mark.parametrize("M,ranks,N,K", [(65536, [1 + 3 * i % 20 for i in range(1024)], 40, 64), (65536, [33], 9, 32),
+                                         (3, [4, 130 - 2], 1 << 20, 32), (2, [20], 5, 1 << 20), (65, [20, 7], 5, 1 << 20)])
+def test_largest_sizes(pkg, cuda, M, ranks, N, K):
+    """The most tokens with the most adapters and with one, the most features, the longest rows."""
+    print(f"case lora {M}x{N}x{K}, {len(ranks)} adapters", flush=True)
+    ids = torch.randint(-1, len(ranks) + 1, (M,), generator=torch.Generator().manual_seed(N)).tolist()
+    _check(pkg, cuda, ids, ranks, N, K, torch.bfloat16, seed=3)
+
+
 def test_strided_rows(pkg, cuda):
     for M in (3, 70):
         _check(pkg, cuda, [i % 2 for i in range(M)], [20, 7], 100, 96, torch.bfloat16, stride=96)

@@ -336,3 +336,55 @@ def test_offsets_beyond_32_bits(pkg, cuda):
     mag = (xd.abs() @ pkg.dequantize(w).double().abs().T).cpu().numpy()
     assert (np.abs(_np(y[-96:]) - ref) <= _sum_error(cols, mag)).all()
     assert torch.equal(pkg.dequantize(t, dtype=torch.bfloat16)[-96:], pkg.dequantize(few, dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("rows,cols", [(1 << 20, 32), (2, 1 << 20)])
+def test_largest_matrices(pkg, cuda, rows, cols):
+    """Quantised, read back and behind the norm, against the oracle on some of their rows."""
+    print(f"case largest {rows}x{cols}", flush=True)
+    base = _rows(min(rows, 96), cols, torch.bfloat16, 9)
+    x = base.to(cuda).repeat(-(-rows // 96), 1)[:rows].contiguous()
+    t = pkg.quantize_mxint8(x)
+    q, scales = pkg.unpack_canonical(t)
+    want, wants = omi.quantize(_np(base))
+    assert np.array_equal(q[:96].cpu().numpy(), want) and np.array_equal(scales[:96].cpu().numpy(), wants)
+    for at in (range(96, rows - 95, 96 * 1021) if rows > 96 else ()):
+        assert torch.equal(q[at:at + 96], q[:96]) and torch.equal(scales[at:at + 96], scales[:96])
+    assert torch.equal(q[-1], q[(rows - 1) % 96]) and torch.equal(scales[-1], scales[(rows - 1) % 96])
+    values = pkg.dequantize(t)
+    assert torch.equal(values, (q.float().view(rows, -1, 32) * torch.exp2(scales.float() - 133)[..., None]).view(rows, cols))
+    w = torch.zeros(cols, dtype=torch.bfloat16, device=cuda)
+    h, n, normed = pkg.add_rmsnorm(x, x, w, output="both")
+    few = pkg.add_rmsnorm(x[:96], x[:96], w, output="both")
+    assert torch.equal(h, 2 * x)
+    for a, b in ((n, few[1]), *zip(pkg.unpack_canonical(normed), pkg.unpack_canonical(few[2]))):
+        assert torch.equal(a[:96], b) and torch.equal(a[-1], b[(rows - 1) % 96])
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 1 << 20, 64), (9, 1 << 20, 64), (70, 1 << 20, 64), (1, 33, 1 << 20), (12, 33, 1 << 20),
+                                   (40, 33, 1 << 20), (300, 33, 1 << 20)])
+def test_products_at_the_largest_sizes(pkg, cuda, M, N, K):
+    """Every block's step is the same and so is every weight's scale, so every product is a whole number of half steps
+    of at most 127 * 12 units.  A random sum of 2^20 of them (a spread of 2^10 times 450 or so) stays below 2^22 units, a
+    digit's part of it too, so no sum rounds.  Behind it the silu's error as elsewhere."""
+    print(f"case largest product {M}x{N}x{K}", flush=True)
+    g = torch.Generator(device=cuda).manual_seed(N)
+    q = torch.randint(-127, 128, (M, K), generator=g, device=cuda).float()
+    q[:, ::32] = 127.0
+    x = q / 64
+    t = pkg.quantize_mxint8(x)
+    assert torch.equal(pkg.dequantize(t), x)
+    byte = 127 - (K.bit_length() - 1) // 2  # the sums have a spread of a few units
+
+    def weight():
+        codes = torch.randint(0, 256, (N, K // 2), generator=g, device=cuda, dtype=torch.uint8)
+        return pkg.pack_canonical(codes, torch.full((N, K // 32), byte, dtype=torch.uint8, device=cuda), "mxfp4")
+
+    w1, w3 = weight(), weight()
+    y1, y3 = (x.double() @ pkg.dequantize(w).double().T.contiguous() for w in (w1, w3))
+    for a in (x, t):
+        for w, y in ((w1, y1), (w3, y3)):
+            assert torch.equal(pkg.w4a8_linear(a, w, out_dtype=torch.float32).double(), y)
+    s = y1 / (1 + torch.exp(-y1)) * y3
+    got = pkg.w4a8_swiglu(t, w1, w3, out_dtype=torch.float32).double()
+    assert ((got - s).abs() <= (8 + y1.abs()) * 2.0 ** -23 * s.abs() + 1.1e-36 * y3.abs()).all()
