@@ -6,6 +6,9 @@
 // T is the residual stream's type: h is rounded once, and the norm is that of the stored h, as where the
 // steps are calls of their own; n is rounded to bf16 as the decoder's separate norm writes it, so that packed
 // is what a quantisation of those rows makes.
+//
+// Bound by memory: 2048 bf16 rows of 5120 take 17.7-18.1 us (42 MB read, 32 written: 4.1 TB/s), 777 rows of an fp32
+// partial on an fp32 stream 13.3 (32 and 20 MB), one row 3.9, of which nearly all is the launch.
 #include <algorithm>
 
 #include "../../include/qwen_mlp.h"

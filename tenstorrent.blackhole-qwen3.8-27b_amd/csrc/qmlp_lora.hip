@@ -15,7 +15,7 @@ namespace qmlp {
 // One workgroup: counts the tokens of each adapter (ids outside [0, adapters) count as none), lays the
 // groups out one after the other, those without an adapter last, and writes tiles and order.  The order inside a
 // group is not fixed; no result depends on it.  Once a batch: its tokens' plan serves every projection of
-// every layer.
+// every layer (4.5 us for 2048 tokens of four adapters, bound by the barriers of its scan).
 constexpr int kPlanThreads = 1024;
 __global__ __launch_bounds__(kPlanThreads) void lora_plan_kernel(const int* __restrict__ ids, int M, int adapters,
                                                                 int* __restrict__ plan, int max_tiles) {
@@ -103,7 +103,9 @@ __device__ __forceinline__ f32x4 lora_product(u32x4 a, u32x4 b, f32x4 c) {
 // every adapter, which its L2 holds.  The waves share the piece's K-steps of 32 out in turn, two neighbouring ones
 // (a line of a 16-bit row) at a time, and add their sums up in a fixed order through LDS.  Rows of x come in by
 // whole lines, 8 lanes to a row, and turn through LDS into operands: read as the operands lie, one row a lane,
-// every lane of a load is an access of its own, and those bounded the kernel (27000 of a CU for 2048 x 17408).
+// every lane of a load is an access of its own, and those bounded the kernel (27000 of a CU for 2048 x 17408).  It
+// takes 22 us there with rank 64: 71 MB of x and, from the L2s, 143 MB of A, which each 32 tokens read again,
+// 9.7 TB/s into the CUs.  Loads of two and three steps under way instead of one change nothing (23.2 and 23.1 us).
 // TU: units of 16 tokens of a tile; RU: rank units at most.
 template <int TU, int RU>
 constexpr int kDownWaves = TU == 1 && RU <= 4 ? 16 : 8;  // 128 ranks take the registers of two waves
@@ -230,7 +232,8 @@ __global__ __launch_bounds__((kDownWaves<TU, RU> * 64), 1) void lora_down_kernel
 // One workgroup of 8 waves per (16 tokens of a tile, run of feature blocks).  It adds the pieces of t up, scales
 // them and splits each fp32 sum into three 16-bit numbers whose sum it is but for 2^-24 of it (bf16), or of the
 // token's largest (fp16: over a power of two that brings the largest near the type's), so the products keep
-// fp32's accuracy; they are laid out in LDS as the products' operands, 32 ranks' parts of one order each.
+// fp32's accuracy; they are laid out in LDS as the products' operands, 32 ranks' parts of one order each.  Bound by
+// memory: 16.7 us for 2048 tokens x 5120 with a bf16 base and rank 64, 70 MB read and written, 4.2 TB/s.
 // DOWN: rank units that a workgroup (of up to 16 waves) makes t of by itself, 0 where lora_down_kernel did: one launch
 // instead of two where that reads little.
 constexpr int kUpParts = 3 * 1024;  // bytes of 32 ranks of 16 tokens
@@ -527,8 +530,9 @@ template <bool F16, bool WHOLE, int BASE, int DOWN>
 static int launch_up(const LoraArgs& a, int max_tiles, int pieces, int num_cus, hipStream_t s) {
   const int blocks = up_div(a.N, 64), tile_units = lora_tile(a.M) / 16;
   const int tiles = std::max(1, std::min(max_tiles * tile_units / 2, up_div(a.M, 16)));
-  // about a workgroup a CU, as far as each wave has a block: 44.1 us at 2048 tokens of 17408 -> 5120 and rank 64,
-  // 48.9 with two (each adds the pieces up again), 48.4 and 45.8 in workgroups of four waves
+  // about a workgroup a CU, as far as each wave has a block: when the two launches took 44.1 us at 2048 tokens of
+  // 17408 -> 5120 and rank 64 (39 now), two workgroups took 48.9 (each adds the pieces up again), one and two of four
+  // waves 48.4 and 45.8
   const int slots = DOWN && max_tiles >= 8 ? up_div(max_tiles, 8) * 8 : max_tiles * tile_units;
   const int most = std::max(1, DOWN ? std::min(up_div(blocks, 4), num_cus / slots)
                                     : std::min(up_div(blocks, kUpWaves<0>), up_div(num_cus, tiles)));

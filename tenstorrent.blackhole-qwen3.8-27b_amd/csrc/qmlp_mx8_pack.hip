@@ -6,7 +6,8 @@ namespace qmlp {
 
 // Two neighbouring lanes own a 32-value block, 16 values each.  A wave covers 8 rows x 4 blocks, so a read
 // touches 256 contiguous bytes of a row (16-bit values) and a write 128 contiguous bytes of a plane; a
-// workgroup of four waves covers 16 rows x 256 K, R times (R * 16 rows).
+// workgroup of four waves covers 16 rows x 256 K, R times (R * 16 rows).  Bound by memory: 20-22 us for 2048 x 17408
+// bf16 values (71 MB in, 37 out, 5.1 TB/s, which is the rate of a large copy), 7 for 777 x 5120 fp16, 3-4 for 16.
 constexpr int kQ8Threads = 256;
 constexpr int kQ8Rows = 16;
 

@@ -476,7 +476,11 @@ static int launch_height(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
 }
 
 // 8-bit activations: two heights, as far as LDS goes; the higher one in waves of 128 features x 32 tokens, which make
-// half the digits of 64 x 64 for as many reads from LDS.
+// half the digits of 64 x 64 for as many reads from LDS.  2048 tokens of 17408 -> 5120 take 177-180 us (2.03-2.06
+// PFLOP/s, 65 % of what two digits' products reach from registers alone) with the matrix cores 57 % busy at 1.70 GHz,
+// 777 of the pair 5120 -> 17408 151-155.  Four waves of 256 x 32, with two thirds of the vector instructions: 182 and
+// 157 (52 % busy at 1.84 GHz).  Digits made a dword at a time beside six groups of products: 177 and 152.  Tiles in
+// bands of eight token blocks and pieces by K, which read 289 MB from behind the L2s instead of 503: no difference.
 template <int MODE>
 static int launch_height8(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
   constexpr int NMAT = MODE == kMxRowsOut ? 1 : 2;
