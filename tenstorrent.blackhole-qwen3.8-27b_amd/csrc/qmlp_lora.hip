@@ -105,7 +105,9 @@ __device__ __forceinline__ f32x4 lora_product(u32x4 a, u32x4 b, f32x4 c) {
 // whole lines, 8 lanes to a row, and turn through LDS into operands: read as the operands lie, one row a lane,
 // every lane of a load is an access of its own, and those bounded the kernel (27000 of a CU for 2048 x 17408).  It
 // takes 22 us there with rank 64: 71 MB of x and, from the L2s, 143 MB of A, which each 32 tokens read again,
-// 9.7 TB/s into the CUs.  Loads of two and three steps under way instead of one change nothing (23.2 and 23.1 us).
+// 9.7 TB/s into the CUs.  Loads of two and three steps under way instead of one change nothing (23.2 and 23.1 us), nor
+// do tiles of 64 tokens, which read A half as often (both launches 33.8 us for 32.6 there, 62.7 for 68.0 at 4096
+// tokens, 18.3 for 16.9 at 777 and rank 16).
 // TU: units of 16 tokens of a tile; RU: rank units at most.
 template <int TU, int RU>
 constexpr int kDownWaves = TU == 1 && RU <= 4 ? 16 : 8;  // 128 ranks take the registers of two waves
