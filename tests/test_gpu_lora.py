@@ -155,10 +155,14 @@ def test_small_and_large_fp16_sums(pkg, cuda, scale):
     assert (np.abs(_np(got) - y) <= err).all()
 
 
-def test_plan_groups_every_token_once(pkg, cuda):
+@pytest.mark.parametrize("run", [0, 1, 63, 64, 100, 700, 65536])
+def test_plan_groups_every_token_once(pkg, cuda, run):
+    """Tokens in any order (0) and in runs of one adapter."""
     for M, L in ((1, 1), (16, 3), (64, 1024), (65, 1), (700, 37), (65536, 1024)):
         g = torch.Generator().manual_seed(M)
         ids = torch.randint(-2, L + 2, (M,), generator=g, dtype=torch.int32)
+        if run:
+            ids = ids.repeat_interleave(run)[:M].contiguous()
         plan = pkg.lora_plan(ids.to(cuda), L)
         w = plan.buf.cpu().numpy()
         T = 16 if M <= 64 else 32
