@@ -69,7 +69,8 @@ __global__ __launch_bounds__(kPlanThreads) void lora_plan_kernel(const int* __re
   __syncthreads();
   const int rows = s_scan[tid] - c0 - c1;
   int* tile = plan + 4;
-  for (int t = tid; t < s_tiles[kPlanThreads - 1]; t += kPlanThreads) {
+  const int tiles = s_tiles[kPlanThreads - 1];
+  for (int t = tid; t < tiles; t += kPlanThreads) {
     int lo = 0, hi = adapters / 2;  // the pair of slots that tile t belongs to
     while (lo < hi) {
       const int mid = (lo + hi) / 2;
@@ -90,7 +91,7 @@ __global__ __launch_bounds__(kPlanThreads) void lora_plan_kernel(const int* __re
     plan[0] = kLoraMagic;
     plan[1] = M;
     plan[2] = adapters;
-    plan[3] = s_tiles[tid];
+    plan[3] = tiles;
   }
   __syncthreads();
   s_count[2 * tid] = rows;  // now the next place of each group
