@@ -165,7 +165,8 @@ __global__ __launch_bounds__(1024) void add_norm_kernel(AddNorm a) {
 }
 
 // Longer rows: 16 values ("a chunk") a thread at a time; the sums are read again from where they were stored (by the
-// same thread).
+// same thread): 64.7 us for 2048 bf16 rows of 17408 (3.9 TB/s without what is read again), 50.0 for rows of 16384 in
+// the kernel above.
 template <int XT, int RT>
 __global__ __launch_bounds__(1024) void add_norm_long_kernel(AddNorm a) {
   __shared__ float s_sum[16];
