@@ -77,13 +77,25 @@ def _units(ranks, size):
     return units, [sum(units[:i]) for i in range(len(units))]
 
 
+def _scale_bits(scale, i):
+    """The bits of adapter ``i``'s scale in fp32, where it has to be a finite number."""
+    try:
+        value = float(scale)
+        packed = struct.pack("<f", value)
+    except OverflowError:  # an integer beyond any float; a finite number beyond fp32
+        value = float("inf")
+    if not abs(value) < float("inf"):
+        raise ValueError(f"adapter {i}: the scale must be finite in fp32, got {scale}")
+    return struct.unpack("<i", packed)[0]
+
+
 def pack_lora(adapters, stream=None):
     """``[(a [rank, K], b [N, rank], scale), ...]`` (GPU tensors, a number) -> ``LoraStack``.  ``scale`` is what the
-    adapter's product is multiplied by (``alpha / rank`` as a rule)."""
+    adapter's product is multiplied by (``alpha / rank`` as a rule), rounded to fp32."""
     adapters = list(adapters)
     if not 1 <= len(adapters) <= MAX_ADAPTERS:
         raise ValueError(f"need 1 to {MAX_ADAPTERS} adapters, got {len(adapters)}")
-    first = adapters[0][0]
+    first, bits = adapters[0][0], []
     for i, (a, b, scale) in enumerate(adapters):
         for name, t in (("a", a), ("b", b)):
             _check_device_tensor(t, f"adapter {i}: {name}")
@@ -101,8 +113,7 @@ def pack_lora(adapters, stream=None):
                              f"{tuple(first.shape)} and {tuple(adapters[0][1].shape)}")
         if K == 0 or K % 32 or b.shape[0] == 0:
             raise ValueError(f"a must have a multiple of 32 columns and b rows, got {K} and {b.shape[0]}")
-        if not abs(float(scale)) < float("inf"):
-            raise ValueError(f"adapter {i}: the scale must be finite, got {scale}")
+        bits.append(_scale_bits(scale, i))
     N, K = adapters[0][1].shape[0], first.shape[1]
     blocks = -(-N // 64)
     ranks = tuple(a.shape[0] for a, _, _ in adapters)
@@ -119,7 +130,6 @@ def pack_lora(adapters, stream=None):
             wide = wide.reshape(blocks, 4, 16, units32[i], 4, 8).permute(0, 3, 1, 4, 2, 5)
             pb[before32[i]:before32[i] + units32[i]] = wide.reshape(units32[i], -1)
         pa = pa.reshape(sum(units), 16, K // 32, 4, 8).permute(0, 2, 3, 1, 4).contiguous()
-        bits = [struct.unpack("<i", struct.pack("<f", float(s)))[0] for _, _, s in adapters]
         meta = torch.tensor(list(zip(ranks, before, bits, before32)), dtype=torch.int32).to(first.device)
     return LoraStack(pa, pb, meta, ranks, max(ranks), len(ranks), N, K)
 

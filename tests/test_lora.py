@@ -78,3 +78,35 @@ def test_python_refusals_need_no_gpu(pkg):
         pkg.lora_plan(torch.zeros(3, dtype=torch.int32), 1)
     with pytest.raises(ValueError, match="LoraStack"):
         pkg.lora_linear(a, None, None)
+
+
+@pytest.fixture
+def cpu_pack(pkg, monkeypatch):
+    """``pack_lora`` without its test for GPU tensors: all it does besides is torch's own operations."""
+    import contextlib
+
+    from qwen_mlp_amd import _lib, lora
+
+    monkeypatch.setattr(lora, "_check_device_tensor", lambda t, name: None)
+    monkeypatch.setattr(_lib, "on_device", lambda device, stream=None: contextlib.nullcontext())
+    return pkg.pack_lora
+
+
+@pytest.mark.parametrize("scale", [float("inf"), float("-inf"), float("nan"), 1e39, -1e39, 2.0 ** 128 - 2.0 ** 103,
+                                   pytest.param(10 ** 400, id="10**400")])
+def test_scales_that_fp32_does_not_hold_are_refused(cpu_pack, scale):
+    """The scale is kept in fp32: what is not a finite number there (from 2^128 - 2^103 on, half a step beyond the
+    largest, a number becomes an infinity) is refused like any other bad argument."""
+    a, b = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(8, 4, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="adapter 1: the scale must be finite"):
+        cpu_pack([(a, b, 1.0), (a, b, scale)])
+
+
+def test_scales_are_rounded_to_fp32(cpu_pack):
+    a, b = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(8, 4, dtype=torch.bfloat16)
+    most = torch.finfo(torch.float32).max
+    scales = [0.1, most, -most, 2.0 ** 128 - 2.0 ** 103 - 2.0 ** 76, 2.0 ** -149, 0.0, 7, torch.tensor(0.3)]
+    meta = cpu_pack([(a, b, s) for s in scales]).meta
+    got = meta[:, 2].contiguous().view(torch.float32)
+    assert torch.equal(got, torch.tensor([float(s) for s in scales], dtype=torch.float64).float())
+    assert torch.isfinite(got).all()
