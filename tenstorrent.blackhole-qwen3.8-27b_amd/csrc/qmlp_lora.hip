@@ -422,7 +422,10 @@ __global__ __launch_bounds__(kUpWaves<DOWN> * 64) void lora_up_kernel(LoraArgs p
         float rest = v[i / 4][i % 4] * inv;
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
-          const uint32_t b = lora_round<F16>(rest);
+          uint32_t b = lora_round<F16>(rest);
+          // bf16: the last 2^-9 of fp32's range round to an infinity, whose rest is none; the number before it, then
+          if constexpr (!F16)
+            if (k == 0 && (b & 0x7fffu) == 0x7f80u && __builtin_isfinite(rest)) --b;
           rest = __builtin_isfinite(rest) ? rest - lora_value<F16>(b) : 0.f;
           part[k][i / 2] = i % 2 ? part[k][i / 2] | b << 16 : b;
         }

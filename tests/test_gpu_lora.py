@@ -194,3 +194,29 @@ def test_offsets_beyond_32_bits(pkg, cuda):
     for rows in (slice(0, 70), slice(M - 70, M)):
         few = pkg.lora_linear(x[rows].contiguous(), stack, pkg.lora_plan(ids[rows].contiguous(), 2))
         assert torch.equal(y[rows], few) and few.abs().max() > 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M", [6, 70])
+def test_sums_next_to_the_largest_number(pkg, cuda, M, dtype):
+    """Scaled sums up to fp32's largest number, where a rounding to bf16 (from 2^128 - 2^119 on) would be an infinity,
+    give finite outputs.  t is one value of x in its first rank, so that the scaled sum is the scale with a sign."""
+    K, N, most = 32, 24, float(np.finfo(np.float32).max)
+    edge = 2.0 ** 128 - 2.0 ** 119  # half way from bf16's largest number to the infinity
+    scales = [edge * (1 - 2.0 ** -24), edge, edge * (1 + 2.0 ** -23), most, -most, 3.4e38]
+    g = torch.Generator().manual_seed(M)
+    adapters = []
+    for s in scales:
+        a = torch.zeros(3, K)
+        a[0, 0], a[1, 1] = 1.0, 2.0 ** -14
+        adapters.append((a.to(dtype), (torch.rand(N, 3, generator=g) * 1.5 - 0.75).to(dtype), s))
+    x = torch.ones(M, K)
+    x[::2] = -1.0
+    x = x.to(dtype)
+    ids = np.arange(M) % len(scales)
+    y, err = _oracle(_np(x), adapters, ids)
+    stack = pkg.pack_lora([(a.to(cuda), b.to(cuda), s) for a, b, s in adapters])
+    got = pkg.lora_linear(x.to(cuda), stack, pkg.lora_plan(torch.tensor(ids, dtype=torch.int32, device=cuda), len(scales)),
+                          out_dtype=torch.float32)
+    assert np.isfinite(y).all() and torch.isfinite(got).all()
+    assert (np.abs(_np(got) - y) <= err).all()
