@@ -403,6 +403,10 @@ int qmlp_mx_plan(int M, int N, int K, int nmat, int num_cus, int* out5);
  * tokens. */
 int qmlp_w4a8_plan(int M, int N, int K, int nmat, int num_cus, int* out5);
 
+/* How qmlp_lora_linear runs for these sizes (host only; adapters: those loaded): out5 = {launches; units of 16 tokens of
+ * a tile; the most units of 16 ranks that the kernels are made for; pieces of the K range; the most that K would give}. */
+int qmlp_lora_path(int M, int N, int K, int adapters, int max_rank, int num_cus, int* out5);
+
 #ifdef __cplusplus
 }
 #endif

@@ -75,6 +75,7 @@ SIGNATURES = {
     "qmlp_lora_plan": (_I, [_P, _I, _I, _P, _SZ, _P]),
     "qmlp_lora_workspace_bytes": (_SZ, [_I, _I, _I]),
     "qmlp_lora_linear": (_I, [_P, _I, _L, _P, _P, _P, _I, _I, _P, _P, _P, _P, _SZ, _I, _I, _I, _I, _P]),
+    "qmlp_lora_path": (_I, [_I, _I, _I, _I, _I, _I, ctypes.POINTER(ctypes.c_int)]),
     "qmlp_w4a8_plan": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(ctypes.c_int)]),
 }
 

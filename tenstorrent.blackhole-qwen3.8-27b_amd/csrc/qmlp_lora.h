@@ -49,8 +49,13 @@ struct LoraArgs {
   int f16, out_f32, base_f32;
 };
 
-// The K range is cut into this many pieces, a workgroup each.
-int lora_pieces(int M, int K, int adapters, int num_cus);
+// How a call runs for its sizes: whether in one launch, units of 16 tokens of a tile, the most units of 16 ranks that the
+// kernels are made for, and (two launches) the pieces of the K range, a workgroup each, of the most that K would give.
+struct LoraPath {
+  bool one;
+  int tile_units, rank_units, pieces, most_pieces;
+};
+LoraPath lora_path(int M, int K, int adapters, int max_rank, int num_cus);
 size_t lora_parts_bytes(int M, int K, int max_rank);
 int launch_lora_plan(const int* ids, int M, int adapters, int* plan, hipStream_t s);
 int launch_lora(const LoraArgs& a, int num_cus, hipStream_t s);

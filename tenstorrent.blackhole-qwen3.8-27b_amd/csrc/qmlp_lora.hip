@@ -536,7 +536,7 @@ static int pieces_of(int K) {
 }
 // Half as many as long as the card is full twice over all the same: 2048 tokens of 17408 and rank 64, 73 tiles at
 // most, take 22.8 us in four pieces, 25.0 in eight and 31.9 in 16 (and 31.8 in six, which no XCD has to itself).
-int lora_pieces(int M, int K, int adapters, int num_cus) {
+static int lora_pieces(int M, int K, int adapters, int num_cus) {
   int pieces = lora_tile(M) == 16 ? pieces_of<1>(K) : pieces_of<2>(K);
   while (pieces > 1 && pieces * lora_max_tiles(M, adapters) >= 2 * num_cus) pieces /= 2;
   return pieces;
@@ -598,23 +598,29 @@ static int launch_up_rows(const LoraArgs& a, int max_tiles, int pieces, int num_
 // 5120 -> 5120 and rank 16, 174 KB: 7.3 / 8.1 (10.3 / 13.0); 16 tokens of 16 adapters of 5120 -> 17408 and rank 32, 492
 // KB: 12.4 / 13.9 (11.7 / 13.2), of one 10.1 / 9.0 (10.3 / 13.1); 2048 -> 2048 and rank 64, 266 KB: 10.7 / 10.0; one
 // token of 17408 -> 5120 and rank 16, 592 KB: 11.5 / 8.4 (11.0 / 13.1); rank 64 of 5120, 666 KB: 15.5 / 10.0.
-static bool lora_one_launch(const LoraArgs& a) {
-  const int ranks = padded_rank(a.max_rank);
-  return lora_tile(a.M) == 16 && (size_t)(ranks + std::min(a.M, 16)) * a.K * 2 <= (ranks <= 32 ? 500000 : 167000);
+static bool lora_one_launch(int M, int K, int max_rank) {
+  const int ranks = padded_rank(max_rank);
+  return lora_tile(M) == 16 && (size_t)(ranks + std::min(M, 16)) * K * 2 <= (ranks <= 32 ? 500000 : 167000);
+}
+
+LoraPath lora_path(int M, int K, int adapters, int max_rank, int num_cus) {
+  const int units = padded_rank(max_rank) / 16, tile_units = lora_tile(M) / 16;
+  return LoraPath{lora_one_launch(M, K, max_rank), tile_units, units <= 1 ? 1 : units <= 2 ? 2 : units <= 4 ? 4 : 8,
+                  lora_pieces(M, K, adapters, num_cus), tile_units == 1 ? pieces_of<1>(K) : pieces_of<2>(K)};
 }
 
 template <bool F16, int TU>
 static int launch_tokens(const LoraArgs& a, int num_cus, hipStream_t s) {
-  const int max_tiles = lora_max_tiles(a.M, a.adapters), pieces = lora_pieces(a.M, a.K, a.adapters, num_cus);
-  const int units = padded_rank(a.max_rank) / 16;
-  if (TU == 1 && lora_one_launch(a))
-    return units <= 1   ? launch_up_rows<F16, 1>(a, max_tiles, pieces, num_cus, s)
-           : units <= 2 ? launch_up_rows<F16, 2>(a, max_tiles, pieces, num_cus, s)
-           : units <= 4 ? launch_up_rows<F16, 4>(a, max_tiles, pieces, num_cus, s)
+  const LoraPath path = lora_path(a.M, a.K, a.adapters, a.max_rank, num_cus);
+  const int max_tiles = lora_max_tiles(a.M, a.adapters), pieces = path.pieces, units = path.rank_units;
+  if (TU == 1 && path.one)
+    return units == 1   ? launch_up_rows<F16, 1>(a, max_tiles, pieces, num_cus, s)
+           : units == 2 ? launch_up_rows<F16, 2>(a, max_tiles, pieces, num_cus, s)
+           : units == 4 ? launch_up_rows<F16, 4>(a, max_tiles, pieces, num_cus, s)
                         : launch_up_rows<F16, 8>(a, max_tiles, pieces, num_cus, s);
-  const int rc = units <= 1   ? launch_down<F16, TU, 1>(a, max_tiles, pieces, s)
-                 : units <= 2 ? launch_down<F16, TU, 2>(a, max_tiles, pieces, s)
-                 : units <= 4 ? launch_down<F16, TU, 4>(a, max_tiles, pieces, s)
+  const int rc = units == 1   ? launch_down<F16, TU, 1>(a, max_tiles, pieces, s)
+                 : units == 2 ? launch_down<F16, TU, 2>(a, max_tiles, pieces, s)
+                 : units == 4 ? launch_down<F16, TU, 4>(a, max_tiles, pieces, s)
                               : launch_down<F16, TU, 8>(a, max_tiles, pieces, s);
   if (rc) return rc;
   return launch_up_rows<F16, 0>(a, max_tiles, pieces, num_cus, s);

@@ -44,6 +44,21 @@ size_t qmlp_lora_workspace_bytes(int M, int K, int max_rank) {
   return tokens_ok(M) && sizes_ok(1, K) && rank_ok(max_rank) ? lora_parts_bytes(M, K, max_rank) : 0;
 }
 
+int qmlp_lora_path(int M, int N, int K, int adapters, int max_rank, int num_cus, int* out5) {
+  const char* fn = "qmlp_lora_path";
+  if (!out5) return set_error(QMLP_E_NULL, "%s: null pointer", fn);
+  if (!tokens_ok(M) || !sizes_ok(N, K) || !adapters_ok(adapters) || !rank_ok(max_rank) || num_cus < 1)
+    return set_error(QMLP_E_SHAPE, "%s: M=%d N=%d K=%d, %d adapters, rank %d on %d CUs", fn, M, N, K, adapters, max_rank,
+                     num_cus);
+  const LoraPath p = lora_path(M, K, adapters, max_rank, num_cus);
+  out5[0] = p.one ? 1 : 2;
+  out5[1] = p.tile_units;
+  out5[2] = p.rank_units;
+  out5[3] = p.one ? 1 : p.pieces;
+  out5[4] = p.one ? 1 : p.most_pieces;
+  return 0;
+}
+
 int qmlp_lora_linear(const void* x, int x_type, int64_t x_stride, const void* a, const void* b, const void* meta,
                      int adapters, int max_rank, const void* plan, const void* base, void* out, void* ws,
                      size_t ws_bytes, int M, int N, int K, int flags, qmlp_stream_t stream) {

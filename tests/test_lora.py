@@ -13,6 +13,19 @@ def P(at):
 
 X, A, B, META, PLAN, BASE, OUT, WS = (P(1 << k) for k in range(32, 40))
 
+# (ids, ranks, N, K): sizes that together take every kernel that lora_linear launches, with A x in one piece of K, in
+# several, and in fewer than K has because many adapters are loaded
+FOUR = [i // 130 for i in range(520)]  # four requests
+PATHS = [
+    ([0, 1, 2], [128, 70, 16], 136, 5120), ([0] * 40, [32], 72, 8192), ([i % 3 for i in range(33)], [64, 40, 1], 65, 2048),
+    (list(range(64)), [16] * 64, 33, 8192), ([5, 0], [8] * 6, 40, 17408), ([1, 1, -1, 0], [1, 9], 23, 512),
+    ([4, 0], [8] * 5, 40, 5120), ([0, 1], [30, 20], 24, 2048), ([0, 1, 0], [30, 20], 25, 1024), ([2, 1, 0], [64, 50, 3], 48, 512),
+    ([0] * 9, [40], 49, 544), ([1, 0, 0], [128, 65], 16, 288), ([0] * 64, [96], 17, 320),
+    ([i % 2 for i in range(65)], [16, 5], 64, 1056), ([i % 2 for i in range(100)], [128, 5], 39, 2048),
+    (FOUR, [17] * 60, 40, 4096), (FOUR, [64] * 4, 72, 4096), (FOUR, [1 + i % 16 for i in range(120)], 41, 4096),
+    (FOUR, [33] * 300, 24, 4096), (FOUR, [2] * 109 + [128], 40, 2560),
+]
+
 
 def test_sizes(pkg):
     lib = pkg.lib()
@@ -65,6 +78,46 @@ def test_linear_refusals(pkg):
                {"out": META}, {"out": A}, {"out": B}, {"ws": X}, {"ws": PLAN}, {"ws": META}, {"ws": A}, {"ws": B}, {"ws": OUT},
                {"ws": BASE, "base": BASE}):
         assert f(**kw) == E_SHAPE, kw
+
+
+def _path(pkg, M, N, K, L, rank, cus=256):
+    out = (ctypes.c_int * 5)()
+    assert pkg.lib().qmlp_lora_path(M, N, K, L, rank, cus, out) == 0
+    return tuple(out)
+
+
+def test_sizes_reach_every_kernel(pkg):
+    """What the tests on the GPU run, both types each: every kernel of one launch and of two, with rows that a vector
+    store fits and others, with K in one piece, in several, and in fewer because many adapters are loaded."""
+    one, down, up, pieces = set(), set(), set(), set()
+    for ids, ranks, N, K in PATHS:
+        launches, tile, units, n, most = _path(pkg, len(ids), N, K, len(ranks), max(ranks))
+        if launches == 1:
+            one.add((units, N % 8 == 0))
+        else:
+            down.add((tile, units))
+            up.add(N % 8 == 0)
+            pieces.add((tile, n, most))
+    assert one == {(u, w) for u in (1, 2, 4, 8) for w in (True, False)}
+    assert down == {(t, u) for t in (1, 2) for u in (1, 2, 4, 8)} and up == {True, False}
+    assert {(2, n, 8) for n in (8, 4, 2, 1)} <= pieces and {(1, 8, 8), (1, 4, 8)} <= pieces  # from eight pieces on
+    assert any(most % 2 and n == most for _, n, most in pieces) and any(most % 2 and n < most for _, n, most in pieces)
+
+
+def test_paths_are_within_the_kernels_limits(pkg):
+    for K in (32, 512, 544, 5120, 17408, 1 << 20):
+        for rank in (1, 16, 17, 33, 65, 128):
+            for M in (1, 16, 17, 64, 65, 520, 2048, 65536):
+                for L in (1, 60, 300, 1024):
+                    launches, tile, units, n, most = _path(pkg, M, 64, K, L, rank)
+                    assert tile == (1 if M <= 64 else 2) and 16 * units >= rank and units <= max(1, rank // 8)
+                    assert 1 <= n <= most <= 8 and (launches == 2 or (tile == 1 and n == 1))
+                    assert launches == 1 or n * -(-rank // 16) * 16 * 4 * M <= pkg.lib().qmlp_lora_workspace_bytes(M, K, rank)
+    out = (ctypes.c_int * 5)()
+    for bad in ((0, 64, 64, 1, 1, 256), (65537, 64, 64, 1, 1, 256), (1, 0, 64, 1, 1, 256), (1, 64, 48, 1, 1, 256),
+                (1, 64, 64, 0, 1, 256), (1, 64, 64, 1025, 1, 256), (1, 64, 64, 1, 129, 256), (1, 64, 64, 1, 1, 0)):
+        assert pkg.lib().qmlp_lora_path(*bad, out) == E_SHAPE
+    assert pkg.lib().qmlp_lora_path(1, 64, 64, 1, 1, 256, None) == E_NULL
 
 
 def test_python_refusals_need_no_gpu(pkg):
