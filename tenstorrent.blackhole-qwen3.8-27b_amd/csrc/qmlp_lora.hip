@@ -417,16 +417,16 @@ __global__ __launch_bounds__(kUpWaves<DOWN> * 64) void lora_up_kernel(LoraArgs p
       float inv = 1.f;
       if constexpr (F16) inv = 1.0f / s_scale[row];  // a power of two: exact
       u32x4 part[3];
+      // The first part is the nearest number of the adapters' type: of sums from 2^128 - 2^119 on bf16's largest, as
+      // the nearest is an infinity and the rest then no number.  What is not finite itself goes into the second part.
+      constexpr float kMost = F16 ? 65504.0f : 0x1.fep127f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float rest = v[i / 4][i % 4] * inv;
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
-          uint32_t b = lora_round<F16>(rest);
-          // bf16: the last 2^-9 of fp32's range round to an infinity, whose rest is none; the number before it, then
-          if constexpr (!F16)
-            if (k == 0 && (b & 0x7fffu) == 0x7f80u && __builtin_isfinite(rest)) --b;
-          rest = __builtin_isfinite(rest) ? rest - lora_value<F16>(b) : 0.f;
+          const uint32_t b = lora_round<F16>(k == 0 ? __builtin_amdgcn_fmed3f(rest, -kMost, kMost) : rest);
+          rest = k == 1 && !__builtin_isfinite(rest) ? 0.f : rest - lora_value<F16>(b);
           part[k][i / 2] = i % 2 ? part[k][i / 2] | b << 16 : b;
         }
       }
