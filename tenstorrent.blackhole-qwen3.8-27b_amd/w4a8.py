@@ -253,7 +253,8 @@ def w4a8_mlp(x, weights, residual=None, out=None, out_dtype=None, adapters=None,
     ``x`` as in ``w4a8_linear``, ``residual`` / ``out`` / ``out_dtype`` as its.  ``adapters`` (``MLPAdapters``) and the
     batch's ``plan``: low-rank adapters beside the projections; those of gate and up read ``x`` as rows (``rows`` where
     ``x`` is an ``Mx8Tensor``), those of down the bf16 rows between the projections, which then are what the down
-    projection quantises.
+    projection quantises, for every token of the call: one without an adapter gets 8-bit values rounded twice, which
+    differ by at most a step from those of a call without adapters of down, quantised from fp32.
     """
     if weights.fmt != "mxfp4":
         raise ValueError(f"8-bit activations need mxfp4 weights, got {weights.fmt}")

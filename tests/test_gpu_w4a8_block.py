@@ -354,3 +354,22 @@ def test_rows_behind_the_last_one_stay(pkg, cuda):
         wide = torch.full((M + 8, 96 + 32), 3.0, dtype=torch.bfloat16, device=cuda)
         pkg.add_rmsnorm(x, x.clone(), torch.zeros(96, dtype=torch.bfloat16, device=cuda), out=wide[:M, :96])
         assert (wide[M:] == 3.0).all() and (wide[:, 96:] == 3.0).all()
+
+
+@pytest.mark.parametrize("M", [1, 30, 130])
+def test_tokens_without_an_adapter_beside_down_adapters(pkg, cuda, M):
+    """With adapters of the down projection in a call every token's h is rounded to bf16 before it is quantised.  A token
+    without one gets what the calls by themselves make of those rows, and 8-bit values at most one step (of the coarser
+    of both scales) from those quantised from fp32: bf16 moves a value by at most a quarter of a step, rounding by half."""
+    mlp = pkg.Qwen36MLP(cuda, _state(cuda, 7), weight_format="mxfp4", activation_format="mxint8", max_tokens=M)
+    _, ad = _adapters(pkg, cuda, 2, which=("w2",))
+    g = torch.Generator().manual_seed(M)
+    x, res = torch.randn(M, H, generator=g).bfloat16().to(cuda), torch.randn(M, H, generator=g).to(cuda)
+    plan = pkg.lora_plan(torch.full((M,), -1, dtype=torch.int32, device=cuda), 3)
+    got = mlp.forward(x, residual=res, out_dtype=torch.float32, adapters=ad, plan=plan)
+    rows = pkg.w4a8_swiglu(x, mlp.weights.w1, mlp.weights.w3)
+    assert torch.equal(got, pkg.w4a8_linear(rows, mlp.weights.w2, residual=res, out_dtype=torch.float32))
+    once, twice = pkg.w4a8_swiglu(x, mlp.weights.w1, mlp.weights.w3, quantize=True), pkg.quantize_mxint8(rows)
+    scale = torch.maximum(*(pkg.unpack_canonical(t)[1] for t in (once, twice))).double()
+    step = torch.exp2(scale - 133).repeat_interleave(32, dim=1)
+    assert ((pkg.dequantize(once).double() - pkg.dequantize(twice).double()).abs() <= step).all()
