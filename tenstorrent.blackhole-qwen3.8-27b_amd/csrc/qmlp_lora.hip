@@ -15,7 +15,8 @@ namespace qmlp {
 // One workgroup: counts the tokens of each adapter (ids outside [0, adapters) count as none), lays the
 // groups out one after the other, those without an adapter last, and writes tiles and order.  The order inside a
 // group is not fixed; no result depends on it.  Once a batch: its tokens' plan serves every projection of
-// every layer.  Bound by its steps' latencies: 4.6 us up to some hundred tokens, 5.5 for 2048, 38 for 65536 (captured).
+// every layer.  Bound by its steps' latencies; captured: 4.1-4.9 us up to 512 tokens, 5.1-6.0 for 2048, and for 65536 36 in
+// any order of eight adapters, 40 of one adapter, 56 in any order of 1024.
 constexpr int kPlanThreads = 1024;
 __global__ __launch_bounds__(kPlanThreads) void lora_plan_kernel(const int* __restrict__ ids, int M, int adapters,
                                                                 int* __restrict__ plan, int max_tiles) {
@@ -30,8 +31,8 @@ __global__ __launch_bounds__(kPlanThreads) void lora_plan_kernel(const int* __re
     return id >= 0 && id < adapters ? id : adapters;
   };
   // The next place of token m's group.  Requests' tokens come in runs, and a wave whose tokens share a group takes
-  // their places at once: 65536 tokens of one adapter take 41 us, 2048 5.6 (with places taken one by one and a group's
-  // tiles written by one thread 193 and 11).
+  // their places at once: with places taken one by one and a group's tiles written by one thread 65536 tokens of one
+  // adapter took 193 us and 2048 11, for 40 and 5.1.
   auto take = [&](int m) {
     const int k = slot(m), first = __builtin_amdgcn_readfirstlane(k);
     if (!__all(k == first)) return atomicAdd(&s_count[k], 1);
@@ -534,8 +535,11 @@ template <int TU>
 static int pieces_of(int K) {
   return std::min(kLoraMaxPieces, up_div(K / 32, 2 * kDownWaves<TU, 1>));
 }
-// Half as many as long as the card is full twice over all the same: 2048 tokens of 17408 and rank 64, 73 tiles at
-// most, take 22.8 us in four pieces, 25.0 in eight and 31.9 in 16 (and 31.8 in six, which no XCD has to itself).
+// Half as many as long as the most tiles that a plan can hold are two workgroups a CU: 2048 tokens of 17408 and rank
+// 64 with eight adapters, 73 tiles at most, take 22.8 us in four pieces, 25.0 in eight and 31.9 in 16 (and 31.8 in six,
+// which no XCD has to itself).  That counts a tile for every adapter that is loaded, used or not, as the host knows no
+// more: four requests there take 33 us (both launches) with 4 to 24 adapters loaded, 41 with 64 (two pieces) and 57-59
+// with 200 to 1024 (one piece, 66 workgroups); 512 tokens 19, 23 and from 512 adapters on 55.
 static int lora_pieces(int M, int K, int adapters, int num_cus) {
   int pieces = lora_tile(M) == 16 ? pieces_of<1>(K) : pieces_of<2>(K);
   while (pieces > 1 && pieces * lora_max_tiles(M, adapters) >= 2 * num_cus) pieces /= 2;
@@ -594,10 +598,15 @@ static int launch_up_rows(const LoraArgs& a, int max_tiles, int pieces, int num_
 }
 
 // Whether t is made by every workgroup that uses it: where that reads at most half a megabyte of A and x, a third of
-// that beyond 32 ranks.  One launch / two, us in a graph (and with the host's time in a loop of calls): one token of
-// 5120 -> 5120 and rank 16, 174 KB: 7.3 / 8.1 (10.3 / 13.0); 16 tokens of 16 adapters of 5120 -> 17408 and rank 32, 492
-// KB: 12.4 / 13.9 (11.7 / 13.2), of one 10.1 / 9.0 (10.3 / 13.1); 2048 -> 2048 and rank 64, 266 KB: 10.7 / 10.0; one
-// token of 17408 -> 5120 and rank 16, 592 KB: 11.5 / 8.4 (11.0 / 13.1); rank 64 of 5120, 666 KB: 15.5 / 10.0.
+// that beyond 32 ranks.  One launch / two, us in a graph (and with the host's time in a loop of calls):
+//   up to 32 ranks: one token of 5120 -> 5120 and rank 16, 174 KB: 6.8 / 7.5 (10.6 / 13.4); 5120 -> 17408 and rank 32,
+//   492 KB: 16 tokens of 16 adapters 12.0 / 13.1 (11.7 / 13.5), of one 8.9 / 8.5 (10.4 / 13.4), of one of 16 loaded 12.1 /
+//   8.7 (12.0 / 13.7), 32 tokens of twelve 11.6 / 11.0 (11.3 / 13.3): near the limit one launch is the host's gain;
+//   one token of 17408 -> 5120 and rank 16, 592 KB: 10.9 / 7.9 (10.9 / 13.8);
+//   rank 64: one token of 1024 -> 5120, 133 KB: 8.9 / 9.5 (10.4 / 13.6), 16 of 16 adapters, 164 KB: 11.9 / 11.2 (11.7 /
+//   13.4); one token of 2048 -> 2048, 266 KB: 10.1 / 9.4 (10.7 / 13.8), of 5120 -> 5120, 666 KB: 14.7 / 9.6 (14.6 / 13.6);
+//   rank 128 would bear a higher limit: one token of 1024 -> 5120, 264 KB: 9.3 / 11.4, 16 of 16 adapters 12.6 / 14.1; of
+//   2048 -> 5120, 528 KB: 11.7 / 11.3.
 static bool lora_one_launch(int M, int K, int max_rank) {
   const int ranks = padded_rank(max_rank);
   return lora_tile(M) == 16 && (size_t)(ranks + std::min(M, 16)) * K * 2 <= (ranks <= 32 ? 500000 : 167000);

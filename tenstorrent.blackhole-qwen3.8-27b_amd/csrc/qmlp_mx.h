@@ -152,7 +152,7 @@ struct MxProduct {
 constexpr size_t kMxPartBytes = 64u << 20;
 constexpr int kMxInside = 4;  // at most this many token rows are quantised inside the streamed product
 bool mx_quantizes_inside(int M, int K, bool a8);
-constexpr int kMxFewTokens = 32;  // up to here every product is streamed
+constexpr int kMxFewTokens = 32;  // up to here no product is tiled: streamed, or (8-bit activations) the few-token kernel's
 
 // How a product runs (mx_plan, qmlp_mx_plan.hip).  Streamed: a workgroup of 32 features x 32 tokens, four
 // waves with one unit of K under way (kMxStream) or two (kMxStreamDeep, one matrix only), or eight with

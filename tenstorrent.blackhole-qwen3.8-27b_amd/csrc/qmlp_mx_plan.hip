@@ -161,7 +161,12 @@ static MxPlan plan_a8(int M, int N, int K, int nmat, int num_cus) {
 // Whether the streamed product quantises unpacked rows by itself, every workgroup all of them, rather than
 // leaving it to a launch in front.  Inside / in front, us: one token 12.1 / 13.6 at 5120 x 17408, 10.7 /
 // 13.6 at 17408 x 5120, 19.6 / 21.4 for two such matrices, 4.1 / 5.5 at 2048 x 2048; two tokens of K = 17408
-// 13.5 / 13.6, three 14.9 / 13.6; four tokens of K = 5120 13.7 / 14.9, for two matrices 21.8 / 21.5.
+// 13.5 / 13.6, three 14.9 / 13.6; four tokens of K = 5120 13.7 / 14.9, for two matrices 21.8 / 21.5.  8-bit activations
+// (the few-token kernel), captured, eight matrices in turn: one token 3.6 / 5.7 at 2048 x 2048, 11.6 / 14.7 at 17408 x
+// 5120 (N x K), 13.2 / 18.4 at 5120 x 17408, 18.9 / 22.8 for two of 17408 x 5120; three tokens of K = 5120 (60 units)
+// 7.1 / 8.3 at N = 5120, 13.8 / 14.1 at 17408, two matrices 20.5 / 21.6; two of K = 8704 (68) 9.4 / 10.9.  Beyond, either
+// may win: four of K = 5120 (80) 7.9 / 8.4, 15.5 / 13.8 and 21.0 / 21.4; of K = 8704 three (102) 10.1 / 10.6, four (136)
+// 11.3 / 10.5.
 bool mx_quantizes_inside(int M, int K, bool a8) { return M <= kMxInside && mx_ksb(K) * M <= (a8 ? 68 : 136); }
 
 }  // namespace qmlp

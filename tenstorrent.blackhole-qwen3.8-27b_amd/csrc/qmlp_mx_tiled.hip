@@ -481,6 +481,8 @@ static int launch_height(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
 // 777 of the pair 5120 -> 17408 151-155.  Four waves of 256 x 32, with two thirds of the vector instructions: 182 and
 // 157 (52 % busy at 1.84 GHz).  Digits made a dword at a time beside six groups of products: 177 and 152.  Tiles in
 // bands of eight token blocks and pieces by K, which read 289 MB from behind the L2s instead of 503: no difference.
+// gate_add and up_add cost the pair's 369 us at 2048 tokens 49 (143 MB each, read in the epilogue; 5.8 TB/s), at 777 13 of 157;
+// a packed output or rows take the same time.
 template <int MODE>
 static int launch_height8(const MxProduct& p, const MxPlan& pl, hipStream_t s) {
   constexpr int NMAT = MODE == kMxRowsOut ? 1 : 2;
