@@ -539,7 +539,7 @@ static int pieces_of(int K) {
 // 64 with eight adapters, 73 tiles at most, take 22.8 us in four pieces, 25.0 in eight and 31.9 in 16 (and 31.8 in six,
 // which no XCD has to itself).  That counts a tile for every adapter that is loaded, used or not, as the host knows no
 // more: four requests there take 33 us (both launches) with 4 to 24 adapters loaded, 41 with 64 (two pieces) and 57-59
-// with 200 to 1024 (one piece, 66 workgroups); 512 tokens 19, 23 and from 512 adapters on 55.
+// with 200 to 1024 (one piece, 64 workgroups); 512 tokens 19, 23 and from 512 adapters on 55.
 static int lora_pieces(int M, int K, int adapters, int num_cus) {
   int pieces = lora_tile(M) == 16 ? pieces_of<1>(K) : pieces_of<2>(K);
   while (pieces > 1 && pieces * lora_max_tiles(M, adapters) >= 2 * num_cus) pieces /= 2;
